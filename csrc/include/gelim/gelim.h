@@ -261,6 +261,57 @@ int gelim_gpu_matmul_f32_ex(const float* dA, int64_t lda, const float* dB, int64
                             float* dC, int64_t ldc, int64_t M, int64_t N, int64_t K,
                             int accumulate, int kernel, void* stream);
 
+/* ---- low-rank adapters beside a shared projection ------------------------
+ * Row t of X (T x K) with the adapter i = index[t]:
+ *   Y_t = X_t W + s_i (X_t A_i) B_i,   W (K x N), A_i (K x r), B_i (r x N)
+ * index NULL: every row has adapter 0; -1: the row has none; any other value
+ * outside [0, n): the row of Y (of dX) is NaN and adds to no gradient.
+ * W, A and B are row-major (trans = 0) or stored transposed (trans = 1: W as
+ * (N, K), A as (n, r, K), B as (n, N, r)); ld* is the distance of two rows as
+ * stored, *_stride the distance of two adapters, all in elements.
+ * The gradient: dX (T x K, NULL: not wanted), dA and dB in the layouts of A
+ * and B without gaps (NULL: not wanted).  No call allocates, synchronises or
+ * keeps anything; the results do not depend on the order of anything's run. */
+enum { GELIM_T_F32 = 0, GELIM_T_BF16 = 1, GELIM_T_F16 = 2 };
+#define GELIM_ADAPTER_MAX_RANK 256
+typedef struct gelim_adapter_args {
+  int64_t dtype, T, K, N, r, n;
+  const void* X;
+  int64_t ldx;
+  const void* W;
+  int64_t ldw, w_trans;
+  const void* A;
+  int64_t a_stride, lda, a_trans;
+  const void* B;
+  int64_t b_stride, ldb, b_trans;
+  const int32_t* index;
+  const float* scale; /* n factors on the device, or NULL: scale_value */
+  double scale_value;
+  void* Y; /* the product; the gradient reads dY in its place */
+  int64_t ldy;
+  void* dX;
+  int64_t lddx;
+  void *dA, *dB;
+  void* ws; /* 16-byte aligned device memory, gelim_adapter_workspace bytes */
+  int64_t ws_bytes;
+} gelim_adapter_args;
+/* sizeof (which = 0) or the offset of T / index / ws_bytes (1 / 2 / 3) */
+int64_t gelim_adapter_args_layout(int32_t which);
+int64_t gelim_adapter_workspace(const gelim_adapter_args* a, int grad);
+int gelim_adapter_matmul(const gelim_adapter_args* a, void* stream);
+int gelim_adapter_matmul_grad(const gelim_adapter_args* a, void* stream);
+
+/* ---- 2-norm over many tensors, and clipping ------------------------------
+ * norm = sqrt(sum of squares of all elements), out = in * min(1, max_norm /
+ * (norm + 1e-6)); max_norm = infinity only measures (in place) or copies.
+ * in / out / sizes / dtypes: host arrays of `count` entries (device pointers,
+ * elements, GELIM_T_*); out[i] is in[i] (in place) or memory that no other
+ * entry uses.  d_norm: one float on the device.  ws: gelim_clip_workspace
+ * bytes, 8-byte aligned. */
+int64_t gelim_clip_workspace(int64_t count);
+int gelim_clip_norm(const void* const* in, void* const* out, const int64_t* sizes, const int8_t* dtypes,
+                    int64_t count, double max_norm, float* d_norm, void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

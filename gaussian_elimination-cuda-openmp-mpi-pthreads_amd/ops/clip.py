@@ -1,0 +1,87 @@
+"""2-norm over many tensors and clipping by it (csrc/hip/clip.hip)."""
+from __future__ import annotations
+
+import math
+from array import array
+from typing import Sequence
+
+import torch
+
+from .. import _native
+from ..utils.tensors import stream_handle
+from .adapter import TYPES
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t fills its memory without gaps, in any order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    size = 1
+    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda d: d[1]):
+        if s != size:
+            return False
+        size *= n
+    return True
+
+
+def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
+                     out: Sequence[torch.Tensor] | None = None) -> torch.Tensor:
+    """Scales all tensors by min(1, max_norm / (norm + 1e-6)), norm the 2-norm of
+    all their elements together, and returns that norm (a float32 scalar on
+    the device, nothing waits for it).
+
+    tensors: float32, bfloat16 and float16 in any mixture, on one device, each
+    without gaps in memory (any order of dimensions); none twice.
+    out: tensors of the same shapes, types and strides that get the scaled
+    copies, the inputs staying as they are; None: in place.
+    max_norm = math.inf only measures.  As the factor comes from the norm, a NaN anywhere
+    makes all of them NaN, and an infinity makes the finite elements zero.
+    Squares and their sum are held in float64, in an order that does not change
+    from run to run.  May be captured into a graph."""
+    tensors = list(tensors)
+    max_norm = float(max_norm)
+    if math.isnan(max_norm) or max_norm < 0:
+        raise ValueError("max_norm must be a number and not negative")
+    if not tensors:
+        raise ValueError("no tensors")
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise ValueError("clip_global_norm needs CUDA tensors")
+    try:
+        types = bytes([TYPES[t.dtype] for t in tensors])
+    except KeyError as e:
+        raise TypeError(f"clip_global_norm takes float32, bfloat16 and float16, not {e.args[0]}") from None
+    if any(t.device != dev for t in tensors):
+        raise ValueError("all tensors must be on one device")
+    if not all(_dense(t) for t in tensors):
+        raise ValueError("a tensor has gaps in memory, or overlaps itself")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError("clip_global_norm is not recorded by autograd: pass the gradients themselves, or call it "
+                         "under torch.no_grad()")
+    src = array("Q", [t.data_ptr() for t in tensors])
+    if out is None:
+        dst = src
+    else:
+        out = list(out)
+        if len(out) != len(tensors):
+            raise ValueError("out must have one tensor per input")
+        for t, o in zip(tensors, out):
+            if o.dtype != t.dtype or o.device != dev or o.shape != t.shape or o.stride() != t.stride():
+                raise ValueError("each out must have the shape, type, strides and device of its input")
+        dst = array("Q", [t.data_ptr() for t in out])
+    sizes = array("q", [t.numel() for t in tensors])
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    lib = _native.lib()
+    ws = torch.empty(lib.gelim_clip_workspace(len(tensors)), dtype=torch.uint8, device=dev)
+
+    def call():
+        _native.check(lib.gelim_clip_norm(src.buffer_info()[0], dst.buffer_info()[0], sizes.buffer_info()[0], types,
+                                          len(tensors), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(),
+                                          stream_handle(dev)), "clip_global_norm")
+
+    if torch.cuda.current_device() == dev.index:
+        call()
+    else:
+        with torch.cuda.device(dev):
+            call()
+    return norm
