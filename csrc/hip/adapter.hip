@@ -4,10 +4,22 @@
 //   D = dY B_i^T (T x r)       dX = dY W^T + s_i D A_i^T
 //   dA_i = s_i sum_t X_t^T D_t     dB_i = s_i sum_t S_t^T dY_t    (rows t of adapter i)
 //
-// Plain form: every sum in fp32 on the vector units, any layout.
+// Names: U (T x C) is the operand with a row per token, F_i the factor that
+// brings it down to r columns, G_i the factor that brings those up again, so
+// that dX is the same product as Y with the operands turned.
+//
+// Few rows (a decoding step): bound by reading W once.  Two launches: partial
+// sums of U W over pieces of C and of U F_i beside them, then their sums and
+// the product with G_i.
+// Many rows: bound by the matrix units.  The rows are ordered by adapter, so a
+// tile of the large product has few adapters; the factors are laid out for the
+// matrix units once per call; U F_i is one pass over U; the large product adds
+// s_i (U F_i) G_i to its accumulators at the end.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstddef>
+#include <type_traits>
 #include <utility>
 
 #include "device_common.h"
@@ -16,155 +28,1273 @@
 namespace gelim {
 namespace {
 
-// a matrix, or one matrix per adapter: element (i, j) of adapter a at p[a * as + i * rs + j * cs]
-template <class T>
+using dev::f4;
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+// A matrix, or one matrix per adapter: element (i, j) of adapter a is p[a as + i rs + j cs]; rs or cs is 1.
 struct View {
-  T* p;
+  const void* p;
   int64_t as, rs, cs;
 };
 
+// 16 bytes of a type, and the matrix instruction over them: lane l of a wave
+// holds row (column) l % 16 and, of a step of kStep values along the sum, the
+// kE ones from (l / 16) kE on.  In D lane l has column l % 16, rows 4 (l / 16) .. + 3.
+template <class T>
+struct Mma;
+template <>
+struct Mma<__bf16> {
+  static constexpr int kE = 8, kStep = 32;
+  using Frag = bf8;
+  static __device__ __forceinline__ f4 mma(Frag a, Frag b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<_Float16> {
+  static constexpr int kE = 8, kStep = 32;
+  using Frag = h8;
+  static __device__ __forceinline__ f4 mma(Frag a, Frag b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<float> {
+  static constexpr int kE = 4, kStep = 16;
+  using Frag = f4;
+  static __device__ __forceinline__ f4 mma(Frag a, Frag b, f4 c) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <class T>
+struct __attribute__((packed, aligned(sizeof(T)))) Unaligned {
+  typename Mma<T>::Frag v;
+};
+// 16 bytes from any element's address; with fewer than kE elements there, zeros in the others' place
+template <class T>
+__device__ __forceinline__ typename Mma<T>::Frag load16(const T* p) {
+  return ((const Unaligned<T>*)p)->v;
+}
+template <class T>
+__device__ __forceinline__ typename Mma<T>::Frag load_part(const T* p, int64_t have) {
+  constexpr int E = Mma<T>::kE;
+  if (have >= E) return load16(p);
+  typename Mma<T>::Frag v = {};
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (e < have) v[e] = p[e];
+  return v;
+}
+
+// kE rows (along the sum) of kE columns each, in registers, turned: out[j] holds column j's kE values.
+// 16-bit types: 32 byte permutes for 64 elements.
+template <class T>
+__device__ __forceinline__ void turn(const typename Mma<T>::Frag (&in)[Mma<T>::kE],
+                                     typename Mma<T>::Frag (&out)[Mma<T>::kE]) {
+  if constexpr (sizeof(T) == 2) {
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    u4 o[8];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const u4 a = __builtin_bit_cast(u4, in[2 * p]), b = __builtin_bit_cast(u4, in[2 * p + 1]);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        o[2 * d][p] = __builtin_amdgcn_perm(b[d], a[d], 0x05040100);
+        o[2 * d + 1][p] = __builtin_amdgcn_perm(b[d], a[d], 0x07060302);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = __builtin_bit_cast(typename Mma<T>::Frag, o[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) out[j][k] = in[k][j];
+  }
+}
+
+// What the rows are: adapter of each, its factor, and how many there are of both.
 struct Rows {
   const int32_t* index;
   const float* scale;
   float scale_value;
-  int n;
+  int n, T;
 };
-
 __device__ __forceinline__ int adapter_of(const Rows& g, int64_t t) { return g.index ? g.index[t] : 0; }
 __device__ __forceinline__ float scale_of(const Rows& g, int i) { return g.scale ? g.scale[i] : g.scale_value; }
 
-// low (T x r) = U (T x C) F_i (C x r); one workgroup per row
+// ---- few rows -------------------------------------------------------------
+
+struct Few {
+  const void* U;
+  int64_t ldu;
+  View W, F, G;
+  Rows rows;
+  float *part, *low;  // part: splits x T x ldp, low: low_splits x T x r
+  int C, N, r, ldp, splits, blocks, low_splits;
+  void* Y;
+  int64_t ldy;
+};
+
+// One wave: 16 kE columns of W, its steps of the sum; W_KC: W's sum runs along its rows in memory.
+// Each 16-byte load of 16 neighbouring lanes covers 256 bytes of a row of W (64 where W_KC: two steps make the line).
+template <class T, bool W_KC, int TT, bool EDGE>
+__device__ __forceinline__ void few_steps(const Few& a, int n0, int s0, int s1, f4 (&acc)[Mma<T>::kE][TT]) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int E = M::kE;
+  const int l16 = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+  const T* W = (const T*)a.W.p;
+  const T* U = (const T*)a.U;
+#pragma unroll 2
+  for (int s = s0; s < s1; ++s) {
+    const int k = s * M::kStep + g * E;
+    Frag w[E], x[TT];
+    if constexpr (W_KC) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int n = n0 + j * 16 + l16;
+        if constexpr (EDGE) w[j] = load_part(W + (int64_t)min(n, a.N - 1) * a.W.cs + k, a.C - k);
+        else w[j] = load16(W + (int64_t)n * a.W.cs + k);
+      }
+    } else {
+      Frag in[E];
+      const int n = n0 + l16 * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if constexpr (EDGE) in[e] = load_part(W + (int64_t)(k + e) * a.W.rs + n, k + e < a.C ? a.N - n : 0);
+        else in[e] = load16(W + (int64_t)(k + e) * a.W.rs + n);
+      }
+      turn<T>(in, w);
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const T* row = U + (int64_t)min(t * 16 + l16, a.rows.T - 1) * a.ldu;
+      if constexpr (EDGE) x[t] = load_part(row + k, a.C - k);
+      else x[t] = load16(row + k);
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) acc[j][t] = M::mma(w[j], x[t], acc[j][t]);
+  }
+}
+
+// low (T x r) of one row over one piece of C, on the vector units: F_i is read once per row that uses it.
 template <class T>
-__global__ __launch_bounds__(256) void low_kernel(View<const T> U, View<const T> F, Rows g, float* low, int C, int r) {
-  const int64_t t = blockIdx.x;
-  const int i = adapter_of(g, t);
-  if (i < 0 || i >= g.n) return;
-  __shared__ float part[4];
-  for (int j = 0; j < r; ++j) {
-    float s = 0.f;
-    for (int c = threadIdx.x; c < C; c += 256)
-      s += (float)U.p[t * U.rs + c * U.cs] * (float)F.p[i * F.as + c * F.rs + j * F.cs];
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = s;
+__device__ __forceinline__ void few_low(const Few& a, int t, int split, float* lds) {
+  using M = Mma<T>;
+  constexpr int E = M::kE;
+  const int i = adapter_of(a.rows, t);
+  if (i < 0 || i >= a.rows.n) return;
+  const int piece = (a.C + a.low_splits - 1) / a.low_splits, c0 = split * piece, c1 = min(a.C, c0 + piece);
+  const T* u = (const T*)a.U + t * a.ldu;
+  const T* f = (const T*)a.F.p + i * a.F.as;
+  float* out = a.low + ((int64_t)split * a.rows.T + t) * a.r;
+  if (a.F.rs != 1) {
+    // r values side by side: thread (c, chunk of E ranks)
+    const int chunks = (a.r + E - 1) / E, lanes = 256 / chunks;
+    const int j0 = threadIdx.x % chunks * E, cl = threadIdx.x / chunks;
+    float acc[E] = {};
+    if (cl < lanes)
+#pragma unroll 4
+      for (int c = c0 + cl; c < c1; c += lanes) {
+        const auto v = load_part(f + c * a.F.rs + j0, a.r - j0);
+        const float x = (float)u[c];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += x * (float)v[e];
+      }
+    // thread layout [cl][chunk][e] is [cl][rank]: sum over cl
+#pragma unroll
+    for (int e = 0; e < E; ++e) lds[threadIdx.x * E + e] = acc[e];
     __syncthreads();
-    if (threadIdx.x == 0) low[t * r + j] = part[0] + part[1] + part[2] + part[3];
+    const int width = chunks * E;
+    for (int j = threadIdx.x; j < a.r; j += 256) {
+      float s = 0.f;
+      for (int c = 0; c < lanes; ++c) s += lds[c * width + j];
+      out[j] = s;
+    }
+  } else {
+    // the sum runs along memory: a wave per rank
+    const int lane = threadIdx.x % 64;
+    for (int j = threadIdx.x / 64; j < a.r; j += 4) {
+      const T* fj = f + j * a.F.cs;
+      float s = 0.f;
+      for (int c = c0 + lane * E; c < c1; c += 64 * E) {
+        const auto v = load_part(fj + c, c1 - c), x = load_part(u + c, c1 - c);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += (float)v[e] * (float)x[e];
+      }
+#pragma unroll
+      for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+      if (lane == 0) out[j] = s;
+    }
+  }
+}
+
+// The first launch: blocks x splits workgroups of the large product, then T x low_splits of the low one.
+// Four waves share a block of 16 kE columns and cut its steps once more; their sums meet in LDS.
+template <class T, bool W_KC, int TT>
+__global__ __launch_bounds__(256) void few_kernel(Few a) {
+  using M = Mma<T>;
+  constexpr int E = M::kE, kCols = 16 * E;
+  constexpr int kFrags = E * TT;
+  __shared__ f4 lds[2 * kFrags * 64];
+  const int b = blockIdx.x;
+  if (b >= a.blocks * a.splits) {
+    static_assert(sizeof(lds) >= 256 * E * sizeof(float), "few_low's sums");
+    const int q = b - a.blocks * a.splits;
+    few_low<T>(a, q / a.low_splits, q % a.low_splits, (float*)lds);
+    return;
+  }
+  const int block = b % a.blocks, split = b / a.blocks, n0 = block * kCols;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int steps = (a.C + M::kStep - 1) / M::kStep, parts = a.splits * 4, part = split * 4 + wave;
+  const int s0 = (int)((int64_t)steps * part / parts), s1 = (int)((int64_t)steps * (part + 1) / parts);
+  f4 acc[E][TT] = {};
+  if (n0 + kCols <= a.N && s1 * M::kStep <= a.C) few_steps<T, W_KC, TT, false>(a, n0, s0, s1, acc);
+  else few_steps<T, W_KC, TT, true>(a, n0, s0, s1, acc);
+  // waves 2 and 3 hand theirs to 0 and 1, then 1 to 0
+#pragma unroll
+  for (int half = 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half)
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) lds[((wave - half) * kFrags + j * TT + t) * 64 + lane] = acc[j][t];
+    __syncthreads();
+    if (wave < half)
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[j][t] += lds[(wave * kFrags + j * TT + t) * 64 + lane];
+    __syncthreads();
+  }
+  if (wave) return;
+  const int l16 = lane % 16, g = lane / 16;
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int row = t * 16 + l16;
+    if (row >= a.rows.T) continue;
+    float* out = a.part + ((int64_t)split * a.rows.T + row) * a.ldp + n0;
+    if constexpr (W_KC) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) *(f4*)(out + j * 16 + g * 4) = acc[j][t];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < E; j += 4) {
+          const f4 v = {acc[j][t][i], acc[j + 1][t][i], acc[j + 2][t][i], acc[j + 3][t][i]};
+          *(f4*)(out + (g * 4 + i) * E + j) = v;
+        }
+    }
+  }
+}
+
+// The second launch: sums of the pieces, the product with G_i, the result.
+// A workgroup takes 256 columns of one row; its four waves share the pieces and the ranks.
+struct Finish {
+  const float *part, *low;
+  View G;
+  Rows rows;
+  const int32_t* perm;  // the row at each place of part and low; null: in order
+  int N, r, ldp, splits, low_splits, ldl, blocks;
+  void* Y;
+  int64_t ldy;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void finish_kernel(Finish a) {
+  __shared__ float s[GELIM_ADAPTER_MAX_RANK];
+  __shared__ f4 sums[3][64];
+  const int at = blockIdx.x / a.blocks, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int64_t t = a.perm ? a.perm[at] : at;
+  const int i = adapter_of(a.rows, t);
+  const bool has = i >= 0 && i < a.rows.n;
+  const int n = blockIdx.x % a.blocks * 256 + lane * 4;
+  f4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (n < a.N)
+#pragma unroll 4
+    for (int p = wave; p < a.splits; p += 4) acc += *(const f4*)(a.part + ((int64_t)p * a.rows.T + at) * a.ldp + n);
+  if (has) {
+    const float f = scale_of(a.rows, i);
+    for (int j = threadIdx.x; j < a.r; j += 256) {
+      float v = 0.f;
+      for (int p = 0; p < a.low_splits; ++p) v += a.low[((int64_t)p * a.rows.T + at) * a.ldl + j];
+      s[j] = f * v;
+    }
+    __syncthreads();
+    const T* G = (const T*)a.G.p + i * a.G.as;
+    if (n < a.N) {
+      const int have = min(4, a.N - n);
+      if (a.G.cs == 1 && have == 4) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Four {
+          T v[4];
+        };
+#pragma unroll 4
+        for (int j = wave; j < a.r; j += 4) {
+          const Four v = *(const Four*)(G + j * a.G.rs + n);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += s[j] * (float)v.v[e];
+        }
+      } else {
+        for (int j = wave; j < a.r; j += 4)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < have) acc[e] += s[j] * (float)G[j * a.G.rs + (n + e) * a.G.cs];
+      }
+    }
+  }
+  if (wave) sums[wave - 1][lane] = acc;
+  __syncthreads();
+  if (wave || n >= a.N) return;
+  acc += sums[0][lane] + sums[1][lane] + sums[2][lane];
+  if (!has && i != -1) acc = acc * __builtin_nanf("");
+  T* y = (T*)a.Y + t * a.ldy + n;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < a.N) y[e] = (T)acc[e];
+}
+
+// ---- many rows ------------------------------------------------------------
+//
+// The rows in order of their adapter: perm (T places), start (n + 1): adapter
+// i's places are start[i] .. start[i + 1] - 1, rows without one come last.  With one adapter
+// and no index both are null and the order is the rows' own.
+
+struct Order {
+  const int32_t *perm, *start;
+};
+__device__ __forceinline__ int64_t row_at(const Order& o, int64_t at) { return o.perm ? o.perm[at] : at; }
+
+// Pieces of at most `size` places, each within one adapter.  Adapter i's
+// pieces have the numbers from start[i] / size + i on: distinct for different adapters, as
+// floor((s + c) / size) - floor(s / size) + 1 >= ceil(c / size), and without a
+// table.  Numbers in between stay empty (count 0).
+struct Piece {
+  int adapter, begin, count;
+};
+__device__ __forceinline__ int first_piece(const Order& o, int i, int size) { return o.start ? o.start[i] / size + i : 0; }
+__device__ __forceinline__ Piece piece_of(const Order& o, const Rows& g, int number, int size) {
+  if (!o.start) return {0, number * size, max(0, min(size, g.T - number * size))};
+  int lo = 0, hi = g.n - 1;  // the last adapter whose pieces begin at or before the number
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (first_piece(o, mid, size) <= number) lo = mid;
+    else hi = mid - 1;
+  }
+  const int begin = o.start[lo] + (number - first_piece(o, lo, size)) * size;
+  return {lo, begin, max(0, min(size, o.start[lo + 1] - begin))};
+}
+int pieces(int64_t T, int64_t n, bool ordered, int size) { return (int)(T / size + (ordered ? n : 1)); }
+
+// A matrix (one per adapter) copied as rows x ld values, zeros behind the source's rows and columns.
+struct Copy {
+  View src;
+  void* dst;
+  int rows, cols, ld, count;  // of the copy (rows, ld) and how many matrices
+  int have;                   // rows of the source; the others are zeros
+  int first;                  // workgroups before this copy's
+};
+constexpr int kCopies = 6, kCopyTile = 64;
+struct Prepare {
+  Rows rows;
+  int32_t *perm, *start;
+  int order_groups;  // n + 1, or 0: the order is not needed
+  Copy copy[kCopies];
+  int copies;
+};
+
+// Adapter i's rows (i = n: those without one), in order, by one workgroup:
+// it counts the rows of lower adapters, then writes its own behind those.
+__device__ __forceinline__ void order_rows(const Prepare& p, int i) {
+  __shared__ int lower[16], own[16];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = p.rows.n;
+  auto adapter = [&](int t) {
+    const int a = p.rows.index ? p.rows.index[t] : 0;
+    return a < 0 || a >= n ? n : a;
+  };
+  int c = 0;
+  for (int64_t t = threadIdx.x; t < p.rows.T; t += 1024) c += adapter((int)t) < i;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
+  if (lane == 0) lower[wave] = c;
+  __syncthreads();
+  int at = 0;
+  for (int w = 0; w < 16; ++w) at += lower[w];
+  if (threadIdx.x == 0) p.start[i] = at;
+  for (int64_t t0 = 0; t0 < p.rows.T; t0 += 1024) {
+    const int64_t t = t0 + threadIdx.x;
+    const bool mine = t < p.rows.T && adapter((int)t) == i;
+    const uint64_t all = __ballot(mine);
+    if (lane == 0) own[wave] = __popcll(all);
+    __syncthreads();
+    int before = at;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += own[w];
+      at += own[w];
+    }
+    if (mine) p.perm[before + __popcll(all & ((1ull << lane) - 1))] = (int32_t)t;
     __syncthreads();
   }
 }
 
-// Y (T x N) = X (T x K) W (K x N) + s_i low G_i (r x N); one thread per element of a 16 x 16 tile
+// One 64 x 64 tile of a copy, read along the source's memory and written along the destination's.
 template <class T>
-__global__ __launch_bounds__(256) void product_kernel(View<const T> X, View<const T> W, View<const T> G, Rows g,
-                                                      const float* low, View<T> Y, int64_t Tn, int K, int N, int r) {
-  __shared__ float xs[16][17], ws[16][17];
-  const int x = threadIdx.x % 16, y = threadIdx.x / 16;
-  const int64_t t = (int64_t)blockIdx.y * 16 + y;
-  const int64_t n = (int64_t)blockIdx.x * 16 + x;
-  float acc = 0.f;
-  for (int k0 = 0; k0 < K; k0 += 16) {
-    xs[y][x] = t < Tn && k0 + x < K ? (float)X.p[t * X.rs + (k0 + x) * X.cs] : 0.f;
-    ws[y][x] = n < N && k0 + y < K ? (float)W.p[(k0 + y) * W.rs + n * W.cs] : 0.f;
-    __syncthreads();
-    for (int k = 0; k < 16; ++k) acc += xs[y][k] * ws[k][x];
-    __syncthreads();
+__device__ __forceinline__ void copy_tile(const Copy& c, int tile) {
+  __shared__ T lds[kCopyTile][kCopyTile + 2];
+  const int across = (c.ld + kCopyTile - 1) / kCopyTile, down = (c.rows + kCopyTile - 1) / kCopyTile;
+  const int m = tile / (across * down), r0 = tile / across % down * kCopyTile, c0 = tile % across * kCopyTile;
+  const T* src = (const T*)c.src.p + m * c.src.as;
+  T* dst = (T*)c.dst + (int64_t)m * c.rows * c.ld;
+  const int fast = threadIdx.x % 64, slow = threadIdx.x / 64;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int a = slow + 16 * k;
+    const int i = c.src.cs == 1 ? a : fast, j = c.src.cs == 1 ? fast : a;
+    lds[i][j] = r0 + i < c.have && c0 + j < c.cols ? src[(r0 + i) * c.src.rs + (c0 + j) * c.src.cs] : (T)0.f;
   }
-  if (t >= Tn || n >= N) return;
-  const int i = adapter_of(g, t);
-  if (i >= 0 && i < g.n) {
-    float s = 0.f;
-    for (int j = 0; j < r; ++j) s += low[t * r + j] * (float)G.p[i * G.as + j * G.rs + n * G.cs];
-    acc += scale_of(g, i) * s;
-  } else if (i != -1) {
-    acc = __builtin_nanf("");
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int i = slow + 16 * k;
+    if (r0 + i < c.rows && c0 + fast < c.ld) dst[(int64_t)(r0 + i) * c.ld + c0 + fast] = lds[i][fast];
   }
-  Y.p[t * Y.rs + n * Y.cs] = (T)acc;
 }
 
-// F_i (C x r) = s_i sum over the rows t of adapter i of U_t^T low_t; one thread per column of U
+// The first launch: the order, the factors laid out for the matrix units, and
+// an operand whose rows do not begin at multiples of 16 bytes copied to where they do.
 template <class T>
-__global__ __launch_bounds__(256) void factor_grad_kernel(View<const T> U, const float* low, Rows g, View<T> F,
-                                                          int64_t Tn, int C, int r) {
-  const int c = blockIdx.x * 256 + threadIdx.x, i = blockIdx.y, j = blockIdx.z;
-  if (c >= C) return;
-  float s = 0.f;
-  for (int64_t t = 0; t < Tn; ++t)
-    if (adapter_of(g, t) == i) s += (float)U.p[t * U.rs + c * U.cs] * low[t * r + j];
-  F.p[i * F.as + c * F.rs + j * F.cs] = (T)(scale_of(g, i) * s);
+__global__ __launch_bounds__(1024) void prepare_kernel(Prepare p) {
+  int b = blockIdx.x;
+  if (b < p.order_groups) return order_rows(p, b);
+  b -= p.order_groups;
+  int k = p.copies - 1;
+  while (k > 0 && b < p.copy[k].first) --k;
+  copy_tile<T>(p.copy[k], b - p.copy[k].first);
+}
+
+// low (split, place, rank) = U F_i, 32 places of one adapter by a workgroup, whose four waves cut the sum.
+// F is laid out as rp ranks x ldf along the sum, zeros behind C.
+struct Low {
+  const void *U, *F;
+  int64_t ldu;
+  float* low;
+  int cu, ldf, splits, pieces;  // cu: values in a row of U, a multiple of 16 bytes
+};
+struct LowPair {
+  Low p[2];
+  Rows rows;
+  Order order;
+};
+constexpr int kLowRows = 32;
+
+template <class T, int RB>
+__global__ __launch_bounds__(256) void low_kernel(LowPair both) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int E = M::kE, rp = 16 * RB;
+  __shared__ f4 lds[3][RB * 2][64];
+  const Low& a = both.p[blockIdx.y];
+  const int split = blockIdx.x / a.pieces;
+  if (split >= a.splits) return;
+  const Piece pc = piece_of(both.order, both.rows, blockIdx.x % a.pieces, kLowRows);
+  if (pc.count == 0) return;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
+  const T* u[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    u[t] = (const T*)a.U + row_at(both.order, pc.begin + min(t * 16 + l16, pc.count - 1)) * a.ldu;
+  const T* f = (const T*)a.F + ((int64_t)pc.adapter * rp + l16) * a.ldf;
+  const int steps = (a.cu + M::kStep - 1) / M::kStep, parts = a.splits * 4, part = split * 4 + wave;
+  const int s0 = (int)((int64_t)steps * part / parts), s1 = (int)((int64_t)steps * (part + 1) / parts);
+  f4 acc[RB][2] = {};
+#pragma unroll 4
+  for (int s = s0; s < s1; ++s) {
+    const int k = s * M::kStep + g * E;
+    Frag x[2], w[RB];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x[t] = Frag{};
+      if (k < a.cu) x[t] = *(const Frag*)(u[t] + k);
+    }
+#pragma unroll
+    for (int j = 0; j < RB; ++j) w[j] = *(const Frag*)(f + (int64_t)j * 16 * a.ldf + k);
+#pragma unroll
+    for (int j = 0; j < RB; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) acc[j][t] = M::mma(w[j], x[t], acc[j][t]);
+  }
+  if (wave)
+#pragma unroll
+    for (int j = 0; j < RB; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) lds[wave - 1][j * 2 + t][lane] = acc[j][t];
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    if (t * 16 + l16 >= pc.count) continue;
+    float* out = a.low + ((int64_t)split * both.rows.T + pc.begin + t * 16 + l16) * rp + g * 4;
+#pragma unroll
+    for (int j = 0; j < RB; ++j)
+      *(f4*)(out + j * 16) = acc[j][t] + lds[0][j * 2 + t][lane] + lds[1][j * 2 + t][lane] + lds[2][j * 2 + t][lane];
+  }
+}
+
+// The large product: (U W) of BT places x BN columns, sum in steps of 128 bytes.
+struct Big {
+  const void *U, *W, *G;
+  int64_t ldu, ldw;
+  int cu, cw;  // values of a row of U / of the sum in W that exist (W_KC: multiples of 16 bytes); zeros behind
+  Rows rows;
+  Order order;
+  const float* low;
+  int N, nw, r, rp, low_splits, splits, tiles_t, tiles_n;  // nw: columns of W as stored
+  void* Y;
+  int64_t ldy;
+  float* part;  // splits > 1: partial sums instead of Y
+  int ldp;
+};
+
+__device__ const uint4 g_zeros[1] = {};
+
+// 16 bytes per lane from global memory to LDS, at base + 16 lane
+__device__ __forceinline__ void to_lds(const void* from, void* base) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+}
+
+// Tiles in LDS, as chunks of 16 bytes.  Operands whose sum runs along memory:
+// rows of 8 chunks, chunk c of row i at place c ^ (i / 2 % 8), so that the 16
+// rows a fragment reads lie in 16 different places of 256 bytes.  Otherwise rows
+// (of the sum) of all columns; the 32 (fp32: 64) bytes that a read takes from a
+// row are moved by the row's number, so that the rows of one read fall on different banks.
+template <class T, int kRowChunks>
+__device__ __forceinline__ int swap_columns(int k) {  // in chunks
+  if constexpr (sizeof(T) == 2) return ((k & 3) | (k >> 1 & 4)) * 2 % kRowChunks;
+  else return (k >> 2 & 3) * 4 % kRowChunks;
+}
+
+template <class T, bool W_KC, int BT, int BN, int WT, int WN, bool SPLIT>
+__global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int E = M::kE, BK = 8 * E, kThreads = WT * WN * 64, kWaves = WT * WN;
+  constexpr int TT = BT / WT / 16, TN = BN / WN / 16;
+  constexpr int kLoadU = BT * 8 / kThreads, kLoadW = BN * 8 / kThreads;
+  constexpr int kRowChunks = BN / E;  // chunks in a row of W's tile if not W_KC
+  static_assert(kLoadU * kThreads == BT * 8 && kLoadW * kThreads == BN * 8, "tile and threads");
+  __shared__ __attribute__((aligned(16))) T us[2][BT * BK], ws[2][BN * BK];
+
+  // workgroups go to the 8 XCDs in turn: each XCD gets neighbouring tiles, which share operands in its L2
+  const int tiles = a.tiles_t * a.tiles_n, q = tiles / 8, rem = tiles % 8, xcd = blockIdx.x % 8;
+  const int tile = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + blockIdx.x / 8;
+  const int t0 = tile / a.tiles_n * BT, n0 = tile % a.tiles_n * BN;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
+  const int wt = wave / WN * (BT / WT), wn = wave % WN * (BN / WN);
+
+  const int nk = (max(a.cu, a.cw) + BK - 1) / BK;
+  const int k0 = SPLIT ? (int)((int64_t)nk * blockIdx.y / a.splits) : 0;
+  const int k1 = SPLIT ? (int)((int64_t)nk * (blockIdx.y + 1) / a.splits) : nk;
+
+  // what each lane loads: row of U / chunk along the sum, and the same of W
+  const T *up[kLoadU], *wp[kLoadW];
+  int uk[kLoadU], wk[kLoadW];
+#pragma unroll
+  for (int q = 0; q < kLoadU; ++q) {
+    const int i = (wave * kLoadU + q) * 8 + lane / 8;
+    uk[q] = ((lane % 8) ^ (i >> 1 & 7)) * E;
+    up[q] = (const T*)a.U + row_at(a.order, min(t0 + i, a.rows.T - 1)) * a.ldu + uk[q];
+  }
+#pragma unroll
+  for (int q = 0; q < kLoadW; ++q) {
+    if constexpr (W_KC) {
+      const int i = (wave * kLoadW + q) * 8 + lane / 8;
+      wk[q] = ((lane % 8) ^ (i >> 1 & 7)) * E;
+      wp[q] = (const T*)a.W + (int64_t)min(n0 + i, a.N - 1) * a.ldw + wk[q];
+    } else {
+      const int place = (wave * kLoadW + q) * 64 + lane, k = place / kRowChunks;
+      const int n = n0 + ((place % kRowChunks) ^ swap_columns<T, kRowChunks>(k)) * E;
+      wk[q] = n < a.nw ? k : INT_MAX / 2;
+      wp[q] = (const T*)a.W + (int64_t)k * a.ldw + n;
+    }
+  }
+  const int64_t w_step = W_KC ? BK : BK * a.ldw;
+  auto load = [&](int kt, int buf) {
+    const int k = kt * BK;
+#pragma unroll
+    for (int q = 0; q < kLoadU; ++q)
+      to_lds(k + uk[q] < a.cu ? (const void*)(up[q] + k) : g_zeros, &us[buf][(wave * kLoadU + q) * 64 * E]);
+#pragma unroll
+    for (int q = 0; q < kLoadW; ++q)
+      to_lds(k + wk[q] < a.cw ? (const void*)(wp[q] + kt * w_step) : g_zeros, &ws[buf][(wave * kLoadW + q) * 64 * E]);
+  };
+
+  f4 acc[TN][TT] = {};
+  auto compute = [&](int buf) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      Frag x[TT], w[TN];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int i = wt + t * 16 + l16;
+        x[t] = *(const Frag*)&us[buf][i * BK + ((kk * 4 + g) ^ (i >> 1 & 7)) * E];
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        if constexpr (W_KC) {
+          const int i = wn + j * 16 + l16;
+          w[j] = *(const Frag*)&ws[buf][i * BK + ((kk * 4 + g) ^ (i >> 1 & 7)) * E];
+        } else if constexpr (sizeof(T) == 2) {
+          // 16 lanes read 4 rows (of the sum) x 16 columns, 8 bytes each, and get their column's 4 values
+          s8 v;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = kk * 32 + g * 8 + h * 4 + l16 / 4;
+            const int chunk = ((wn + j * 16) / 8 + (l16 % 4) / 2) ^ swap_columns<T, kRowChunks>(k);
+            const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s4*)&ws[buf][k * BN + chunk * 8 + l16 % 2 * 4]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[h * 4 + e] = r[e];
+          }
+          w[j] = __builtin_bit_cast(Frag, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = kk * 16 + g * 4 + e, n = wn + j * 16 + l16;
+            w[j][e] = ws[buf][k * BN + ((n / E) ^ swap_columns<T, kRowChunks>(k)) * E + n % E];
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[j][t] = M::mma(w[j], x[t], acc[j][t]);
+    }
+  };
+
+  if (k0 < k1) load(k0, 0);
+  __syncthreads();
+  for (int kt = k0; kt < k1; ++kt) {
+    const int buf = (kt - k0) & 1;
+    if (kt + 1 < k1) load(kt + 1, buf ^ 1);
+    compute(buf);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int at = t0 + wt + t * 16 + l16;
+    if constexpr (SPLIT) {
+      if (at < a.rows.T) {
+        float* out = a.part + ((int64_t)blockIdx.y * a.rows.T + at) * a.ldp + n0 + wn + g * 4;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) *(f4*)(out + j * 16) = acc[j][t];
+      }
+    } else {
+      const bool in = at < a.rows.T;
+      const int64_t row = row_at(a.order, min(at, a.rows.T - 1));
+      const int mine = in ? adapter_of(a.rows, row) : -1;
+      const bool has = mine >= 0 && mine < a.rows.n;
+      // s_i (U F_i) G_i: for each adapter among these 16 rows the product of all of them, kept where it is theirs
+      uint64_t left = __ballot(has);
+      if (left) {
+        // 16-bit types: U F_i as the sum of two values of the type, side by side along the sum (16 ranks are a step
+        // of 32); with one, its rounding alone would be as large as the result's.  fp16: first brought
+        // to below 2^14 by a power of two, as it may be beyond the type's range.
+        float up_by = 1.f, down_by = 1.f;
+        const float* lo = a.low + (int64_t)min(at, a.rows.T - 1) * a.rp;
+        auto low_at = [&](int j) {
+          float v = 0.f;
+          for (int p = 0; p < a.low_splits; ++p) v += lo[(int64_t)p * a.rows.T * a.rp + j];
+          return v;
+        };
+        if constexpr (std::is_same_v<T, _Float16>) {
+          float most = 0.f;
+          for (int j = g; j < a.rp; j += 4) {
+            const float v = has ? fabsf(low_at(j)) : 0.f;
+            if (v > most && v <= 3.4e38f) most = v;
+          }
+          most = fmaxf(most, __shfl_xor(most, 16, 64));
+          most = fmaxf(most, __shfl_xor(most, 32, 64));
+          if (most > 0.f) {
+            const int e = min(max(14 - ilogbf(most) - 1, -100), 100);
+            down_by = ldexpf(1.f, e);
+            up_by = ldexpf(1.f, -e);
+          }
+        }
+        while (left) {
+          const int cur = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+          left &= ~__ballot(mine == cur);
+          f4 d[TN] = {};
+          const T* G = (const T*)a.G + (int64_t)cur * a.N * a.rp;
+          for (int b = 0; b < a.rp / 16; ++b) {
+            const int j0 = b * 16 + (sizeof(T) == 2 ? (g & 1) * 8 : g * 4);
+            Frag x;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const float v = has ? low_at(j0 + e) * down_by : 0.f;
+              if constexpr (sizeof(T) == 2) {
+                const T hi = (T)v;
+                const float rest = v - (float)hi;
+                x[e] = g < 2 ? hi : fabsf((float)hi) <= 3.4e38f ? (T)rest : (T)0.f;
+              } else {
+                x[e] = v;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+              const Frag w = *(const Frag*)(G + (int64_t)min(n0 + wn + j * 16 + l16, a.N - 1) * a.rp + j0);
+              d[j] = M::mma(w, x, d[j]);
+            }
+          }
+          const float f = scale_of(a.rows, cur) * up_by;
+          if (mine == cur)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[j][t] += f * d[j];
+        }
+      }
+      if (!in) continue;
+      T* out = (T*)a.Y + row * a.ldy;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int n = n0 + wn + j * 16 + g * 4;
+        f4 v = acc[j][t];
+        if (!has && mine != -1) v = v * __builtin_nanf("");
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < a.N) out[n + e] = (T)v[e];
+      }
+    }
+  }
+}
+
+// The factors' gradients: sum over the places of an adapter of U_t^T V_t, V = S or D.
+// First V turned (a value per place along memory), in pieces of kGradRows places: 16-bit types as two values
+// of the type whose sum has V's upper bits (fp16: brought to below 2^14 by the piece's power of two).
+constexpr int kGradRows = 128;
+struct Turn {
+  const float* low;
+  void* out;    // piece, half (16-bit types), rank, place
+  float* back;  // of each piece, the factor that undoes the power of two
+  int splits;
+};
+struct TurnPair {
+  Turn p[2];
+  Rows rows;
+  Order order;
+  int rp;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void turn_kernel(TurnPair both) {
+  __shared__ float wave_most[4];
+  const Turn& a = both.p[blockIdx.y];
+  const int rp = both.rp;
+  const Piece pc = piece_of(both.order, both.rows, blockIdx.x, kGradRows);
+  if (pc.count == 0) return;
+  const int t = threadIdx.x % kGradRows;
+  auto value = [&](int j) {
+    float v = 0.f;
+    if (t < pc.count)
+      for (int p = 0; p < a.splits; ++p) v += a.low[((int64_t)p * both.rows.T + pc.begin + t) * rp + j];
+    return v;
+  };
+  float by = 1.f, back = 1.f;
+  if constexpr (std::is_same_v<T, _Float16>) {
+    float most = 0.f;
+    for (int j = threadIdx.x / kGradRows; j < rp; j += 256 / kGradRows) {
+      const float v = fabsf(value(j));
+      if (v > most && v <= 3.4e38f) most = v;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    if (threadIdx.x % 64 == 0) wave_most[threadIdx.x / 64] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(wave_most[0], wave_most[1]), fmaxf(wave_most[2], wave_most[3]));
+    if (most > 0.f) {
+      const int e = min(max(13 - ilogbf(most), -100), 100);
+      by = ldexpf(1.f, e);
+      back = ldexpf(1.f, -e);
+    }
+  }
+  if (threadIdx.x == 0) a.back[blockIdx.x] = back;
+  constexpr int kHalves = sizeof(T) == 2 ? 2 : 1;
+  T* out = (T*)a.out + (int64_t)blockIdx.x * kHalves * rp * kGradRows + t;
+  for (int j = threadIdx.x / kGradRows; j < rp; j += 256 / kGradRows) {
+    const float v = value(j) * by;
+    const T hi = (T)v;
+    out[j * kGradRows] = hi;
+    if constexpr (kHalves == 2) out[(rp + j) * kGradRows] = fabsf((float)hi) <= 3.4e38f ? (T)(v - (float)hi) : (T)0.f;
+  }
+}
+
+// Then the products of a piece: a wave takes 16 kE columns of U, whose rows it turns in registers.
+struct Outer {
+  const void *U, *V;
+  int64_t ldu;
+  float* part;  // piece, rank, column
+  int cu, ldp, blocks;
+};
+struct OuterPair {
+  Outer p[2];
+  Rows rows;
+  Order order;
+  int rp, pieces;
+};
+
+template <class T, int RB>
+__global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int E = M::kE, kHalves = sizeof(T) == 2 ? 2 : 1;
+  __shared__ int32_t row[kGradRows];
+  const Outer& a = both.p[blockIdx.y];
+  const int piece = blockIdx.x % both.pieces, block = blockIdx.x / both.pieces;
+  if (block >= a.blocks) return;
+  const Piece pc = piece_of(both.order, both.rows, piece, kGradRows);
+  if (pc.count == 0) return;
+  if (threadIdx.x < kGradRows) row[threadIdx.x] = (int32_t)row_at(both.order, pc.begin + min((int)threadIdx.x, pc.count - 1));
+  __syncthreads();
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
+  const int n0 = (block * 4 + wave) * 16 * E, n = n0 + l16 * E;
+  if (n0 >= a.cu) return;
+  const int j0 = blockIdx.z * RB * 16;
+  const T* V = (const T*)a.V + ((int64_t)piece * kHalves * both.rp + j0 + l16) * kGradRows;
+  const T* U = (const T*)a.U + n;
+  f4 acc[E][RB] = {};
+  const int steps = (pc.count + M::kStep - 1) / M::kStep;
+#pragma unroll 2
+  for (int s = 0; s < steps; ++s) {
+    const int t = s * M::kStep + g * E;
+    Frag in[E], w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      in[e] = Frag{};
+      if (t + e < pc.count && n < a.cu) in[e] = *(const Frag*)(U + row[t + e] * a.ldu);
+    }
+    turn<T>(in, w);
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const Frag v = *(const Frag*)(V + (int64_t)(h * both.rp + b * 16) * kGradRows + t);
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[j][b] = M::mma(w[j], v, acc[j][b]);
+      }
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    float* out = a.part + ((int64_t)piece * both.rp + j0 + b * 16 + l16) * a.ldp + n0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < E; j += 4)
+        *(f4*)(out + (g * 4 + i) * E + j) = f4{acc[j][b][i], acc[j + 1][b][i], acc[j + 2][b][i], acc[j + 3][b][i]};
+  }
+}
+
+// Last their sums, times s_i, in the factor's layout: 64 columns x 16 ranks of one adapter by a workgroup.
+struct Sum {
+  const float *part, *back;
+  void* out;
+  int64_t as, cs, rs;  // adapter, column, rank
+  int cols, ldp, blocks;
+};
+struct SumPair {
+  Sum p[2];
+  Rows rows;
+  Order order;
+  int r, rp;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void sum_kernel(SumPair both) {
+  __shared__ float lds[64][17];
+  const Sum& a = both.p[blockIdx.y];
+  if ((int)blockIdx.x >= a.blocks) return;
+  const int ranks = (both.r + 15) / 16;
+  const int c0 = blockIdx.x / ranks * 64, j0 = blockIdx.x % ranks * 16;
+  for (int i = blockIdx.z; i < both.rows.n; i += gridDim.z) {
+    const int count = both.order.start ? both.order.start[i + 1] - both.order.start[i] : both.rows.T;
+    const int first = first_piece(both.order, i, kGradRows), many = (count + kGradRows - 1) / kGradRows;
+    const float f = scale_of(both.rows, i);
+    const int c = threadIdx.x % 64, jq = threadIdx.x / 64 * 4;
+    float s[4] = {};
+    for (int p = first; p < first + many; ++p) {
+      const float back = a.back[p];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += back * a.part[((int64_t)p * both.rp + j0 + jq + e) * a.ldp + c0 + c];
+    }
+    T* out = (T*)a.out + i * a.as;
+    if (a.cs == 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c0 + c < a.cols && j0 + jq + e < both.r) out[(j0 + jq + e) * a.rs + c0 + c] = (T)(f * s[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lds[c][jq + e] = f * s[e];
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int cc = e * 16 + threadIdx.x / 16, j = threadIdx.x % 16;
+        if (c0 + cc < a.cols && j0 + j < both.r) out[(c0 + cc) * a.cs + (j0 + j) * a.rs] = (T)lds[cc][j];
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+int check_shape(const gelim_adapter_args& a) {
+  if (a.dtype < GELIM_T_F32 || a.dtype > GELIM_T_F16) return GELIM_FAIL(GELIM_E_ARG, "adapter: unknown type");
+  if (a.T < 0 || a.K <= 0 || a.N <= 0 || a.r <= 0 || a.n <= 0) return GELIM_FAIL(GELIM_E_ARG, "adapter: bad shape");
+  if (a.T > GELIM_ADAPTER_MAX_DIM || a.K > GELIM_ADAPTER_MAX_DIM || a.N > GELIM_ADAPTER_MAX_DIM || a.n > 65535)
+    return GELIM_FAIL(GELIM_E_ARG, "adapter: dimension too large");
+  if (a.r > GELIM_ADAPTER_MAX_RANK) return GELIM_FAIL(GELIM_E_ARG, "adapter: rank above 256");
+  return GELIM_OK;
 }
 
 int check(const gelim_adapter_args& a, bool grad) {
-  if (a.dtype < GELIM_T_F32 || a.dtype > GELIM_T_F16) return GELIM_FAIL(GELIM_E_ARG, "adapter: unknown type");
-  if (a.T < 0 || a.K <= 0 || a.N <= 0 || a.r <= 0 || a.n <= 0) return GELIM_FAIL(GELIM_E_ARG, "adapter: bad shape");
-  if (a.T > INT32_MAX || a.K > INT32_MAX || a.N > INT32_MAX || a.n > 65535)
-    return GELIM_FAIL(GELIM_E_ARG, "adapter: dimension too large");
-  if (a.r > GELIM_ADAPTER_MAX_RANK) return GELIM_FAIL(GELIM_E_ARG, "adapter: rank above 256");
+  GELIM_TRY(check_shape(a));
+  if (!a.index && a.n != 1 && a.T)
+    return GELIM_FAIL(GELIM_E_ARG, "adapter: an index is needed with more than one adapter");
   if (!a.W || !a.A || !a.B || (a.T && (!a.X || !a.Y))) return GELIM_FAIL(GELIM_E_ARG, "adapter: null matrix");
   if (a.ws_bytes < gelim_adapter_workspace(&a, grad)) return GELIM_FAIL(GELIM_E_ARG, "adapter: workspace too small");
   return GELIM_OK;
 }
 
-// A as K x r and B as r x N, or with `turn` their transposes
-template <class T>
-View<const T> view_w(const gelim_adapter_args& a, bool turn) {
-  View<const T> v{(const T*)a.W, 0, a.w_trans ? 1 : a.ldw, a.w_trans ? a.ldw : 1};
-  if (turn) std::swap(v.rs, v.cs);
-  return v;
+// Hands out the workspace; with a null base it only counts.
+struct Space {
+  char* base;
+  int64_t used = 0;
+  template <class P>
+  P* take(int64_t count) {
+    P* p = (P*)(base + used);
+    used += up(count * (int64_t)sizeof(P), 256);
+    return p;
+  }
+};
+
+constexpr int kFewRows = 64;
+
+// Y (T x N) = U (T x C) W (C x N) + s_i (U F_i) G_i
+struct Problem {
+  const void* U;
+  int64_t ldu;
+  int C, N;
+  View W, F, G;
+  bool w_kc;
+  void* Y;
+  int64_t ldy;
+};
+
+View turned(View v) { return {v.p, v.as, v.cs, v.rs}; }
+View view_w(const gelim_adapter_args& a) { return {a.W, 0, a.w_trans ? 1 : a.ldw, a.w_trans ? a.ldw : 1}; }
+View view_a(const gelim_adapter_args& a) { return {a.A, a.a_stride, a.a_trans ? 1 : a.lda, a.a_trans ? a.lda : 1}; }
+View view_b(const gelim_adapter_args& a) { return {a.B, a.b_stride, a.b_trans ? 1 : a.ldb, a.b_trans ? a.ldb : 1}; }
+Rows rows_of(const gelim_adapter_args& a) { return {a.index, a.scale, (float)a.scale_value, (int)a.n, (int)a.T}; }
+Problem product_of(const gelim_adapter_args& a) {
+  return {a.X, a.ldx, (int)a.K, (int)a.N, view_w(a), view_a(a), view_b(a), a.w_trans != 0, a.Y, a.ldy};
 }
-template <class T>
-View<const T> view_a(const gelim_adapter_args& a, bool turn) {
-  View<const T> v{(const T*)a.A, a.a_stride, a.a_trans ? 1 : a.lda, a.a_trans ? a.lda : 1};
-  if (turn) std::swap(v.rs, v.cs);
-  return v;
-}
-template <class T>
-View<const T> view_b(const gelim_adapter_args& a, bool turn) {
-  View<const T> v{(const T*)a.B, a.b_stride, a.b_trans ? 1 : a.ldb, a.b_trans ? a.ldb : 1};
-  if (turn) std::swap(v.rs, v.cs);
-  return v;
+Problem back_of(const gelim_adapter_args& a) {
+  return {a.Y, a.ldy, (int)a.N, (int)a.K, turned(view_w(a)), turned(view_b(a)), turned(view_a(a)), a.w_trans == 0,
+          a.dX, a.lddx};
 }
 
+int rank_blocks(int64_t r) {  // of 16, a power of two
+  int b = 1;
+  while (16 * b < r) b *= 2;
+  return b;
+}
+
+// -- few rows
+
 template <class T>
-int product(const gelim_adapter_args& a, hipStream_t s) {
-  const Rows g{a.index, a.scale, (float)a.scale_value, (int)a.n};
-  const View<const T> X{(const T*)a.X, 0, a.ldx, 1};
-  float* low = (float*)a.ws;
-  hipLaunchKernelGGL(low_kernel<T>, dim3((unsigned)a.T), dim3(256), 0, s, X, view_a<T>(a, false), g, low, (int)a.K,
-                     (int)a.r);
-  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.T + 15) / 16));
-  hipLaunchKernelGGL(product_kernel<T>, grid, dim3(256), 0, s, X, view_w<T>(a, false), view_b<T>(a, false), g, low,
-                     View<T>{(T*)a.Y, 0, a.ldy, 1}, a.T, (int)a.K, (int)a.N, (int)a.r);
+int few_product(const Problem& p, const Rows& g, int r, Space& ws, hipStream_t s, bool run) {
+  using M = Mma<T>;
+  Few f{};
+  f.U = p.U, f.ldu = p.ldu, f.W = p.W, f.F = p.F, f.G = p.G, f.rows = g, f.C = p.C, f.N = p.N, f.r = r;
+  f.blocks = (int)((p.N + 16 * M::kE - 1) / (16 * M::kE));
+  const int steps = (p.C + M::kStep - 1) / M::kStep;
+  f.splits = std::clamp(512 / f.blocks, 1, std::max(1, std::min(64, steps / 4)));
+  f.low_splits = std::clamp(256 / g.T, 1, std::max(1, std::min(16, p.C / 256)));
+  f.ldp = f.blocks * 16 * M::kE;
+  f.part = ws.take<float>((int64_t)f.splits * g.T * f.ldp);
+  f.low = ws.take<float>((int64_t)f.low_splits * g.T * r);
+  if (!run) return GELIM_OK;
+  const dim3 grid((unsigned)(f.blocks * f.splits + g.T * f.low_splits));
+  const int tt = (g.T + 15) / 16;
+  auto launch = [&](auto kc) {
+    constexpr bool KC = decltype(kc)::value;
+    if (tt == 1) hipLaunchKernelGGL((few_kernel<T, KC, 1>), grid, dim3(256), 0, s, f);
+    else if (tt == 2) hipLaunchKernelGGL((few_kernel<T, KC, 2>), grid, dim3(256), 0, s, f);
+    else hipLaunchKernelGGL((few_kernel<T, KC, 4>), grid, dim3(256), 0, s, f);
+  };
+  if (p.w_kc) launch(std::true_type{});
+  else launch(std::false_type{});
+  Finish e{f.part, f.low, p.G, g, nullptr, p.N, r, f.ldp, f.splits, f.low_splits, r, (p.N + 255) / 256,
+           p.Y, p.ldy};
+  hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)(g.T * e.blocks)), dim3(256), 0, s, e);
   HIP_TRY(hipGetLastError());
   return GELIM_OK;
 }
 
+// -- many rows
+
 template <class T>
-int gradient(const gelim_adapter_args& a, hipStream_t s) {
-  const Rows g{a.index, a.scale, (float)a.scale_value, (int)a.n};
-  const View<const T> X{(const T*)a.X, 0, a.ldx, 1}, dY{(const T*)a.Y, 0, a.ldy, 1};
-  float *S = (float*)a.ws, *D = S + a.T * a.r;
-  if (a.T) {
-    hipLaunchKernelGGL(low_kernel<T>, dim3((unsigned)a.T), dim3(256), 0, s, X, view_a<T>(a, false), g, S, (int)a.K,
-                       (int)a.r);
-    hipLaunchKernelGGL(low_kernel<T>, dim3((unsigned)a.T), dim3(256), 0, s, dY, view_b<T>(a, true), g, D, (int)a.N,
-                       (int)a.r);
-    if (a.dX) {
-      const dim3 grid((unsigned)((a.K + 15) / 16), (unsigned)((a.T + 15) / 16));
-      hipLaunchKernelGGL(product_kernel<T>, grid, dim3(256), 0, s, dY, view_w<T>(a, true), view_a<T>(a, true), g, D,
-                         View<T>{(T*)a.dX, 0, a.lddx, 1}, a.T, (int)a.N, (int)a.K, (int)a.r);
+struct Many {
+  static constexpr int E = Mma<T>::kE;
+  const gelim_adapter_args& a;
+  Rows g;
+  int rb, rp;
+  Prepare prep{};
+  Order order{};
+  unsigned groups = 0;
+  Space& ws;
+
+  Many(const gelim_adapter_args& args, Space& space) : a(args), g(rows_of(args)), ws(space) {
+    rb = rank_blocks(a.r);
+    rp = 16 * rb;
+    prep.rows = g;
+    if (a.index) {
+      prep.perm = ws.template take<int32_t>(a.T);
+      prep.start = ws.template take<int32_t>(a.n + 1);
+      prep.order_groups = (int)a.n + 1;
+      order = {prep.perm, prep.start};
+    }
+    groups = prep.order_groups;
+  }
+
+  T* copy(View src, int rows, int have, int cols, int ld, int count) {
+    Copy& c = prep.copy[prep.copies++];
+    c = {src, ws.template take<T>((int64_t)count * rows * ld), rows, cols, ld, count, have,
+         (int)groups - prep.order_groups};
+    groups += (unsigned)(count * ((rows + kCopyTile - 1) / kCopyTile) * ((ld + kCopyTile - 1) / kCopyTile));
+    return (T*)c.dst;
+  }
+  static bool aligned(const void* p, int64_t ld, int64_t len) {
+    return (uintptr_t)p % 16 == 0 && ld % E == 0 && len % E == 0;
+  }
+  // rows of U as 16-byte chunks: as they are, or copied
+  struct Wide {
+    const void* p;
+    int64_t ld;
+    int cols;  // that may be read
+  };
+  Wide wide(const void* p, int64_t ld, int64_t rows, int cols) {
+    if (aligned(p, ld, cols)) return {p, ld, cols};
+    const int to = (int)up(cols, 64);
+    return {copy({p, 0, ld, 1}, (int)rows, (int)rows, cols, to, 1), to, to};
+  }
+
+  // F laid out for the low product: ranks x the sum
+  Low low_of(const Wide& U, View F, int C) {
+    Low l{};
+    l.ldf = (int)up(C, 64);
+    l.F = copy(turned(F), rp, (int)a.r, C, l.ldf, (int)a.n);
+    l.U = U.p, l.ldu = U.ld, l.cu = U.cols;
+    l.pieces = pieces(a.T, a.n, a.index != nullptr, kLowRows);
+    const int steps = (C + Mma<T>::kStep - 1) / Mma<T>::kStep;
+    l.splits = (int)std::clamp<int64_t>(256 * kLowRows / std::max<int64_t>(a.T, 1), 1, std::clamp(steps / 8, 1, 8));
+    l.low = ws.template take<float>((int64_t)l.splits * a.T * rp);
+    return l;
+  }
+  int run_prepare(hipStream_t s) {
+    if (groups) hipLaunchKernelGGL(prepare_kernel<T>, dim3(groups), dim3(1024), 0, s, prep);
+    return GELIM_OK;
+  }
+  void run_low(const Low* l, int count, hipStream_t s) {
+    LowPair both{};
+    both.rows = g, both.order = order;
+    unsigned most = 0;
+    for (int k = 0; k < count; ++k) {
+      both.p[k] = l[k];
+      most = std::max(most, (unsigned)(l[k].pieces * l[k].splits));
+    }
+    const dim3 grid(most, (unsigned)count);
+    switch (rb) {
+      case 1: hipLaunchKernelGGL((low_kernel<T, 1>), grid, dim3(256), 0, s, both); break;
+      case 2: hipLaunchKernelGGL((low_kernel<T, 2>), grid, dim3(256), 0, s, both); break;
+      case 4: hipLaunchKernelGGL((low_kernel<T, 4>), grid, dim3(256), 0, s, both); break;
+      case 8: hipLaunchKernelGGL((low_kernel<T, 8>), grid, dim3(256), 0, s, both); break;
+      default: hipLaunchKernelGGL((low_kernel<T, 16>), grid, dim3(256), 0, s, both);
     }
   }
-  if (a.dA) {
-    const View<T> dA{(T*)a.dA, a.K * a.r, a.a_trans ? 1 : a.r, a.a_trans ? a.K : 1};
-    const dim3 grid((unsigned)((a.K + 255) / 256), (unsigned)a.n, (unsigned)a.r);
-    hipLaunchKernelGGL(factor_grad_kernel<T>, grid, dim3(256), 0, s, X, D, g, dA, a.T, (int)a.K, (int)a.r);
+
+  // the large product
+  struct Plan {
+    Big b;
+    bool kc;
+    int tile;
+    Problem p;
+    int low_splits;
+  };
+  Plan big_of(const Problem& p, const Wide& U) {
+    Plan q{};
+    Big& b = q.b;
+    q.kc = p.w_kc;
+    q.p = p;
+    b.U = U.p, b.ldu = U.ld, b.cu = U.cols, b.rows = g, b.order = order, b.N = p.N, b.r = (int)a.r, b.rp = rp;
+    b.Y = p.Y, b.ldy = p.ldy;
+    if (p.w_kc) {
+      const Wide w = wide(p.W.p, p.W.cs, p.N, p.C);
+      b.W = w.p, b.ldw = w.ld, b.cw = w.cols;
+    } else {
+      const Wide w = wide(p.W.p, p.W.rs, p.C, p.N);
+      b.W = w.p, b.ldw = w.ld, b.cw = p.C, b.nw = w.cols;
+    }
+    auto tiles = [&](int tile) { return ((a.T + tile - 1) / tile) * ((p.N + tile - 1) / tile); };
+    if (sizeof(T) == 2 && tiles(256) >= 192) q.tile = 256;
+    else if (tiles(128) >= (sizeof(T) == 2 ? 256 : 512)) q.tile = 128;
+    else q.tile = sizeof(T) == 2 && a.T > 64 ? 128 : 64;
+    b.tiles_t = (int)((a.T + q.tile - 1) / q.tile);
+    b.tiles_n = (p.N + q.tile - 1) / q.tile;
+    const int nk = (std::max(b.cu, b.cw) + 8 * E - 1) / (8 * E), all = std::max(1, b.tiles_t * b.tiles_n);
+    b.splits = q.tile == 256 || all >= 256 ? 1 : std::clamp(512 / all, 1, std::clamp(nk / 4, 1, 16));
+    if (b.splits > 1) {
+      b.ldp = b.tiles_n * q.tile;
+      b.part = ws.template take<float>((int64_t)b.splits * a.T * b.ldp);
+    } else {
+      b.G = copy(turned(p.G), p.N, p.N, (int)a.r, rp, (int)a.n);
+    }
+    return q;
   }
-  if (a.dB) {
-    const View<T> dBt{(T*)a.dB, a.r * a.N, a.b_trans ? a.r : 1, a.b_trans ? 1 : a.N};
-    const dim3 grid((unsigned)((a.N + 255) / 256), (unsigned)a.n, (unsigned)a.r);
-    hipLaunchKernelGGL(factor_grad_kernel<T>, grid, dim3(256), 0, s, dY, S, g, dBt, a.T, (int)a.N, (int)a.r);
+  template <bool KC, int BT, int BN, int WT, int WN>
+  void launch(const Big& b, hipStream_t s) {
+    const dim3 grid((unsigned)(b.tiles_t * b.tiles_n), (unsigned)b.splits);
+    if constexpr (BT < 256) {
+      if (b.splits > 1) {
+        hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, true>), grid, dim3(WT * WN * 64), 0, s, b);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, false>), grid, dim3(WT * WN * 64), 0, s, b);
+  }
+  void run_big(Plan& q, const Low& l, hipStream_t s) {
+    Big& b = q.b;
+    b.low = l.low, b.low_splits = l.splits;
+    auto shape = [&](auto kc) {
+      constexpr bool KC = decltype(kc)::value;
+      if (q.tile == 64) launch<KC, 64, 64, 2, 2>(b, s);
+      else if (q.tile == 128) launch<KC, 128, 128, 2, 2>(b, s);
+      else if constexpr (sizeof(T) == 2) launch<KC, 256, 256, 4, 2>(b, s);
+    };
+    if (q.kc) shape(std::true_type{});
+    else shape(std::false_type{});
+    if (b.splits > 1) {
+      Finish e{b.part, l.low, q.p.G, g, order.perm, b.N, (int)a.r, b.ldp, b.splits, l.splits, rp,
+               (b.N + 255) / 256, b.Y, b.ldy};
+      hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)(a.T * e.blocks)), dim3(256), 0, s, e);
+    }
+  }
+};
+
+template <class T>
+int product(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
+  const Problem p = product_of(a);
+  if (a.T == 0) return GELIM_OK;
+  if (a.T <= kFewRows) return few_product<T>(p, rows_of(a), (int)a.r, ws, s, run);
+  Many<T> m(a, ws);
+  const auto U = m.wide(p.U, p.ldu, a.T, p.C);
+  Low l = m.low_of(U, p.F, p.C);
+  auto q = m.big_of(p, U);
+  if (!run) return GELIM_OK;
+  m.run_prepare(s);
+  m.run_low(&l, 1, s);
+  m.run_big(q, l, s);
+  HIP_TRY(hipGetLastError());
+  return GELIM_OK;
+}
+
+template <class T>
+int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
+  const bool all = !run;  // the workspace is for all three
+  Many<T> m(a, ws);
+  const int K = (int)a.K, N = (int)a.N;
+  const auto X = m.wide(a.X, a.ldx, a.T, K), dY = m.wide(a.Y, a.ldy, a.T, N);
+  const Problem back = back_of(a);
+  typename Many<T>::Plan q{};
+  Low low[2];  // D, S
+  low[0] = m.low_of(dY, back.F, N);
+  low[1] = m.low_of(X, view_a(a), K);
+  if ((a.dX && a.T) || all) q = m.big_of(back, dY);
+  // the sides: dA = X^T D, dB^T = dY^T S
+  const int pcs = pieces(a.T, a.n, a.index != nullptr, kGradRows);
+  TurnPair tp{};
+  OuterPair op{};
+  SumPair sp{};
+  tp.rows = op.rows = sp.rows = m.g, tp.order = op.order = sp.order = m.order;
+  tp.rp = op.rp = sp.rp = m.rp, sp.r = (int)a.r, op.pieces = pcs;
+  int sides = 0;
+  unsigned outer_groups = 0, sum_groups = 0;
+  for (int k = 0; k < 2; ++k) {
+    if (!(k ? a.dB : a.dA) && !all) continue;
+    const auto& U = k ? dY : X;
+    const int cols = k ? N : K;
+    constexpr int kHalves = sizeof(T) == 2 ? 2 : 1;
+    Turn& t = tp.p[sides];
+    Outer& o = op.p[sides];
+    Sum& u = sp.p[sides];
+    ++sides;
+    t.low = low[k].low, t.splits = low[k].splits;
+    t.out = ws.take<T>((int64_t)pcs * kHalves * m.rp * kGradRows);
+    t.back = ws.take<float>(pcs);
+    o.U = U.p, o.V = t.out, o.ldu = U.ld, o.cu = U.cols;
+    o.blocks = (U.cols + 64 * Mma<T>::kE - 1) / (64 * Mma<T>::kE);
+    o.ldp = (int)up(U.cols, 16 * Mma<T>::kE);
+    o.part = ws.take<float>((int64_t)pcs * m.rp * o.ldp);
+    u.part = o.part, u.back = t.back, u.out = k ? a.dB : a.dA, u.cols = cols, u.ldp = o.ldp;
+    u.as = (int64_t)a.r * cols;
+    const bool along = k ? !a.b_trans : a.a_trans;  // columns side by side
+    u.cs = along ? 1 : a.r, u.rs = along ? cols : 1;
+    u.blocks = (int)((cols + 63) / 64 * ((a.r + 15) / 16));
+    outer_groups = std::max(outer_groups, (unsigned)(pcs * o.blocks));
+    sum_groups = std::max(sum_groups, (unsigned)u.blocks);
+  }
+  if (!run) return GELIM_OK;
+  m.run_prepare(s);
+  if (a.T) {
+    const bool need_d = a.dX || a.dA, need_s = a.dB != nullptr;
+    m.run_low(need_d ? low : low + 1, need_d + need_s, s);
+    if (a.dX) m.run_big(q, low[0], s);
+  }
+  if (sides) {
+    if (a.T) {
+      hipLaunchKernelGGL(turn_kernel<T>, dim3((unsigned)pcs, (unsigned)sides), dim3(256), 0, s, tp);
+      const int per = std::min(m.rb, 4);
+      const dim3 grid(outer_groups, (unsigned)sides, (unsigned)(m.rb / per));
+      if (per == 1) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, dim3(256), 0, s, op);
+      else if (per == 2) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, dim3(256), 0, s, op);
+      else hipLaunchKernelGGL((outer_kernel<T, 4>), grid, dim3(256), 0, s, op);
+    }
+    hipLaunchKernelGGL(sum_kernel<T>, dim3(sum_groups, (unsigned)sides, (unsigned)std::min<int64_t>(a.n, 4096)),
+                       dim3(256), 0, s, sp);
   }
   HIP_TRY(hipGetLastError());
   return GELIM_OK;
+}
+
+int run_or_count(const gelim_adapter_args& a, bool grad, Space& ws, hipStream_t s, bool run) {
+  if (grad) {
+    if (a.dtype == GELIM_T_F32) return gradient<float>(a, ws, s, run);
+    if (a.dtype == GELIM_T_BF16) return gradient<__bf16>(a, ws, s, run);
+    return gradient<_Float16>(a, ws, s, run);
+  }
+  if (a.dtype == GELIM_T_F32) return product<float>(a, ws, s, run);
+  if (a.dtype == GELIM_T_BF16) return product<__bf16>(a, ws, s, run);
+  return product<_Float16>(a, ws, s, run);
 }
 
 }  // namespace
@@ -181,20 +1311,20 @@ extern "C" int64_t gelim_adapter_args_layout(int32_t which) {
 }
 
 extern "C" int64_t gelim_adapter_workspace(const gelim_adapter_args* a, int grad) {
-  return (grad ? 8 : 4) * a->T * a->r;
+  GELIM_TRY(gelim::check_shape(*a));
+  gelim::Space ws{nullptr};
+  gelim::run_or_count(*a, grad != 0, ws, nullptr, false);
+  return ws.used;
 }
 
 extern "C" int gelim_adapter_matmul(const gelim_adapter_args* a, void* stream) {
   GELIM_TRY(gelim::check(*a, false));
-  if (a->T == 0) return GELIM_OK;
-  if (a->dtype == GELIM_T_F32) return gelim::product<float>(*a, (hipStream_t)stream);
-  if (a->dtype == GELIM_T_BF16) return gelim::product<__bf16>(*a, (hipStream_t)stream);
-  return gelim::product<_Float16>(*a, (hipStream_t)stream);
+  gelim::Space ws{(char*)a->ws};
+  return gelim::run_or_count(*a, false, ws, (hipStream_t)stream, true);
 }
 
 extern "C" int gelim_adapter_matmul_grad(const gelim_adapter_args* a, void* stream) {
   GELIM_TRY(gelim::check(*a, true));
-  if (a->dtype == GELIM_T_F32) return gelim::gradient<float>(*a, (hipStream_t)stream);
-  if (a->dtype == GELIM_T_BF16) return gelim::gradient<__bf16>(*a, (hipStream_t)stream);
-  return gelim::gradient<_Float16>(*a, (hipStream_t)stream);
+  gelim::Space ws{(char*)a->ws};
+  return gelim::run_or_count(*a, true, ws, (hipStream_t)stream, true);
 }

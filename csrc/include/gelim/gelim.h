@@ -274,6 +274,7 @@ int gelim_gpu_matmul_f32_ex(const float* dA, int64_t lda, const float* dB, int64
  * keeps anything; the results do not depend on the order of anything's run. */
 enum { GELIM_T_F32 = 0, GELIM_T_BF16 = 1, GELIM_T_F16 = 2 };
 #define GELIM_ADAPTER_MAX_RANK 256
+#define GELIM_ADAPTER_MAX_DIM ((1 << 30) - 64) /* T, K and N */
 typedef struct gelim_adapter_args {
   int64_t dtype, T, K, N, r, n;
   const void* X;

@@ -93,10 +93,10 @@ def _check(X, W, A, B, index, scale):
 @lru_cache(maxsize=4096)
 def _workspace_bytes(grad: bool, *layout) -> int:
     """What a call of these sizes and layouts needs."""
-    dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, odd = layout
+    dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, ldy, odd, indexed = layout
     # the addresses' low bits choose between aligned and unaligned loads, so they take the place of the addresses
-    args = _ARGS.pack(dtype, T, K, N, r, n, odd, ldx, odd, ldw, wt, 0, 0, lda, at, 0, 0, ldb, bt, 0, 0, 0.0,
-                      odd, 0, 0, 0, 0, 0, 0, 0)
+    args = _ARGS.pack(dtype, T, K, N, r, n, odd, ldx, odd, ldw, wt, 0, 0, lda, at, 0, 0, ldb, bt, indexed, 0, 0.0,
+                      odd, ldy, 0, 0, 0, 0, 0, 0)
     return _native.lib().gelim_adapter_workspace(args, grad)
 
 
@@ -115,7 +115,8 @@ def _call(grad, dev, T, K, N, n, r, X, W, A, B, index, scale, Y, dX=None, dA=Non
         index = index.contiguous()
     dtype = TYPES[X.dtype]
     xp, wp, yp = X.data_ptr(), W.data_ptr(), Y.data_ptr()
-    ws_bytes = _workspace_bytes(grad, dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, (xp | wp | yp) & 15)
+    ws_bytes = _workspace_bytes(grad, dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, ldy,
+                                (xp | wp | yp) & 15, index is not None)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     args = _ARGS.pack(dtype, T, K, N, r, n, xp, ldx, wp, ldw, wt, A.data_ptr(), A.stride(0), lda, at, B.data_ptr(),
                       B.stride(0), ldb, bt, 0 if index is None else index.data_ptr(),
