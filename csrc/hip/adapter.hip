@@ -72,6 +72,25 @@ struct Mma<float> {
   }
 };
 
+// The same over 32 rows and columns: lane l has row (column) l % 32 and, of a step of 2 kE values along the
+// sum, those from (l / 32) kE on.  In D it has column l % 32 and the rows 8 (r / 4) + 4 (l / 32) + r % 4.
+typedef float f16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f16 mma32(bf8 a, bf8 b, f16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16 mma32(h8 a, h8 b, f16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16 mma32(f4 a, f4 b, f16 c) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], c, 0, 0, 0);
+  return c;
+}
+
+template <class T>
+struct __attribute__((packed, aligned(sizeof(T)))) Four {
+  T v[4];
+};
 template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) Unaligned {
   typename Mma<T>::Frag v;
@@ -335,12 +354,9 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish a) {
     if (n < a.N) {
       const int have = min(4, a.N - n);
       if (a.G.cs == 1 && have == 4) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Four {
-          T v[4];
-        };
 #pragma unroll 4
         for (int j = wave; j < a.r; j += 4) {
-          const Four v = *(const Four*)(G + j * a.G.rs + n);
+          const Four<T> v = *(const Four<T>*)(G + j * a.G.rs + n);
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[e] += s[j] * (float)v.v[e];
         }
@@ -481,13 +497,18 @@ __global__ __launch_bounds__(1024) void prepare_kernel(Prepare p) {
   copy_tile<T>(p.copy[k], b - p.copy[k].first);
 }
 
-// low (split, place, rank) = U F_i, 32 places of one adapter by a workgroup, whose four waves cut the sum.
-// F is laid out as rp ranks x ldf along the sum, zeros behind C.
+// low (place, rank) = U F_i, 32 places of one adapter by a workgroup, whose waves cut the sum.
+// F is laid out as rp ranks x ldf along the sum, zeros behind C.  Bound by
+// reading U and, for every 32 rows, F_i: each wave keeps several steps' loads in flight.
+// 16-bit types: also as the sum of two values of the type, 8 ranks' upper and then lower parts side by side, for
+// the matrix units of the large product.  One value's rounding alone would be as large as the
+// result's.  fp16: a row is first brought to below 2^14 by a power of two (`by`), as it may be beyond the type's range.
 struct Low {
   const void *U, *F;
   int64_t ldu;
-  float* low;
-  int cu, ldf, splits, pieces;  // cu: values in a row of U, a multiple of 16 bytes
+  float *low, *by;
+  void* split;
+  int cu, ldf, pieces;  // cu: values in a row of U, a multiple of 16 bytes
 };
 struct LowPair {
   Low p[2];
@@ -495,17 +516,27 @@ struct LowPair {
   Order order;
 };
 constexpr int kLowRows = 32;
+constexpr int low_waves(int rank_blocks) { return rank_blocks <= 8 ? 16 : 8; }
+
+// v as upper and lower part of the type; the lower is 0 beside an infinity or NaN
+template <class T>
+__device__ __forceinline__ void two_parts(float v, T& hi, T& lo) {
+  hi = (T)v;
+  lo = fabsf((float)hi) <= 3.4e38f ? (T)(v - (float)hi) : (T)0.f;
+}
+// a power of two that brings fp16's `most` to [2^13, 2^14)
+__device__ __forceinline__ int to_fp16_range(float most) {
+  return most > 0.f ? min(max(13 - ilogbf(most), -100), 100) : 0;
+}
 
 template <class T, int RB>
-__global__ __launch_bounds__(256) void low_kernel(LowPair both) {
+__global__ __launch_bounds__(low_waves(RB) * 64) void low_kernel(LowPair both) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int E = M::kE, rp = 16 * RB;
-  __shared__ f4 lds[3][RB * 2][64];
+  constexpr int E = M::kE, rp = 16 * RB, kWaves = low_waves(RB);
+  __shared__ f4 lds[kWaves / 2][RB * 2][64];
   const Low& a = both.p[blockIdx.y];
-  const int split = blockIdx.x / a.pieces;
-  if (split >= a.splits) return;
-  const Piece pc = piece_of(both.order, both.rows, blockIdx.x % a.pieces, kLowRows);
+  const Piece pc = piece_of(both.order, both.rows, blockIdx.x, kLowRows);
   if (pc.count == 0) return;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
   const T* u[2];
@@ -513,39 +544,83 @@ __global__ __launch_bounds__(256) void low_kernel(LowPair both) {
   for (int t = 0; t < 2; ++t)
     u[t] = (const T*)a.U + row_at(both.order, pc.begin + min(t * 16 + l16, pc.count - 1)) * a.ldu;
   const T* f = (const T*)a.F + ((int64_t)pc.adapter * rp + l16) * a.ldf;
-  const int steps = (a.cu + M::kStep - 1) / M::kStep, parts = a.splits * 4, part = split * 4 + wave;
-  const int s0 = (int)((int64_t)steps * part / parts), s1 = (int)((int64_t)steps * (part + 1) / parts);
+  const int steps = (a.cu + M::kStep - 1) / M::kStep;
+  const int s0 = (int)((int64_t)steps * wave / kWaves), s1 = (int)((int64_t)steps * (wave + 1) / kWaves);
   f4 acc[RB][2] = {};
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) {
-    const int k = s * M::kStep + g * E;
-    Frag x[2], w[RB];
+  constexpr int kFlight = RB <= 2 ? 4 : RB == 4 ? 2 : 1;  // by the registers that a wave may have
+  for (int s = s0; s < s1; s += kFlight) {
+    Frag x[kFlight][2], w[kFlight][RB];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      x[t] = Frag{};
-      if (k < a.cu) x[t] = *(const Frag*)(u[t] + k);
+    for (int q = 0; q < kFlight; ++q) {
+      // a step behind the last one repeats it, with zeros for U
+      const int k = min(s + q, s1 - 1) * M::kStep + g * E;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        x[q][t] = Frag{};
+        if (k < a.cu && s + q < s1) x[q][t] = *(const Frag*)(u[t] + k);
+      }
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        w[q][j] = Frag{};
+        if (s + q < s1) w[q][j] = *(const Frag*)(f + (int64_t)j * 16 * a.ldf + k);
+      }
     }
 #pragma unroll
-    for (int j = 0; j < RB; ++j) w[j] = *(const Frag*)(f + (int64_t)j * 16 * a.ldf + k);
+    for (int q = 0; q < kFlight; ++q)
 #pragma unroll
-    for (int j = 0; j < RB; ++j)
+      for (int j = 0; j < RB; ++j)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) acc[j][t] = M::mma(w[j], x[t], acc[j][t]);
+        for (int t = 0; t < 2; ++t) acc[j][t] = M::mma(w[q][j], x[q][t], acc[j][t]);
   }
-  if (wave)
 #pragma unroll
-    for (int j = 0; j < RB; ++j)
+  for (int half = kWaves / 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) lds[wave - 1][j * 2 + t][lane] = acc[j][t];
-  __syncthreads();
+      for (int j = 0; j < RB; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) lds[wave - half][j * 2 + t][lane] = acc[j][t];
+    __syncthreads();
+    if (wave < half)
+#pragma unroll
+      for (int j = 0; j < RB; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) acc[j][t] += lds[wave][j * 2 + t][lane];
+    __syncthreads();
+  }
   if (wave) return;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    if (t * 16 + l16 >= pc.count) continue;
-    float* out = a.low + ((int64_t)split * both.rows.T + pc.begin + t * 16 + l16) * rp + g * 4;
+    const bool in = t * 16 + l16 < pc.count;
+    const int64_t at = pc.begin + t * 16 + l16;
+    float by = 1.f;
+    if constexpr (std::is_same_v<T, _Float16>) {
+      float most = 0.f;
 #pragma unroll
-    for (int j = 0; j < RB; ++j)
-      *(f4*)(out + j * 16) = acc[j][t] + lds[0][j * 2 + t][lane] + lds[1][j * 2 + t][lane] + lds[2][j * 2 + t][lane];
+      for (int j = 0; j < RB; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = fabsf(acc[j][t][i]);
+          if (v > most && v <= 3.4e38f) most = v;
+        }
+      most = fmaxf(most, __shfl_xor(most, 16, 64));
+      most = fmaxf(most, __shfl_xor(most, 32, 64));
+      const int e = to_fp16_range(most);
+      by = ldexpf(1.f, e);
+      if (in && g == 0) a.by[at] = ldexpf(1.f, -e);
+    }
+    if (!in) continue;
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+      *(f4*)(a.low + at * rp + j * 16 + g * 4) = acc[j][t];
+      if constexpr (sizeof(T) == 2) {
+        Four<T> hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) two_parts(acc[j][t][i] * by, hi.v[i], lo.v[i]);
+        T* out = (T*)a.split + at * 2 * rp + (j * 2 + g / 2) * 16 + g % 2 * 4;
+        *(Four<T>*)out = hi;
+        *(Four<T>*)(out + 8) = lo;
+      }
+    }
   }
 }
 
@@ -556,8 +631,9 @@ struct Big {
   int cu, cw;  // values of a row of U / of the sum in W that exist (W_KC: multiples of 16 bytes); zeros behind
   Rows rows;
   Order order;
-  const float* low;
-  int N, nw, r, rp, low_splits, splits, tiles_t, tiles_n;  // nw: columns of W as stored
+  const float *low, *by;
+  const void* split;
+  int N, nw, r, rp, splits, tiles_t, tiles_n;  // nw: columns of W as stored
   void* Y;
   int64_t ldy;
   float* part;  // splits > 1: partial sums instead of Y
@@ -566,40 +642,47 @@ struct Big {
 
 __device__ const uint4 g_zeros[1] = {};
 
-// 16 bytes per lane from global memory to LDS, at base + 16 lane
-__device__ __forceinline__ void to_lds(const void* from, void* base) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                   (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+// 16 bytes per lane from global memory to LDS, at `at` + 16 lane; s_waitcnt vmcnt waits for it.  In assembly, as
+// the compiler waits for all such loads before a transposing read of LDS, whatever that reads.
+__device__ __forceinline__ void to_lds(const void* from, unsigned at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from)
+               : "memory", "m0");
+}
+template <class T>
+__device__ __forceinline__ unsigned lds_address(T* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)p;
 }
 
 // Tiles in LDS, as chunks of 16 bytes.  Operands whose sum runs along memory:
-// rows of 8 chunks, chunk c of row i at place c ^ (i / 2 % 8), so that the 16
+// rows of 8 chunks, chunk c of row i at place c ^ (i / 2 % 8), so that any 16
 // rows a fragment reads lie in 16 different places of 256 bytes.  Otherwise rows
-// (of the sum) of all columns; the 32 (fp32: 64) bytes that a read takes from a
+// (of the sum) of all columns; the 32 (fp32: 128) bytes that a read takes from a
 // row are moved by the row's number, so that the rows of one read fall on different banks.
 template <class T, int kRowChunks>
 __device__ __forceinline__ int swap_columns(int k) {  // in chunks
   if constexpr (sizeof(T) == 2) return ((k & 3) | (k >> 1 & 4)) * 2 % kRowChunks;
-  else return (k >> 2 & 3) * 4 % kRowChunks;
+  else return (k >> 2 & 1) * 8 % kRowChunks;
 }
 
-template <class T, bool W_KC, int BT, int BN, int WT, int WN, bool SPLIT>
-__global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
-  using M = Mma<T>;
-  using Frag = typename M::Frag;
-  constexpr int E = M::kE, BK = 8 * E, kThreads = WT * WN * 64, kWaves = WT * WN;
-  constexpr int TT = BT / WT / 16, TN = BN / WN / 16;
-  constexpr int kLoadU = BT * 8 / kThreads, kLoadW = BN * 8 / kThreads;
+// Four waves, each a quarter of the tile in blocks of 32 x 32.  Two tiles in
+// LDS and two sets of fragments in registers: while one quarter of a tile is
+// multiplied the next is read; when the last quarter is in registers the
+// tile's place is loaded again, a whole tile's time before the barrier that waits for it.
+template <class T, bool W_KC, int BT, int BN, bool SPLIT>
+__global__ __launch_bounds__(256, 1) void big_kernel(Big a) {
+  using Frag = typename Mma<T>::Frag;
+  constexpr int E = Mma<T>::kE, BK = 8 * E;
+  constexpr int TT = BT / 64, TN = BN / 64;
+  constexpr int kLoadU = BT / 32, kLoadW = BN / 32;
   constexpr int kRowChunks = BN / E;  // chunks in a row of W's tile if not W_KC
-  static_assert(kLoadU * kThreads == BT * 8 && kLoadW * kThreads == BN * 8, "tile and threads");
-  __shared__ __attribute__((aligned(16))) T us[2][BT * BK], ws[2][BN * BK];
+  __shared__ __attribute__((aligned(16))) T us0[BT * BK], us1[BT * BK], ws0[BN * BK], ws1[BN * BK];
 
   // workgroups go to the 8 XCDs in turn: each XCD gets neighbouring tiles, which share operands in its L2
   const int tiles = a.tiles_t * a.tiles_n, q = tiles / 8, rem = tiles % 8, xcd = blockIdx.x % 8;
   const int tile = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + blockIdx.x / 8;
   const int t0 = tile / a.tiles_n * BT, n0 = tile % a.tiles_n * BN;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
-  const int wt = wave / WN * (BT / WT), wn = wave % WN * (BN / WN);
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l32 = lane % 32, half = lane / 32;
+  const int wt = wave / 2 * (BT / 2), wn = wave % 2 * (BN / 2);
 
   const int nk = (max(a.cu, a.cw) + BK - 1) / BK;
   const int k0 = SPLIT ? (int)((int64_t)nk * blockIdx.y / a.splits) : 0;
@@ -622,156 +705,199 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
       wp[q] = (const T*)a.W + (int64_t)min(n0 + i, a.N - 1) * a.ldw + wk[q];
     } else {
       const int place = (wave * kLoadW + q) * 64 + lane, k = place / kRowChunks;
-      const int n = n0 + ((place % kRowChunks) ^ swap_columns<T, kRowChunks>(k)) * E;
-      wk[q] = n < a.nw ? k : INT_MAX / 2;
+      const int n = min(n0 + ((place % kRowChunks) ^ swap_columns<T, kRowChunks>(k)) * E, a.nw - E);
+      wk[q] = k;
       wp[q] = (const T*)a.W + (int64_t)k * a.ldw + n;
     }
   }
   const int64_t w_step = W_KC ? BK : BK * a.ldw;
-  auto load = [&](int kt, int buf) {
+  // the q-th load of a tile; guard: with zeros behind the sum's end, also for tiles that nothing uses
+  auto load = [&](auto guard, int kt, T* us, T* ws, int q) {
     const int k = kt * BK;
-#pragma unroll
-    for (int q = 0; q < kLoadU; ++q)
-      to_lds(k + uk[q] < a.cu ? (const void*)(up[q] + k) : g_zeros, &us[buf][(wave * kLoadU + q) * 64 * E]);
-#pragma unroll
-    for (int q = 0; q < kLoadW; ++q)
-      to_lds(k + wk[q] < a.cw ? (const void*)(wp[q] + kt * w_step) : g_zeros, &ws[buf][(wave * kLoadW + q) * 64 * E]);
+    const void* from;
+    unsigned to;
+    if (q < kLoadU) {
+      from = up[q] + k;
+      if (decltype(guard)::value && k + uk[q] >= a.cu) from = g_zeros;
+      to = lds_address(us + (wave * kLoadU + q) * 64 * E);
+    } else {
+      q -= kLoadU;
+      from = wp[q] + kt * w_step;
+      if (decltype(guard)::value && k + wk[q] >= a.cw) from = g_zeros;
+      to = lds_address(ws + (wave * kLoadW + q) * 64 * E);
+    }
+    to_lds(from, __builtin_amdgcn_readfirstlane(to));
   };
 
-  f4 acc[TN][TT] = {};
-  auto compute = [&](int buf) {
+  f16 acc[TN][TT] = {};
+  struct Frags {
+    Frag x[TT], w[TN];
+  };
+  // the q-th fragment of a quarter
+  auto read = [&](const T* us, const T* ws, int part, Frags& f, int q) {
+    if (q < TT) {
+      const int i = wt + q * 32 + l32;
+      f.x[q] = *(const Frag*)&us[i * BK + ((part * 2 + half) ^ (i >> 1 & 7)) * E];
+      return;
+    }
+    const int j = q - TT;
+    if constexpr (W_KC) {
+      const int i = wn + j * 32 + l32;
+      f.w[j] = *(const Frag*)&ws[i * BK + ((part * 2 + half) ^ (i >> 1 & 7)) * E];
+    } else if constexpr (sizeof(T) == 2) {
+      // 16 lanes read 4 rows (of the sum) x 16 columns, 8 bytes each, and get their column's 4 values
+      s8 v;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      Frag x[TT], w[TN];
+      for (int h = 0; h < 2; ++h) {
+        const int k = part * 16 + half * 8 + h * 4 + lane % 16 / 4;
+        const int chunk = ((wn + j * 32) / 8 + l32 / 16 * 2 + lane % 4 / 2) ^ swap_columns<T, kRowChunks>(k);
+        const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s4*)&ws[k * BN + chunk * 8 + lane % 2 * 4]);
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const int i = wt + t * 16 + l16;
-        x[t] = *(const Frag*)&us[buf][i * BK + ((kk * 4 + g) ^ (i >> 1 & 7)) * E];
+        for (int e = 0; e < 4; ++e) v[h * 4 + e] = r[e];
       }
+      f.w[j] = __builtin_bit_cast(Frag, v);
+    } else {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        if constexpr (W_KC) {
-          const int i = wn + j * 16 + l16;
-          w[j] = *(const Frag*)&ws[buf][i * BK + ((kk * 4 + g) ^ (i >> 1 & 7)) * E];
-        } else if constexpr (sizeof(T) == 2) {
-          // 16 lanes read 4 rows (of the sum) x 16 columns, 8 bytes each, and get their column's 4 values
-          s8 v;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k = kk * 32 + g * 8 + h * 4 + l16 / 4;
-            const int chunk = ((wn + j * 16) / 8 + (l16 % 4) / 2) ^ swap_columns<T, kRowChunks>(k);
-            const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s4*)&ws[buf][k * BN + chunk * 8 + l16 % 2 * 4]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[h * 4 + e] = r[e];
-          }
-          w[j] = __builtin_bit_cast(Frag, v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = kk * 16 + g * 4 + e, n = wn + j * 16 + l16;
-            w[j][e] = ws[buf][k * BN + ((n / E) ^ swap_columns<T, kRowChunks>(k)) * E + n % E];
-          }
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int k = part * 8 + half * 4 + e, n = wn + j * 32 + l32;
+        f.w[j][e] = ws[k * BN + ((n / E) ^ swap_columns<T, kRowChunks>(k)) * E + n % E];
       }
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int t = 0; t < TT; ++t) acc[j][t] = M::mma(w[j], x[t], acc[j][t]);
     }
   };
-
-  if (k0 < k1) load(k0, 0);
-  __syncthreads();
-  for (int kt = k0; kt < k1; ++kt) {
-    const int buf = (kt - k0) & 1;
-    if (kt + 1 < k1) load(kt + 1, buf ^ 1);
-    compute(buf);
+  // A quarter: `now` is multiplied; in between, in this order, quarter `part` is read into `next` in the first
+  // half and, with kLoads, a tile is loaded.
+  constexpr int kMma = TT * TN, kReads = TT + TN, kLoads = kLoadU + kLoadW;
+  auto quarter = [&](const Frags& now, const T* us, const T* ws, int part, Frags& next, auto loads, auto guard, int kt,
+                     T* us_to, T* ws_to) {
+#pragma unroll
+    for (int m = 0; m < kMma; ++m) {
+      constexpr int kSpan = (kMma + 1) / 2;
+#pragma unroll
+      for (int q = 0; q < kReads; ++q)
+        if (q * kSpan / kReads == m) read(us, ws, part, next, q);
+      if constexpr (decltype(loads)::value)
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q)
+          if (q * kMma / kLoads == m) load(guard, kt, us_to, ws_to, q);
+      acc[m / TT][m % TT] = mma32(now.w[m / TT], now.x[m % TT], acc[m / TT][m % TT]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  Frags f0, f1;
+  // one tile from its place in LDS; its first quarter is in f0, and the next tile's will be
+  auto step = [&](auto guard, int kt, T* us, T* ws, const T* us_next, const T* ws_next) {
+    constexpr std::false_type no{};
+    quarter(f0, us, ws, 1, f1, no, no, 0, us, ws);
+    quarter(f1, us, ws, 2, f0, no, no, 0, us, ws);
+    quarter(f0, us, ws, 3, f1, no, no, 0, us, ws);
+    // this wave's loads have landed (vmcnt 0) and its reads are done, then everybody's
+    __builtin_amdgcn_s_waitcnt(0x0070);
     __syncthreads();
+    quarter(f1, us_next, ws_next, 0, f0, std::true_type{}, guard, kt + 2, us, ws);
+  };
+#pragma unroll
+  for (int q = 0; q < kLoads; ++q) load(std::true_type{}, k0, us0, ws0, q);
+#pragma unroll
+  for (int q = 0; q < kLoads; ++q) load(std::true_type{}, k0 + 1, us1, ws1, q);
+  if constexpr (!SPLIT) {
+    // The accumulators begin with s_i (U F_i) G_i, while the first tiles load: for each adapter among 32 rows the
+    // product of all of them, kept where it is theirs.
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const int at = t0 + wt + t * 32 + l32;
+      const int64_t place = min(at, a.rows.T - 1);
+      const int mine = at < a.rows.T ? adapter_of(a.rows, row_at(a.order, place)) : -1;
+      const bool has = mine >= 0 && mine < a.rows.n;
+      // U F_i comes as two values of the type (fp32: itself), so 8 ranks are one step.  All loads of kBatch
+      // steps come before their products: nothing else hides their latency here.
+      constexpr int kBatch = 4;
+      uint64_t left = __ballot(has);
+      const Frag* x_at = sizeof(T) == 2 ? (const Frag*)((const T*)a.split + place * 2 * a.rp) + half
+                                        : (const Frag*)(a.low + place * a.rp) + half;
+      while (left) {
+        const int cur = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+        left &= ~__ballot(mine == cur);
+        f16 d[TN] = {};
+        for (int b = 0; b < a.r; b += 8 * kBatch) {
+          Frag x[kBatch], w[TN][kBatch];
+#pragma unroll
+          for (int q = 0; q < kBatch; ++q) {
+            const bool more = b + q * 8 < a.rp;
+            x[q] = Frag{};
+            if (more && has) x[q] = x_at[(b / 8 + q) * 2];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+              const int n = min(n0 + wn + j * 32 + l32, a.N - 1);
+              w[j][q] = Frag{};
+              if (more)
+                w[j][q] = *(const Frag*)((const T*)a.G + ((int64_t)cur * a.N + n) * a.rp + b + q * 8 +
+                                         (sizeof(T) == 2 ? 0 : half * 4));
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < kBatch; ++q)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) d[j] = mma32(w[j][q], x[q], d[j]);
+        }
+        float f = scale_of(a.rows, cur);
+        if constexpr (std::is_same_v<T, _Float16>) f *= has ? a.by[place] : 0.f;
+        if (mine == cur)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[j][t] = f * d[j];
+      }
+    }
   }
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kReads; ++q) read(us0, ws0, 0, f0, q);
+  const int whole = min(k1, min(a.cu, a.cw) / BK);  // tiles without a part behind the end
+  int kt = k0;
+  for (; kt + 3 < whole; kt += 2) {
+    step(std::false_type{}, kt, us0, ws0, us1, ws1);
+    step(std::false_type{}, kt + 1, us1, ws1, us0, ws0);
+  }
+  for (; kt < k1; kt += 2) {
+    step(std::true_type{}, kt, us0, ws0, us1, ws1);
+    if (kt + 1 < k1) step(std::true_type{}, kt + 1, us1, ws1, us0, ws0);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);  // no load may land in LDS that is not this workgroup's any more
 
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
-    const int at = t0 + wt + t * 16 + l16;
+    const int at = t0 + wt + t * 32 + l32;
     if constexpr (SPLIT) {
       if (at < a.rows.T) {
-        float* out = a.part + ((int64_t)blockIdx.y * a.rows.T + at) * a.ldp + n0 + wn + g * 4;
+        float* out = a.part + ((int64_t)blockIdx.y * a.rows.T + at) * a.ldp + n0 + wn + half * 4;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) *(f4*)(out + j * 16) = acc[j][t];
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; r += 4)
+            *(f4*)(out + j * 32 + r * 2) = f4{acc[j][t][r], acc[j][t][r + 1], acc[j][t][r + 2], acc[j][t][r + 3]};
       }
     } else {
       const bool in = at < a.rows.T;
       const int64_t row = row_at(a.order, min(at, a.rows.T - 1));
       const int mine = in ? adapter_of(a.rows, row) : -1;
       const bool has = mine >= 0 && mine < a.rows.n;
-      // s_i (U F_i) G_i: for each adapter among these 16 rows the product of all of them, kept where it is theirs
-      uint64_t left = __ballot(has);
-      if (left) {
-        // 16-bit types: U F_i as the sum of two values of the type, side by side along the sum (16 ranks are a step
-        // of 32); with one, its rounding alone would be as large as the result's.  fp16: first brought
-        // to below 2^14 by a power of two, as it may be beyond the type's range.
-        float up_by = 1.f, down_by = 1.f;
-        const float* lo = a.low + (int64_t)min(at, a.rows.T - 1) * a.rp;
-        auto low_at = [&](int j) {
-          float v = 0.f;
-          for (int p = 0; p < a.low_splits; ++p) v += lo[(int64_t)p * a.rows.T * a.rp + j];
-          return v;
-        };
-        if constexpr (std::is_same_v<T, _Float16>) {
-          float most = 0.f;
-          for (int j = g; j < a.rp; j += 4) {
-            const float v = has ? fabsf(low_at(j)) : 0.f;
-            if (v > most && v <= 3.4e38f) most = v;
-          }
-          most = fmaxf(most, __shfl_xor(most, 16, 64));
-          most = fmaxf(most, __shfl_xor(most, 32, 64));
-          if (most > 0.f) {
-            const int e = min(max(14 - ilogbf(most) - 1, -100), 100);
-            down_by = ldexpf(1.f, e);
-            up_by = ldexpf(1.f, -e);
-          }
-        }
-        while (left) {
-          const int cur = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-          left &= ~__ballot(mine == cur);
-          f4 d[TN] = {};
-          const T* G = (const T*)a.G + (int64_t)cur * a.N * a.rp;
-          for (int b = 0; b < a.rp / 16; ++b) {
-            const int j0 = b * 16 + (sizeof(T) == 2 ? (g & 1) * 8 : g * 4);
-            Frag x;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const float v = has ? low_at(j0 + e) * down_by : 0.f;
-              if constexpr (sizeof(T) == 2) {
-                const T hi = (T)v;
-                const float rest = v - (float)hi;
-                x[e] = g < 2 ? hi : fabsf((float)hi) <= 3.4e38f ? (T)rest : (T)0.f;
-              } else {
-                x[e] = v;
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-              const Frag w = *(const Frag*)(G + (int64_t)min(n0 + wn + j * 16 + l16, a.N - 1) * a.rp + j0);
-              d[j] = M::mma(w, x, d[j]);
-            }
-          }
-          const float f = scale_of(a.rows, cur) * up_by;
-          if (mine == cur)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[j][t] += f * d[j];
-        }
-      }
       if (!in) continue;
       T* out = (T*)a.Y + row * a.ldy;
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const int n = n0 + wn + j * 16 + g * 4;
-        f4 v = acc[j][t];
+        f16 v = acc[j][t];
         if (!has && mine != -1) v = v * __builtin_nanf("");
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < a.N) out[n + e] = (T)v[e];
+        for (int r = 0; r < 16; r += 4) {
+          const int n = n0 + wn + j * 32 + r * 2 + half * 4;
+          if (n + 4 <= a.N) {
+            *(Four<T>*)(out + n) = Four<T>{(T)v[r], (T)v[r + 1], (T)v[r + 2], (T)v[r + 3]};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < a.N) out[n + e] = (T)v[r + e];
+          }
+        }
       }
     }
   }
@@ -785,7 +911,6 @@ struct Turn {
   const float* low;
   void* out;    // piece, half (16-bit types), rank, place
   float* back;  // of each piece, the factor that undoes the power of two
-  int splits;
 };
 struct TurnPair {
   Turn p[2];
@@ -802,12 +927,7 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnPair both) {
   const Piece pc = piece_of(both.order, both.rows, blockIdx.x, kGradRows);
   if (pc.count == 0) return;
   const int t = threadIdx.x % kGradRows;
-  auto value = [&](int j) {
-    float v = 0.f;
-    if (t < pc.count)
-      for (int p = 0; p < a.splits; ++p) v += a.low[((int64_t)p * both.rows.T + pc.begin + t) * rp + j];
-    return v;
-  };
+  auto value = [&](int j) { return t < pc.count ? a.low[(int64_t)(pc.begin + t) * rp + j] : 0.f; };
   float by = 1.f, back = 1.f;
   if constexpr (std::is_same_v<T, _Float16>) {
     float most = 0.f;
@@ -820,20 +940,18 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnPair both) {
     if (threadIdx.x % 64 == 0) wave_most[threadIdx.x / 64] = most;
     __syncthreads();
     most = fmaxf(fmaxf(wave_most[0], wave_most[1]), fmaxf(wave_most[2], wave_most[3]));
-    if (most > 0.f) {
-      const int e = min(max(13 - ilogbf(most), -100), 100);
-      by = ldexpf(1.f, e);
-      back = ldexpf(1.f, -e);
-    }
+    const int e = to_fp16_range(most);
+    by = ldexpf(1.f, e);
+    back = ldexpf(1.f, -e);
   }
   if (threadIdx.x == 0) a.back[blockIdx.x] = back;
   constexpr int kHalves = sizeof(T) == 2 ? 2 : 1;
   T* out = (T*)a.out + (int64_t)blockIdx.x * kHalves * rp * kGradRows + t;
   for (int j = threadIdx.x / kGradRows; j < rp; j += 256 / kGradRows) {
-    const float v = value(j) * by;
-    const T hi = (T)v;
+    T hi, lo;
+    two_parts(value(j) * by, hi, lo);
     out[j * kGradRows] = hi;
-    if constexpr (kHalves == 2) out[(rp + j) * kGradRows] = fabsf((float)hi) <= 3.4e38f ? (T)(v - (float)hi) : (T)0.f;
+    if constexpr (kHalves == 2) out[(rp + j) * kGradRows] = lo;
   }
 }
 
@@ -1106,9 +1224,9 @@ struct Many {
     l.F = copy(turned(F), rp, (int)a.r, C, l.ldf, (int)a.n);
     l.U = U.p, l.ldu = U.ld, l.cu = U.cols;
     l.pieces = pieces(a.T, a.n, a.index != nullptr, kLowRows);
-    const int steps = (C + Mma<T>::kStep - 1) / Mma<T>::kStep;
-    l.splits = (int)std::clamp<int64_t>(256 * kLowRows / std::max<int64_t>(a.T, 1), 1, std::clamp(steps / 8, 1, 8));
-    l.low = ws.template take<float>((int64_t)l.splits * a.T * rp);
+    l.low = ws.template take<float>(a.T * rp);
+    if (sizeof(T) == 2) l.split = ws.template take<T>(a.T * 2 * rp);
+    if (std::is_same_v<T, _Float16>) l.by = ws.template take<float>(a.T);
     return l;
   }
   int run_prepare(hipStream_t s) {
@@ -1121,15 +1239,15 @@ struct Many {
     unsigned most = 0;
     for (int k = 0; k < count; ++k) {
       both.p[k] = l[k];
-      most = std::max(most, (unsigned)(l[k].pieces * l[k].splits));
+      most = std::max(most, (unsigned)l[k].pieces);
     }
     const dim3 grid(most, (unsigned)count);
     switch (rb) {
-      case 1: hipLaunchKernelGGL((low_kernel<T, 1>), grid, dim3(256), 0, s, both); break;
-      case 2: hipLaunchKernelGGL((low_kernel<T, 2>), grid, dim3(256), 0, s, both); break;
-      case 4: hipLaunchKernelGGL((low_kernel<T, 4>), grid, dim3(256), 0, s, both); break;
-      case 8: hipLaunchKernelGGL((low_kernel<T, 8>), grid, dim3(256), 0, s, both); break;
-      default: hipLaunchKernelGGL((low_kernel<T, 16>), grid, dim3(256), 0, s, both);
+      case 1: hipLaunchKernelGGL((low_kernel<T, 1>), grid, dim3(low_waves(1) * 64), 0, s, both); break;
+      case 2: hipLaunchKernelGGL((low_kernel<T, 2>), grid, dim3(low_waves(2) * 64), 0, s, both); break;
+      case 4: hipLaunchKernelGGL((low_kernel<T, 4>), grid, dim3(low_waves(4) * 64), 0, s, both); break;
+      case 8: hipLaunchKernelGGL((low_kernel<T, 8>), grid, dim3(low_waves(8) * 64), 0, s, both); break;
+      default: hipLaunchKernelGGL((low_kernel<T, 16>), grid, dim3(low_waves(16) * 64), 0, s, both);
     }
   }
 
@@ -1139,7 +1257,6 @@ struct Many {
     bool kc;
     int tile;
     Problem p;
-    int low_splits;
   };
   Plan big_of(const Problem& p, const Wide& U) {
     Plan q{};
@@ -1171,30 +1288,30 @@ struct Many {
     }
     return q;
   }
-  template <bool KC, int BT, int BN, int WT, int WN>
+  template <bool KC, int BT, int BN>
   void launch(const Big& b, hipStream_t s) {
     const dim3 grid((unsigned)(b.tiles_t * b.tiles_n), (unsigned)b.splits);
     if constexpr (BT < 256) {
       if (b.splits > 1) {
-        hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, true>), grid, dim3(WT * WN * 64), 0, s, b);
+        hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, true>), grid, dim3(256), 0, s, b);
         return;
       }
     }
-    hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, false>), grid, dim3(WT * WN * 64), 0, s, b);
+    hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, false>), grid, dim3(256), 0, s, b);
   }
   void run_big(Plan& q, const Low& l, hipStream_t s) {
     Big& b = q.b;
-    b.low = l.low, b.low_splits = l.splits;
+    b.low = l.low, b.by = l.by, b.split = l.split;
     auto shape = [&](auto kc) {
       constexpr bool KC = decltype(kc)::value;
-      if (q.tile == 64) launch<KC, 64, 64, 2, 2>(b, s);
-      else if (q.tile == 128) launch<KC, 128, 128, 2, 2>(b, s);
-      else if constexpr (sizeof(T) == 2) launch<KC, 256, 256, 4, 2>(b, s);
+      if (q.tile == 64) launch<KC, 64, 64>(b, s);
+      else if (q.tile == 128) launch<KC, 128, 128>(b, s);
+      else if constexpr (sizeof(T) == 2) launch<KC, 256, 256>(b, s);
     };
     if (q.kc) shape(std::true_type{});
     else shape(std::false_type{});
     if (b.splits > 1) {
-      Finish e{b.part, l.low, q.p.G, g, order.perm, b.N, (int)a.r, b.ldp, b.splits, l.splits, rp,
+      Finish e{b.part, l.low, q.p.G, g, order.perm, b.N, (int)a.r, b.ldp, b.splits, 1, rp,
                (b.N + 255) / 256, b.Y, b.ldy};
       hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)(a.T * e.blocks)), dim3(256), 0, s, e);
     }
@@ -1248,7 +1365,7 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
     Outer& o = op.p[sides];
     Sum& u = sp.p[sides];
     ++sides;
-    t.low = low[k].low, t.splits = low[k].splits;
+    t.low = low[k].low;
     t.out = ws.take<T>((int64_t)pcs * kHalves * m.rp * kGradRows);
     t.back = ws.take<float>(pcs);
     o.U = U.p, o.V = t.out, o.ldu = U.ld, o.cu = U.cols;
