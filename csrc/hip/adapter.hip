@@ -677,10 +677,15 @@ __global__ __launch_bounds__(256, 1) void big_kernel(Big a) {
   constexpr int kRowChunks = BN / E;  // chunks in a row of W's tile if not W_KC
   __shared__ __attribute__((aligned(16))) T us0[BT * BK], us1[BT * BK], ws0[BN * BK], ws1[BN * BK];
 
-  // workgroups go to the 8 XCDs in turn: each XCD gets neighbouring tiles, which share operands in its L2
+  // Workgroups go to the 8 XCDs in turn: each XCD gets neighbouring tiles, and those that run at a time (a 256 x
+  // 256 tile or two smaller ones on each of 32 CUs) are kGroup tiles high and about as wide, so that its L2 reads few
+  // operands for many tiles.
+  constexpr int kGroup = BT == 256 ? 4 : 8;
   const int tiles = a.tiles_t * a.tiles_n, q = tiles / 8, rem = tiles % 8, xcd = blockIdx.x % 8;
-  const int tile = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + blockIdx.x / 8;
-  const int t0 = tile / a.tiles_n * BT, n0 = tile % a.tiles_n * BN;
+  const int number = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + blockIdx.x / 8;
+  const int band = number / (kGroup * a.tiles_n), in_band = number % (kGroup * a.tiles_n);
+  const int high = min(kGroup, a.tiles_t - band * kGroup);
+  const int t0 = (band * kGroup + in_band % high) * BT, n0 = in_band / high * BN;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l32 = lane % 32, half = lane / 32;
   const int wt = wave / 2 * (BT / 2), wn = wave % 2 * (BN / 2);
 
