@@ -664,16 +664,16 @@ __device__ __forceinline__ int swap_columns(int k) {  // in chunks
   else return (k >> 2 & 1) * 8 % kRowChunks;
 }
 
-// Four waves, each a quarter of the tile in blocks of 32 x 32.  Two tiles in
+// WT x WN waves share a tile in blocks of 32 x 32.  Two tiles in
 // LDS and two sets of fragments in registers: while one quarter of a tile is
 // multiplied the next is read; when the last quarter is in registers the
 // tile's place is loaded again, a whole tile's time before the barrier that waits for it.
-template <class T, bool W_KC, int BT, int BN, bool SPLIT>
-__global__ __launch_bounds__(256, 1) void big_kernel(Big a) {
+template <class T, bool W_KC, int BT, int BN, int WT, int WN, bool SPLIT>
+__global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   using Frag = typename Mma<T>::Frag;
   constexpr int E = Mma<T>::kE, BK = 8 * E;
-  constexpr int TT = BT / 64, TN = BN / 64;
-  constexpr int kLoadU = BT / 32, kLoadW = BN / 32;
+  constexpr int TT = BT / WT / 32, TN = BN / WN / 32;
+  constexpr int kLoadU = BT / (WT * WN * 8), kLoadW = BN / (WT * WN * 8);
   constexpr int kRowChunks = BN / E;  // chunks in a row of W's tile if not W_KC
   __shared__ __attribute__((aligned(16))) T us0[BT * BK], us1[BT * BK], ws0[BN * BK], ws1[BN * BK];
 
@@ -687,7 +687,7 @@ __global__ __launch_bounds__(256, 1) void big_kernel(Big a) {
   const int high = min(kGroup, a.tiles_t - band * kGroup);
   const int t0 = (band * kGroup + in_band % high) * BT, n0 = in_band / high * BN;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l32 = lane % 32, half = lane / 32;
-  const int wt = wave / 2 * (BT / 2), wn = wave % 2 * (BN / 2);
+  const int wt = wave / WN * (BT / WT), wn = wave % WN * (BN / WN);
 
   const int nk = (max(a.cu, a.cw) + BK - 1) / BK;
   const int k0 = SPLIT ? (int)((int64_t)nk * blockIdx.y / a.splits) : 0;
@@ -1293,25 +1293,25 @@ struct Many {
     }
     return q;
   }
-  template <bool KC, int BT, int BN>
+  template <bool KC, int BT, int BN, int WT, int WN>
   void launch(const Big& b, hipStream_t s) {
     const dim3 grid((unsigned)(b.tiles_t * b.tiles_n), (unsigned)b.splits);
     if constexpr (BT < 256) {
       if (b.splits > 1) {
-        hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, true>), grid, dim3(256), 0, s, b);
+        hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, true>), grid, dim3(WT * WN * 64), 0, s, b);
         return;
       }
     }
-    hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, false>), grid, dim3(256), 0, s, b);
+    hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, false>), grid, dim3(WT * WN * 64), 0, s, b);
   }
   void run_big(Plan& q, const Low& l, hipStream_t s) {
     Big& b = q.b;
     b.low = l.low, b.by = l.by, b.split = l.split;
     auto shape = [&](auto kc) {
       constexpr bool KC = decltype(kc)::value;
-      if (q.tile == 64) launch<KC, 64, 64>(b, s);
-      else if (q.tile == 128) launch<KC, 128, 128>(b, s);
-      else if constexpr (sizeof(T) == 2) launch<KC, 256, 256>(b, s);
+      if (q.tile == 64) launch<KC, 64, 64, 2, 2>(b, s);
+      else if (q.tile == 128) launch<KC, 128, 128, 2, 2>(b, s);
+      else if constexpr (sizeof(T) == 2) launch<KC, 256, 256, 2, 4>(b, s);
     };
     if (q.kc) shape(std::true_type{});
     else shape(std::false_type{});
