@@ -318,7 +318,8 @@ __global__ __launch_bounds__(256) void few_kernel(Few a) {
 }
 
 // The second launch: sums of the pieces, the product with G_i, the result.
-// A workgroup takes 256 columns of one row; its four waves share the pieces and the ranks.
+// A workgroup takes 256 columns of one row, its four waves sharing the pieces and the ranks, or (ONE_ROW false: with
+// enough rows to fill the chip) of four rows, a wave each.
 struct Finish {
   const float *part, *low;
   View G;
@@ -329,11 +330,15 @@ struct Finish {
   int64_t ldy;
 };
 
-template <class T>
+template <class T, bool ONE_ROW>
 __global__ __launch_bounds__(256) void finish_kernel(Finish a) {
-  __shared__ float s[GELIM_ADAPTER_MAX_RANK];
+  constexpr int kShare = ONE_ROW ? 4 : 1;
+  __shared__ float s_all[ONE_ROW ? 1 : 4][GELIM_ADAPTER_MAX_RANK];
   __shared__ f4 sums[3][64];
-  const int at = blockIdx.x / a.blocks, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, part = ONE_ROW ? wave : 0;
+  const int at = ONE_ROW ? blockIdx.x / a.blocks : blockIdx.x / a.blocks * 4 + wave;
+  if (!ONE_ROW && at >= a.rows.T) return;
+  float* s = s_all[ONE_ROW ? 0 : wave];
   const int64_t t = a.perm ? a.perm[at] : at;
   const int i = adapter_of(a.rows, t);
   const bool has = i >= 0 && i < a.rows.n;
@@ -341,42 +346,59 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish a) {
   f4 acc = {0.f, 0.f, 0.f, 0.f};
   if (n < a.N)
 #pragma unroll 4
-    for (int p = wave; p < a.splits; p += 4) acc += *(const f4*)(a.part + ((int64_t)p * a.rows.T + at) * a.ldp + n);
+    for (int p = part; p < a.splits; p += kShare)
+      acc += *(const f4*)(a.part + ((int64_t)p * a.rows.T + at) * a.ldp + n);
   if (has) {
     const float f = scale_of(a.rows, i);
-    for (int j = threadIdx.x; j < a.r; j += 256) {
+    for (int j = ONE_ROW ? threadIdx.x : lane; j < a.r; j += ONE_ROW ? 256 : 64) {
       float v = 0.f;
       for (int p = 0; p < a.low_splits; ++p) v += a.low[((int64_t)p * a.rows.T + at) * a.ldl + j];
       s[j] = f * v;
     }
-    __syncthreads();
+  }
+  if constexpr (ONE_ROW) __syncthreads();
+  else __builtin_amdgcn_wave_barrier();
+  if (has && n < a.N) {
     const T* G = (const T*)a.G.p + i * a.G.as;
-    if (n < a.N) {
-      const int have = min(4, a.N - n);
-      if (a.G.cs == 1 && have == 4) {
+    const int have = min(4, a.N - n);
+    if (a.G.cs == 1 && have == 4) {
 #pragma unroll 4
-        for (int j = wave; j < a.r; j += 4) {
-          const Four<T> v = *(const Four<T>*)(G + j * a.G.rs + n);
+      for (int j = part; j < a.r; j += kShare) {
+        const Four<T> v = *(const Four<T>*)(G + j * a.G.rs + n);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] += s[j] * (float)v.v[e];
-        }
-      } else {
-        for (int j = wave; j < a.r; j += 4)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < have) acc[e] += s[j] * (float)G[j * a.G.rs + (n + e) * a.G.cs];
+        for (int e = 0; e < 4; ++e) acc[e] += s[j] * (float)v.v[e];
       }
+    } else {
+#pragma unroll 2
+      for (int j = part; j < a.r; j += kShare)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < have) acc[e] += s[j] * (float)G[j * a.G.rs + (n + e) * a.G.cs];
     }
   }
-  if (wave) sums[wave - 1][lane] = acc;
-  __syncthreads();
-  if (wave || n >= a.N) return;
-  acc += sums[0][lane] + sums[1][lane] + sums[2][lane];
+  if constexpr (ONE_ROW) {
+    if (wave) sums[wave - 1][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+    acc += sums[0][lane] + sums[1][lane] + sums[2][lane];
+  }
+  if (n >= a.N) return;
   if (!has && i != -1) acc = acc * __builtin_nanf("");
   T* y = (T*)a.Y + t * a.ldy + n;
+  if (n + 4 <= a.N) {
+    *(Four<T>*)y = Four<T>{(T)acc[0], (T)acc[1], (T)acc[2], (T)acc[3]};
+  } else {
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (n + e < a.N) y[e] = (T)acc[e];
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.N) y[e] = (T)acc[e];
+  }
+}
+
+template <class T>
+void finish(const Finish& e, hipStream_t s) {
+  const int64_t groups = (int64_t)e.rows.T * e.blocks;
+  if (groups < 2048) hipLaunchKernelGGL((finish_kernel<T, true>), dim3((unsigned)groups), dim3(256), 0, s, e);
+  else hipLaunchKernelGGL((finish_kernel<T, false>), dim3((unsigned)((e.rows.T + 3) / 4 * e.blocks)), dim3(256), 0, s, e);
 }
 
 // ---- many rows ------------------------------------------------------------
@@ -411,12 +433,15 @@ __device__ __forceinline__ Piece piece_of(const Order& o, const Rows& g, int num
 }
 int pieces(int64_t T, int64_t n, bool ordered, int size) { return (int)(T / size + (ordered ? n : 1)); }
 
-// A matrix (one per adapter) copied as rows x ld values, zeros behind the source's rows and columns.
+// A matrix (one per adapter) copied as rows x ld values, zeros behind the source's rows and columns; `steps`: as the
+// matrix instruction's fragments, so that a wave's load of one is 1 KB without gaps: step along ld, block of 16
+// rows, lane, kE values.
 struct Copy {
   View src;
   void* dst;
   int rows, cols, ld, count;  // of the copy (rows, ld) and how many matrices
   int have;                   // rows of the source; the others are zeros
+  bool steps, straight;
   int first;                  // workgroups before this copy's
 };
 constexpr int kCopies = 6, kCopyTile = 64;
@@ -462,6 +487,24 @@ __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
   }
 }
 
+// 64 KB of a copy whose source runs along its rows: 16 bytes a thread, from any element's address.
+constexpr int kStraight = 4096;  // chunks of 16 bytes
+template <class T>
+__device__ __forceinline__ void copy_straight(const Copy& c, int part) {
+  constexpr int E = Mma<T>::kE;
+  const int across = c.ld / E;
+  const int64_t all = (int64_t)c.count * c.rows * across;
+#pragma unroll
+  for (int q = 0; q < kStraight / 1024; ++q) {
+    const int64_t o = (int64_t)part * kStraight + q * 1024 + threadIdx.x;
+    if (o >= all) return;
+    const int64_t row = o / across, m = row / c.rows, i = row % c.rows;
+    const int j = (int)(o % across) * E;
+    *((typename Mma<T>::Frag*)c.dst + o) =
+        load_part((const T*)c.src.p + m * c.src.as + i * c.src.rs + j, i < c.have ? c.cols - j : 0);
+  }
+}
+
 // One 64 x 64 tile of a copy, read along the source's memory and written along the destination's.
 template <class T>
 __device__ __forceinline__ void copy_tile(const Copy& c, int tile) {
@@ -478,6 +521,17 @@ __device__ __forceinline__ void copy_tile(const Copy& c, int tile) {
     lds[i][j] = r0 + i < c.have && c0 + j < c.cols ? src[(r0 + i) * c.src.rs + (c0 + j) * c.src.cs] : (T)0.f;
   }
   __syncthreads();
+  if (c.steps) {
+    using M = Mma<T>;
+    constexpr int kBlock = 64 * M::kE, kInTile = kCopyTile / M::kStep;
+    const int blocks = c.rows / 16, here = min(4, blocks - r0 / 16);  // of 16 rows, in all and in this tile
+    for (int o = threadIdx.x; o < kInTile * here * kBlock; o += 1024) {
+      const int step = o / (here * kBlock), rb = o / kBlock % here, lane = o / M::kE % 64;
+      dst[((int64_t)(c0 / M::kStep + step) * blocks + r0 / 16 + rb) * kBlock + o % kBlock] =
+          lds[rb * 16 + lane % 16][step * M::kStep + lane / 16 * M::kE + o % M::kE];
+    }
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int i = slow + 16 * k;
@@ -494,11 +548,12 @@ __global__ __launch_bounds__(1024) void prepare_kernel(Prepare p) {
   b -= p.order_groups;
   int k = p.copies - 1;
   while (k > 0 && b < p.copy[k].first) --k;
-  copy_tile<T>(p.copy[k], b - p.copy[k].first);
+  if (p.copy[k].straight) copy_straight<T>(p.copy[k], b - p.copy[k].first);
+  else copy_tile<T>(p.copy[k], b - p.copy[k].first);
 }
 
 // low (place, rank) = U F_i, 32 places of one adapter by a workgroup, whose waves cut the sum.
-// F is laid out as rp ranks x ldf along the sum, zeros behind C.  Bound by
+// F is laid out in fragments, ldf values along the sum with zeros behind C.  Bound by
 // reading U and, for every 32 rows, F_i: each wave keeps several steps' loads in flight.
 // 16-bit types: also as the sum of two values of the type, 8 ranks' upper and then lower parts side by side, for
 // the matrix units of the large product.  One value's rounding alone would be as large as the
@@ -516,7 +571,7 @@ struct LowPair {
   Order order;
 };
 constexpr int kLowRows = 32;
-constexpr int low_waves(int rank_blocks) { return rank_blocks <= 8 ? 16 : 8; }
+constexpr int kLowWaves = 8;
 
 // v as upper and lower part of the type; the lower is 0 beside an infinity or NaN
 template <class T>
@@ -530,10 +585,10 @@ __device__ __forceinline__ int to_fp16_range(float most) {
 }
 
 template <class T, int RB>
-__global__ __launch_bounds__(low_waves(RB) * 64) void low_kernel(LowPair both) {
+__global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int E = M::kE, rp = 16 * RB, kWaves = low_waves(RB);
+  constexpr int E = M::kE, rp = 16 * RB, kWaves = kLowWaves;
   __shared__ f4 lds[kWaves / 2][RB * 2][64];
   const Low& a = both.p[blockIdx.y];
   const Piece pc = piece_of(both.order, both.rows, blockIdx.x, kLowRows);
@@ -543,17 +598,17 @@ __global__ __launch_bounds__(low_waves(RB) * 64) void low_kernel(LowPair both) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
     u[t] = (const T*)a.U + row_at(both.order, pc.begin + min(t * 16 + l16, pc.count - 1)) * a.ldu;
-  const T* f = (const T*)a.F + ((int64_t)pc.adapter * rp + l16) * a.ldf;
+  const Frag* f = (const Frag*)((const T*)a.F + (int64_t)pc.adapter * rp * a.ldf) + lane;
   const int steps = (a.cu + M::kStep - 1) / M::kStep;
   const int s0 = (int)((int64_t)steps * wave / kWaves), s1 = (int)((int64_t)steps * (wave + 1) / kWaves);
   f4 acc[RB][2] = {};
-  constexpr int kFlight = RB <= 2 ? 4 : RB == 4 ? 2 : 1;  // by the registers that a wave may have
+  constexpr int kFlight = RB <= 2 ? 4 : RB == 4 ? 2 : 1;  // by the registers of two workgroups a CU
   for (int s = s0; s < s1; s += kFlight) {
     Frag x[kFlight][2], w[kFlight][RB];
 #pragma unroll
     for (int q = 0; q < kFlight; ++q) {
       // a step behind the last one repeats it, with zeros for U
-      const int k = min(s + q, s1 - 1) * M::kStep + g * E;
+      const int step = min(s + q, s1 - 1), k = step * M::kStep + g * E;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         x[q][t] = Frag{};
@@ -562,7 +617,7 @@ __global__ __launch_bounds__(low_waves(RB) * 64) void low_kernel(LowPair both) {
 #pragma unroll
       for (int j = 0; j < RB; ++j) {
         w[q][j] = Frag{};
-        if (s + q < s1) w[q][j] = *(const Frag*)(f + (int64_t)j * 16 * a.ldf + k);
+        if (s + q < s1) w[q][j] = f[((int64_t)step * RB + j) * 64];
       }
     }
 #pragma unroll
@@ -908,63 +963,16 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   }
 }
 
-// The factors' gradients: sum over the places of an adapter of U_t^T V_t, V = S or D.
-// First V turned (a value per place along memory), in pieces of kGradRows places: 16-bit types as two values
-// of the type whose sum has V's upper bits (fp16: brought to below 2^14 by the piece's power of two).
+// The factors' gradients: sum over the places of an adapter of U_t^T V_t, V = S or D, in pieces of kGradRows
+// places.  A workgroup takes 64 kE columns of U, a wave 16 kE, whose rows it turns in registers.  V is turned on its
+// way to LDS, as upper and lower part of the type (fp16: brought to below 2^14 by the
+// piece's power of two).  Bound by reading U once: each wave keeps two steps' rows in flight.
 constexpr int kGradRows = 128;
-struct Turn {
-  const float* low;
-  void* out;    // piece, half (16-bit types), rank, place
-  float* back;  // of each piece, the factor that undoes the power of two
-};
-struct TurnPair {
-  Turn p[2];
-  Rows rows;
-  Order order;
-  int rp;
-};
-
-template <class T>
-__global__ __launch_bounds__(256) void turn_kernel(TurnPair both) {
-  __shared__ float wave_most[4];
-  const Turn& a = both.p[blockIdx.y];
-  const int rp = both.rp;
-  const Piece pc = piece_of(both.order, both.rows, blockIdx.x, kGradRows);
-  if (pc.count == 0) return;
-  const int t = threadIdx.x % kGradRows;
-  auto value = [&](int j) { return t < pc.count ? a.low[(int64_t)(pc.begin + t) * rp + j] : 0.f; };
-  float by = 1.f, back = 1.f;
-  if constexpr (std::is_same_v<T, _Float16>) {
-    float most = 0.f;
-    for (int j = threadIdx.x / kGradRows; j < rp; j += 256 / kGradRows) {
-      const float v = fabsf(value(j));
-      if (v > most && v <= 3.4e38f) most = v;
-    }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-    if (threadIdx.x % 64 == 0) wave_most[threadIdx.x / 64] = most;
-    __syncthreads();
-    most = fmaxf(fmaxf(wave_most[0], wave_most[1]), fmaxf(wave_most[2], wave_most[3]));
-    const int e = to_fp16_range(most);
-    by = ldexpf(1.f, e);
-    back = ldexpf(1.f, -e);
-  }
-  if (threadIdx.x == 0) a.back[blockIdx.x] = back;
-  constexpr int kHalves = sizeof(T) == 2 ? 2 : 1;
-  T* out = (T*)a.out + (int64_t)blockIdx.x * kHalves * rp * kGradRows + t;
-  for (int j = threadIdx.x / kGradRows; j < rp; j += 256 / kGradRows) {
-    T hi, lo;
-    two_parts(value(j) * by, hi, lo);
-    out[j * kGradRows] = hi;
-    if constexpr (kHalves == 2) out[(rp + j) * kGradRows] = lo;
-  }
-}
-
-// Then the products of a piece: a wave takes 16 kE columns of U, whose rows it turns in registers.
 struct Outer {
-  const void *U, *V;
+  const void* U;
   int64_t ldu;
-  float* part;  // piece, rank, column
+  const float* low;  // V
+  float* part;       // piece, rank, column
   int cu, ldp, blocks;
 };
 struct OuterPair {
@@ -978,41 +986,90 @@ template <class T, int RB>
 __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int E = M::kE, kHalves = sizeof(T) == 2 ? 2 : 1;
+  constexpr int E = M::kE, kHalves = sizeof(T) == 2 ? 2 : 1, kRanks = RB * 16, kPitch = kGradRows + 16 / sizeof(T);
+  __shared__ __attribute__((aligned(16))) T vs[kHalves][kRanks][kPitch];
   __shared__ int32_t row[kGradRows];
+  __shared__ float wave_most[4];
   const Outer& a = both.p[blockIdx.y];
   const int piece = blockIdx.x % both.pieces, block = blockIdx.x / both.pieces;
   if (block >= a.blocks) return;
   const Piece pc = piece_of(both.order, both.rows, piece, kGradRows);
   if (pc.count == 0) return;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
+  const int j0 = blockIdx.z * kRanks;
   if (threadIdx.x < kGradRows) row[threadIdx.x] = (int32_t)row_at(both.order, pc.begin + min((int)threadIdx.x, pc.count - 1));
   __syncthreads();
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
   const int n0 = (block * 4 + wave) * 16 * E, n = n0 + l16 * E;
-  if (n0 >= a.cu) return;
-  const int j0 = blockIdx.z * RB * 16;
-  const T* V = (const T*)a.V + ((int64_t)piece * kHalves * both.rp + j0 + l16) * kGradRows;
   const T* U = (const T*)a.U + n;
-  f4 acc[E][RB] = {};
-  const int steps = (pc.count + M::kStep - 1) / M::kStep;
-#pragma unroll 2
-  for (int s = 0; s < steps; ++s) {
-    const int t = s * M::kStep + g * E;
-    Frag in[E], w[E];
+  constexpr int kFlight = 2;
+  Frag in[kFlight][E];
+  auto fetch = [&](int s) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      in[e] = Frag{};
-      if (t + e < pc.count && n < a.cu) in[e] = *(const Frag*)(U + row[t + e] * a.ldu);
-    }
-    turn<T>(in, w);
+    for (int q = 0; q < kFlight; ++q)
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        const Frag v = *(const Frag*)(V + (int64_t)(h * both.rp + b * 16) * kGradRows + t);
-#pragma unroll
-        for (int j = 0; j < E; ++j) acc[j][b] = M::mma(w[j], v, acc[j][b]);
+      for (int e = 0; e < E; ++e) {
+        const int t = (s + q) * M::kStep + g * E + e;
+        in[q][e] = Frag{};
+        if (t < pc.count && n < a.cu) in[q][e] = *(const Frag*)(U + row[t] * a.ldu);
       }
+  };
+  fetch(0);  // while V is laid out
+  // V: thread (place, every other 4 ranks)
+  constexpr int kMine = kRanks / 8;
+  const int t = threadIdx.x / 2;
+  f4 v[kMine];
+#pragma unroll
+  for (int q = 0; q < kMine; ++q) {
+    v[q] = f4{0.f, 0.f, 0.f, 0.f};
+    if (t < pc.count) v[q] = *(const f4*)(a.low + (int64_t)(pc.begin + t) * both.rp + j0 + q * 8 + threadIdx.x % 2 * 4);
+  }
+  float by = 1.f, back = 1.f;
+  if constexpr (std::is_same_v<T, _Float16>) {
+    float most = 0.f;
+#pragma unroll
+    for (int q = 0; q < kMine; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = fabsf(v[q][e]);
+        if (x > most && x <= 3.4e38f) most = x;
+      }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    if (lane == 0) wave_most[wave] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(wave_most[0], wave_most[1]), fmaxf(wave_most[2], wave_most[3]));
+    const int e = to_fp16_range(most);
+    by = ldexpf(1.f, e);
+    back = ldexpf(1.f, -e);
+  }
+#pragma unroll
+  for (int q = 0; q < kMine; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = q * 8 + threadIdx.x % 2 * 4 + e;
+      if constexpr (kHalves == 2) two_parts(v[q][e] * by, vs[0][j][t], vs[1][j][t]);
+      else vs[0][j][t] = v[q][e];
+    }
+  __syncthreads();
+  if (n0 >= a.cu) return;
+  f4 acc[E][RB] = {};
+  for (int s = 0;;) {
+#pragma unroll
+    for (int q = 0; q < kFlight; ++q) {
+      Frag w[E];
+      turn<T>(in[q], w);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          const Frag x = *(const Frag*)&vs[h][b * 16 + l16][(s + q) * M::kStep + g * E];
+#pragma unroll
+          for (int j = 0; j < E; ++j) acc[j][b] = M::mma(w[j], x, acc[j][b]);
+        }
+    }
+    s += kFlight;
+    if (s * M::kStep >= pc.count) break;
+    fetch(s);
   }
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -1021,13 +1078,15 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < E; j += 4)
-        *(f4*)(out + (g * 4 + i) * E + j) = f4{acc[j][b][i], acc[j + 1][b][i], acc[j + 2][b][i], acc[j + 3][b][i]};
+        *(f4*)(out + (g * 4 + i) * E + j) =
+            back * f4{acc[j][b][i], acc[j + 1][b][i], acc[j + 2][b][i], acc[j + 3][b][i]};
   }
 }
 
-// Last their sums, times s_i, in the factor's layout: 64 columns x 16 ranks of one adapter by a workgroup.
+// Last their sums, times s_i, in the factor's layout: 64 columns x 4 ranks of one adapter by a workgroup, whose four
+// waves share the pieces.
 struct Sum {
-  const float *part, *back;
+  const float* part;
   void* out;
   int64_t as, cs, rs;  // adapter, column, rank
   int cols, ldp, blocks;
@@ -1041,38 +1100,37 @@ struct SumPair {
 
 template <class T>
 __global__ __launch_bounds__(256) void sum_kernel(SumPair both) {
-  __shared__ float lds[64][17];
+  __shared__ f4 lds[3][64];
   const Sum& a = both.p[blockIdx.y];
   if ((int)blockIdx.x >= a.blocks) return;
-  const int ranks = (both.r + 15) / 16;
-  const int c0 = blockIdx.x / ranks * 64, j0 = blockIdx.x % ranks * 16;
+  const int fours = (both.r + 3) / 4, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int c = blockIdx.x / fours * 64 + lane, j0 = blockIdx.x % fours * 4;
   for (int i = blockIdx.z; i < both.rows.n; i += gridDim.z) {
     const int count = both.order.start ? both.order.start[i + 1] - both.order.start[i] : both.rows.T;
     const int first = first_piece(both.order, i, kGradRows), many = (count + kGradRows - 1) / kGradRows;
-    const float f = scale_of(both.rows, i);
-    const int c = threadIdx.x % 64, jq = threadIdx.x / 64 * 4;
-    float s[4] = {};
-    for (int p = first; p < first + many; ++p) {
-      const float back = a.back[p];
+    f4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = wave; p < many; p += 4) {
+      const float* from = a.part + ((int64_t)(first + p) * both.rp + j0) * a.ldp + c;
+      f4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] += back * a.part[((int64_t)p * both.rp + j0 + jq + e) * a.ldp + c0 + c];
+      for (int e = 0; e < 4; ++e) v[e] = from[e * (int64_t)a.ldp];
+      s += v;
     }
-    T* out = (T*)a.out + i * a.as;
-    if (a.cs == 1) {
+    if (wave) lds[wave - 1][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < a.cols) {
+      s = (s + lds[0][lane] + lds[1][lane] + lds[2][lane]) * scale_of(both.rows, i);
+      T* out = (T*)a.out + i * a.as + c * a.cs + j0 * a.rs;
+      if (a.rs == 1 && j0 + 4 <= both.r) {
+        *(Four<T>*)out = Four<T>{(T)s[0], (T)s[1], (T)s[2], (T)s[3]};
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c0 + c < a.cols && j0 + jq + e < both.r) out[(j0 + jq + e) * a.rs + c0 + c] = (T)(f * s[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) lds[c][jq + e] = f * s[e];
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int cc = e * 16 + threadIdx.x / 16, j = threadIdx.x % 16;
-        if (c0 + cc < a.cols && j0 + j < both.r) out[(c0 + cc) * a.cs + (j0 + j) * a.rs] = (T)lds[cc][j];
+        for (int e = 0; e < 4; ++e)
+          if (j0 + e < both.r) out[e * a.rs] = (T)s[e];
       }
-      __syncthreads();
     }
+    __syncthreads();
   }
 }
 
@@ -1169,7 +1227,7 @@ int few_product(const Problem& p, const Rows& g, int r, Space& ws, hipStream_t s
   else launch(std::false_type{});
   Finish e{f.part, f.low, p.G, g, nullptr, p.N, r, f.ldp, f.splits, f.low_splits, r, (p.N + 255) / 256,
            p.Y, p.ldy};
-  hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)(g.T * e.blocks)), dim3(256), 0, s, e);
+  finish<T>(e, s);
   HIP_TRY(hipGetLastError());
   return GELIM_OK;
 }
@@ -1200,11 +1258,12 @@ struct Many {
     groups = prep.order_groups;
   }
 
-  T* copy(View src, int rows, int have, int cols, int ld, int count) {
+  T* copy(View src, int rows, int have, int cols, int ld, int count, bool steps = false) {
     Copy& c = prep.copy[prep.copies++];
-    c = {src, ws.template take<T>((int64_t)count * rows * ld), rows, cols, ld, count, have,
-         (int)groups - prep.order_groups};
-    groups += (unsigned)(count * ((rows + kCopyTile - 1) / kCopyTile) * ((ld + kCopyTile - 1) / kCopyTile));
+    c = {src, ws.template take<T>((int64_t)count * rows * ld), rows, cols, ld, count, have, steps,
+         !steps && src.cs == 1, (int)groups - prep.order_groups};
+    groups += c.straight ? (unsigned)(((int64_t)count * rows * (ld / E) + kStraight - 1) / kStraight)
+                         : (unsigned)(count * ((rows + kCopyTile - 1) / kCopyTile) * ((ld + kCopyTile - 1) / kCopyTile));
     return (T*)c.dst;
   }
   static bool aligned(const void* p, int64_t ld, int64_t len) {
@@ -1226,7 +1285,7 @@ struct Many {
   Low low_of(const Wide& U, View F, int C) {
     Low l{};
     l.ldf = (int)up(C, 64);
-    l.F = copy(turned(F), rp, (int)a.r, C, l.ldf, (int)a.n);
+    l.F = copy(turned(F), rp, (int)a.r, C, l.ldf, (int)a.n, true);
     l.U = U.p, l.ldu = U.ld, l.cu = U.cols;
     l.pieces = pieces(a.T, a.n, a.index != nullptr, kLowRows);
     l.low = ws.template take<float>(a.T * rp);
@@ -1248,11 +1307,11 @@ struct Many {
     }
     const dim3 grid(most, (unsigned)count);
     switch (rb) {
-      case 1: hipLaunchKernelGGL((low_kernel<T, 1>), grid, dim3(low_waves(1) * 64), 0, s, both); break;
-      case 2: hipLaunchKernelGGL((low_kernel<T, 2>), grid, dim3(low_waves(2) * 64), 0, s, both); break;
-      case 4: hipLaunchKernelGGL((low_kernel<T, 4>), grid, dim3(low_waves(4) * 64), 0, s, both); break;
-      case 8: hipLaunchKernelGGL((low_kernel<T, 8>), grid, dim3(low_waves(8) * 64), 0, s, both); break;
-      default: hipLaunchKernelGGL((low_kernel<T, 16>), grid, dim3(low_waves(16) * 64), 0, s, both);
+      case 1: hipLaunchKernelGGL((low_kernel<T, 1>), grid, dim3(kLowWaves * 64), 0, s, both); break;
+      case 2: hipLaunchKernelGGL((low_kernel<T, 2>), grid, dim3(kLowWaves * 64), 0, s, both); break;
+      case 4: hipLaunchKernelGGL((low_kernel<T, 4>), grid, dim3(kLowWaves * 64), 0, s, both); break;
+      case 8: hipLaunchKernelGGL((low_kernel<T, 8>), grid, dim3(kLowWaves * 64), 0, s, both); break;
+      default: hipLaunchKernelGGL((low_kernel<T, 16>), grid, dim3(kLowWaves * 64), 0, s, both);
     }
   }
 
@@ -1284,7 +1343,7 @@ struct Many {
     b.tiles_t = (int)((a.T + q.tile - 1) / q.tile);
     b.tiles_n = (p.N + q.tile - 1) / q.tile;
     const int nk = (std::max(b.cu, b.cw) + 8 * E - 1) / (8 * E), all = std::max(1, b.tiles_t * b.tiles_n);
-    b.splits = q.tile == 256 || all >= 256 ? 1 : std::clamp(512 / all, 1, std::clamp(nk / 4, 1, 16));
+    b.splits = q.tile == 256 || all >= 160 ? 1 : std::clamp(512 / all, 1, std::clamp(nk / 4, 1, 16));
     if (b.splits > 1) {
       b.ldp = b.tiles_n * q.tile;
       b.part = ws.template take<float>((int64_t)b.splits * a.T * b.ldp);
@@ -1318,7 +1377,7 @@ struct Many {
     if (b.splits > 1) {
       Finish e{b.part, l.low, q.p.G, g, order.perm, b.N, (int)a.r, b.ldp, b.splits, 1, rp,
                (b.N + 255) / 256, b.Y, b.ldy};
-      hipLaunchKernelGGL(finish_kernel<T>, dim3((unsigned)(a.T * e.blocks)), dim3(256), 0, s, e);
+      finish<T>(e, s);
     }
   }
 };
@@ -1354,34 +1413,28 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   if ((a.dX && a.T) || all) q = m.big_of(back, dY);
   // the sides: dA = X^T D, dB^T = dY^T S
   const int pcs = pieces(a.T, a.n, a.index != nullptr, kGradRows);
-  TurnPair tp{};
   OuterPair op{};
   SumPair sp{};
-  tp.rows = op.rows = sp.rows = m.g, tp.order = op.order = sp.order = m.order;
-  tp.rp = op.rp = sp.rp = m.rp, sp.r = (int)a.r, op.pieces = pcs;
+  op.rows = sp.rows = m.g, op.order = sp.order = m.order;
+  op.rp = sp.rp = m.rp, sp.r = (int)a.r, op.pieces = pcs;
   int sides = 0;
   unsigned outer_groups = 0, sum_groups = 0;
   for (int k = 0; k < 2; ++k) {
     if (!(k ? a.dB : a.dA) && !all) continue;
     const auto& U = k ? dY : X;
     const int cols = k ? N : K;
-    constexpr int kHalves = sizeof(T) == 2 ? 2 : 1;
-    Turn& t = tp.p[sides];
     Outer& o = op.p[sides];
     Sum& u = sp.p[sides];
     ++sides;
-    t.low = low[k].low;
-    t.out = ws.take<T>((int64_t)pcs * kHalves * m.rp * kGradRows);
-    t.back = ws.take<float>(pcs);
-    o.U = U.p, o.V = t.out, o.ldu = U.ld, o.cu = U.cols;
+    o.U = U.p, o.low = low[k].low, o.ldu = U.ld, o.cu = U.cols;
     o.blocks = (U.cols + 64 * Mma<T>::kE - 1) / (64 * Mma<T>::kE);
     o.ldp = (int)up(U.cols, 16 * Mma<T>::kE);
     o.part = ws.take<float>((int64_t)pcs * m.rp * o.ldp);
-    u.part = o.part, u.back = t.back, u.out = k ? a.dB : a.dA, u.cols = cols, u.ldp = o.ldp;
+    u.part = o.part, u.out = k ? a.dB : a.dA, u.cols = cols, u.ldp = o.ldp;
     u.as = (int64_t)a.r * cols;
     const bool along = k ? !a.b_trans : a.a_trans;  // columns side by side
     u.cs = along ? 1 : a.r, u.rs = along ? cols : 1;
-    u.blocks = (int)((cols + 63) / 64 * ((a.r + 15) / 16));
+    u.blocks = (int)((cols + 63) / 64 * ((a.r + 3) / 4));
     outer_groups = std::max(outer_groups, (unsigned)(pcs * o.blocks));
     sum_groups = std::max(sum_groups, (unsigned)u.blocks);
   }
@@ -1394,7 +1447,6 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   }
   if (sides) {
     if (a.T) {
-      hipLaunchKernelGGL(turn_kernel<T>, dim3((unsigned)pcs, (unsigned)sides), dim3(256), 0, s, tp);
       const int per = std::min(m.rb, 4);
       const dim3 grid(outer_groups, (unsigned)sides, (unsigned)(m.rb / per));
       if (per == 1) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, dim3(256), 0, s, op);
