@@ -161,6 +161,8 @@ struct Few {
   int64_t ldy;
 };
 
+constexpr int kFewFlight = 2;  // steps whose loads a wave has in flight
+constexpr int kFewGroups = 512;
 // One wave: 16 kE columns of W, its steps of the sum; W_KC: W's sum runs along its rows in memory.
 // Each 16-byte load of 16 neighbouring lanes covers 256 bytes of a row of W (64 where W_KC: two steps make the line).
 template <class T, bool W_KC, int TT, bool EDGE>
@@ -171,37 +173,49 @@ __device__ __forceinline__ void few_steps(const Few& a, int n0, int s0, int s1, 
   const int l16 = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
   const T* W = (const T*)a.W.p;
   const T* U = (const T*)a.U;
-#pragma unroll 2
-  for (int s = s0; s < s1; ++s) {
-    const int k = s * M::kStep + g * E;
-    Frag w[E], x[TT];
-    if constexpr (W_KC) {
+  for (int s = s0; s < s1; s += kFewFlight) {
+    Frag w[kFewFlight][E], x[kFewFlight][TT];
+#pragma unroll
+    for (int q = 0; q < kFewFlight; ++q) {
+      const bool in = s + q < s1;  // a step behind the last one: zeros
+      const int k = (in ? s + q : s) * M::kStep + g * E;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const int n = n0 + j * 16 + l16;
-        if constexpr (EDGE) w[j] = load_part(W + (int64_t)min(n, a.N - 1) * a.W.cs + k, a.C - k);
-        else w[j] = load16(W + (int64_t)n * a.W.cs + k);
+        w[q][j] = Frag{};
+        if (!in) continue;
+        if constexpr (W_KC) {
+          const int n = n0 + j * 16 + l16;
+          if constexpr (EDGE) w[q][j] = load_part(W + (int64_t)min(n, a.N - 1) * a.W.cs + k, a.C - k);
+          else w[q][j] = load16(W + (int64_t)n * a.W.cs + k);
+        } else {
+          const int n = n0 + l16 * E;
+          if constexpr (EDGE) w[q][j] = load_part(W + (int64_t)(k + j) * a.W.rs + n, k + j < a.C ? a.N - n : 0);
+          else w[q][j] = load16(W + (int64_t)(k + j) * a.W.rs + n);
+        }
       }
-    } else {
-      Frag in[E];
-      const int n = n0 + l16 * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if constexpr (EDGE) in[e] = load_part(W + (int64_t)(k + e) * a.W.rs + n, k + e < a.C ? a.N - n : 0);
-        else in[e] = load16(W + (int64_t)(k + e) * a.W.rs + n);
+      for (int t = 0; t < TT; ++t) {
+        const T* row = U + (int64_t)min(t * 16 + l16, a.rows.T - 1) * a.ldu;
+        x[q][t] = Frag{};
+        if (!in) continue;
+        if constexpr (EDGE) x[q][t] = load_part(row + k, a.C - k);
+        else x[q][t] = load16(row + k);
       }
-      turn<T>(in, w);
     }
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const T* row = U + (int64_t)min(t * 16 + l16, a.rows.T - 1) * a.ldu;
-      if constexpr (EDGE) x[t] = load_part(row + k, a.C - k);
-      else x[t] = load16(row + k);
+    for (int q = 0; q < kFewFlight; ++q) {
+      Frag v[E];
+      if constexpr (W_KC) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = w[q][j];
+      } else {
+        turn<T>(w[q], v);
+      }
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[j][t] = M::mma(v[j], x[q][t], acc[j][t]);
     }
-#pragma unroll
-    for (int j = 0; j < E; ++j)
-#pragma unroll
-      for (int t = 0; t < TT; ++t) acc[j][t] = M::mma(w[j], x[t], acc[j][t]);
   }
 }
 
@@ -1209,7 +1223,7 @@ int few_product(const Problem& p, const Rows& g, int r, Space& ws, hipStream_t s
   f.U = p.U, f.ldu = p.ldu, f.W = p.W, f.F = p.F, f.G = p.G, f.rows = g, f.C = p.C, f.N = p.N, f.r = r;
   f.blocks = (int)((p.N + 16 * M::kE - 1) / (16 * M::kE));
   const int steps = (p.C + M::kStep - 1) / M::kStep;
-  f.splits = std::clamp(512 / f.blocks, 1, std::max(1, std::min(64, steps / 4)));
+  f.splits = std::clamp(kFewGroups / f.blocks, 1, std::max(1, std::min(64, steps / 4)));
   f.low_splits = std::clamp(256 / g.T, 1, std::max(1, std::min(16, p.C / 256)));
   f.ldp = f.blocks * 16 * M::kE;
   f.part = ws.take<float>((int64_t)f.splits * g.T * f.ldp);

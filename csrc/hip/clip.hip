@@ -1,10 +1,10 @@
 // 2-norm over many tensors, and their copies scaled by min(1, max_norm / (norm + 1e-6)).
 //
 // Memory-bound: every element is read twice (the factor needs all of them) and
-// written once.  Two passes over the tensors; a pass is one launch per
-// kPerLaunch tensors, whose table travels in the kernel's arguments, so a
+// written once.  Two passes over the tensors; a pass is one launch per 264
+// tensors (172 with outputs apart), whose table travels in the kernel's arguments, so a
 // captured graph needs no table in device memory.  The tensors are cut into
-// chunks and workgroup b takes the chunks b, b + grid, ...; its sum goes to its
+// chunks and each workgroup takes a run of them; its sum goes to its
 // own slot of the workspace, onto that of the launch before, and every
 // workgroup of the second pass adds the slots up in one fixed order: no
 // atomics, the same bits every time.
@@ -15,6 +15,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <climits>
+#include <string>
 #include <vector>
 
 #include "device_common.h"
@@ -23,18 +25,20 @@
 namespace gelim {
 namespace {
 
-constexpr int kPerLaunch = 128, kSlots = 1024, kThreads = 256;
-constexpr int64_t kChunk = 16384;  // elements
+constexpr int kSlots = 1024, kThreads = 256;
+constexpr int kChunk = 16384;  // elements
 
+template <bool APART>
 struct Table {
-  const void* in[kPerLaunch];
-  void* out[kPerLaunch];
-  int64_t size[kPerLaunch];
-  int32_t first[kPerLaunch];  // chunks before this tensor
-  int8_t type[kPerLaunch];
-  int32_t count, chunks;
+  static constexpr int kMost = APART ? 172 : 264;  // within 4 KB of arguments
+  const void* in[kMost];
+  void* out[APART ? kMost : 1];
+  int32_t first[kMost + 1];  // chunks before this tensor
+  uint16_t tail[kMost];      // elements of its last chunk
+  int8_t type[kMost];
+  int32_t count;
 };
-static_assert(sizeof(Table) <= 4000, "kernel arguments");
+static_assert(sizeof(Table<true>) <= 4000 && sizeof(Table<false>) <= 4000, "kernel arguments");
 
 // 16 bytes at any element's address: the hardware takes unaligned vector accesses
 template <class T>
@@ -45,21 +49,29 @@ struct Pack {
   };
 };
 
-__device__ __forceinline__ int tensor_of(const Table& tb, int chunk) {
-  int lo = 0, hi = tb.count - 1;  // the last tensor that begins at or before the chunk
+// The chunks [begin, end) of one workgroup, one after the other: f(tensor, first element, elements, type).
+template <bool APART, class F>
+__device__ __forceinline__ void each_chunk(const Table<APART>& tb, F f) {
+  const int all = tb.first[tb.count];
+  const int begin = (int)((int64_t)all * blockIdx.x / gridDim.x), end = (int)((int64_t)all * (blockIdx.x + 1) / gridDim.x);
+  if (begin == end) return;
+  int lo = 0, hi = tb.count - 1;  // the last tensor that begins at or before `begin`
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
-    if (tb.first[mid] <= chunk) lo = mid;
+    if (tb.first[mid] <= begin) lo = mid;
     else hi = mid - 1;
   }
-  return lo;
+  for (int c = begin; c < end; ++c) {
+    while (c >= tb.first[lo + 1]) ++lo;
+    f(lo, (int64_t)(c - tb.first[lo]) * kChunk, c + 1 == tb.first[lo + 1] ? tb.tail[lo] : kChunk, tb.type[lo]);
+  }
 }
 
 template <class T>
-__device__ __forceinline__ double squares(const T* p, int64_t len) {
+__device__ __forceinline__ double squares(const T* p, int len) {
   constexpr int L = Pack<T>::kLen;
   double s = 0.0;
-  int64_t e = (int64_t)threadIdx.x * L;
+  int e = threadIdx.x * L;
 #pragma unroll 4
   for (; e + L <= len; e += kThreads * L) {
     const typename Pack<T>::Mem m = *(const typename Pack<T>::Mem*)(p + e);
@@ -86,23 +98,21 @@ __device__ __forceinline__ double block_sum(double v) {
   return s;
 }
 
-__global__ __launch_bounds__(kThreads) void squares_kernel(const Table tb, double* slots, int fresh) {
+__global__ __launch_bounds__(kThreads) void squares_kernel(const Table<false> tb, double* slots, int fresh) {
   double s = 0.0;
-  for (int c = blockIdx.x; c < tb.chunks; c += gridDim.x) {
-    const int i = tensor_of(tb, c);
-    const int64_t at = (int64_t)(c - tb.first[i]) * kChunk, len = min(tb.size[i] - at, kChunk);
-    if (tb.type[i] == GELIM_T_F32) s += squares((const float*)tb.in[i] + at, len);
-    else if (tb.type[i] == GELIM_T_BF16) s += squares((const __bf16*)tb.in[i] + at, len);
+  each_chunk(tb, [&](int i, int64_t at, int len, int type) {
+    if (type == GELIM_T_F32) s += squares((const float*)tb.in[i] + at, len);
+    else if (type == GELIM_T_BF16) s += squares((const __bf16*)tb.in[i] + at, len);
     else s += squares((const _Float16*)tb.in[i] + at, len);
-  }
+  });
   s = block_sum(s);
   if (threadIdx.x == 0) slots[blockIdx.x] = fresh ? s : slots[blockIdx.x] + s;
 }
 
 template <class T>
-__device__ __forceinline__ void scaled(const T* p, T* q, int64_t len, float f) {
+__device__ __forceinline__ void scaled(const T* p, T* q, int len, float f) {
   constexpr int L = Pack<T>::kLen;
-  int64_t e = (int64_t)threadIdx.x * L;
+  int e = threadIdx.x * L;
 #pragma unroll 4
   for (; e + L <= len; e += kThreads * L) {
     typename Pack<T>::Mem m = *(const typename Pack<T>::Mem*)(p + e);
@@ -113,7 +123,8 @@ __device__ __forceinline__ void scaled(const T* p, T* q, int64_t len, float f) {
   for (; e < len; ++e) q[e] = (T)((float)p[e] * f);
 }
 
-__global__ __launch_bounds__(kThreads) void scale_kernel(const Table tb, const double* slots, int nslots,
+template <bool APART>
+__global__ __launch_bounds__(kThreads) void scale_kernel(const Table<APART> tb, const double* slots, int nslots,
                                                          double max_norm, float* norm_out) {
   double s = 0.0;
   for (int i = threadIdx.x; i < nslots; i += kThreads) s += slots[i];
@@ -122,15 +133,14 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(const Table tb, const d
   double f = isinf(max_norm) ? 1.0 : max_norm / (norm + 1e-6);
   if (f > 1.0) f = 1.0;
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
-  for (int k = blockIdx.x; k < tb.chunks; k += gridDim.x) {
-    const int c = tb.chunks - 1 - k;  // the first pass's last chunks are the likeliest in a cache
-    const int i = tensor_of(tb, c);
-    if (f == 1.0 && tb.in[i] == tb.out[i]) continue;
-    const int64_t at = (int64_t)(c - tb.first[i]) * kChunk, len = min(tb.size[i] - at, kChunk);
-    if (tb.type[i] == GELIM_T_F32) scaled((const float*)tb.in[i] + at, (float*)tb.out[i] + at, len, (float)f);
-    else if (tb.type[i] == GELIM_T_BF16) scaled((const __bf16*)tb.in[i] + at, (__bf16*)tb.out[i] + at, len, (float)f);
-    else scaled((const _Float16*)tb.in[i] + at, (_Float16*)tb.out[i] + at, len, (float)f);
-  }
+  if (!APART && f == 1.0) return;
+  each_chunk(tb, [&](int i, int64_t at, int len, int type) {
+    const void* in = tb.in[i];
+    void* out = APART ? tb.out[i] : const_cast<void*>(in);
+    if (type == GELIM_T_F32) scaled((const float*)in + at, (float*)out + at, len, (float)f);
+    else if (type == GELIM_T_BF16) scaled((const __bf16*)in + at, (__bf16*)out + at, len, (float)f);
+    else scaled((const _Float16*)in + at, (_Float16*)out + at, len, (float)f);
+  });
 }
 
 // An output may be its own input and must not touch any other tensor.
@@ -158,39 +168,58 @@ int check_overlap(const void* const* in, void* const* out, const int64_t* sizes,
   return GELIM_OK;
 }
 
+// Calls launch(table, whether it is the first) for tables of all tensors.
+template <bool APART, class F>
+void each_table(const void* const* in, void* const* out, const int64_t* sizes, const int8_t* types, int64_t count,
+                F launch) {
+  Table<APART> t;
+  t.count = t.first[0] = 0;
+  bool first = true;
+  for (int64_t i = 0; i < count; ++i) {
+    if (!sizes[i]) continue;
+    const int64_t chunks = (sizes[i] + kChunk - 1) / kChunk;
+    if (t.count == t.kMost || t.first[t.count] + chunks > INT32_MAX) {
+      launch(t, first);
+      first = false;
+      t.count = 0;
+    }
+    t.in[t.count] = in[i];
+    if (APART) t.out[t.count] = out[i];
+    t.tail[t.count] = (uint16_t)(sizes[i] - (chunks - 1) * kChunk);
+    t.type[t.count++] = types[i];
+    t.first[t.count] = t.first[t.count - 1] + (int32_t)chunks;
+  }
+  launch(t, first);  // without any tensor as well: it clears the slots and writes the norm
+}
+
 int clip(const void* const* in, void* const* out, const int64_t* sizes, const int8_t* types, int64_t count,
          double max_norm, float* d_norm, double* slots, hipStream_t s) {
   if (!(max_norm >= 0)) return GELIM_FAIL(GELIM_E_ARG, "clip: max_norm must be a number and not negative");
   if (!d_norm || !slots) return GELIM_FAIL(GELIM_E_ARG, "clip: null norm or workspace");
-  std::vector<Table> tables(1);
-  int64_t most = 0;
-  tables[0].count = tables[0].chunks = 0;
+  int64_t chunks = 0;
+  bool apart = false;
   for (int64_t i = 0; i < count; ++i) {
     if (sizes[i] < 0 || (sizes[i] && (!in[i] || !out[i])) || types[i] < GELIM_T_F32 || types[i] > GELIM_T_F16)
       return GELIM_FAIL(GELIM_E_ARG, "clip: bad tensor " + std::to_string(i));
-    if (!sizes[i]) continue;
-    const int64_t chunks = (sizes[i] + kChunk - 1) / kChunk;
-    if (tables.back().count == kPerLaunch || tables.back().chunks + chunks > INT32_MAX) {
-      tables.emplace_back();
-      tables.back().count = tables.back().chunks = 0;
-    }
-    Table& t = tables.back();
-    if (chunks > INT32_MAX) return GELIM_FAIL(GELIM_E_ARG, "clip: tensor too large");
-    t.in[t.count] = in[i];
-    t.out[t.count] = out[i];
-    t.size[t.count] = sizes[i];
-    t.type[t.count] = types[i];
-    t.first[t.count++] = t.chunks;
-    t.chunks += (int32_t)chunks;
-    most = std::max<int64_t>(most, t.chunks);
+    if (sizes[i] > (int64_t)INT32_MAX * kChunk) return GELIM_FAIL(GELIM_E_ARG, "clip: tensor too large");
+    chunks += (sizes[i] + kChunk - 1) / kChunk;
+    apart |= sizes[i] && in[i] != out[i];
   }
   GELIM_TRY(check_overlap(in, out, sizes, types, count));
-  const int grid = (int)std::clamp<int64_t>(most, 1, kSlots);
-  for (size_t k = 0; k < tables.size(); ++k)
-    hipLaunchKernelGGL(squares_kernel, dim3(grid), dim3(kThreads), 0, s, tables[k], slots, k == 0);
-  for (size_t k = tables.size(); k-- > 0;)
-    hipLaunchKernelGGL(scale_kernel, dim3(grid), dim3(kThreads), 0, s, tables[k], slots, grid, max_norm,
-                       k == 0 ? d_norm : nullptr);
+  const int grid = (int)std::clamp<int64_t>(chunks, 1, kSlots);
+  each_table<false>(in, out, sizes, types, count, [&](const Table<false>& t, bool first) {
+    hipLaunchKernelGGL(squares_kernel, dim3(grid), dim3(kThreads), 0, s, t, slots, first);
+  });
+  if (apart)
+    each_table<true>(in, out, sizes, types, count, [&](const Table<true>& t, bool first) {
+      hipLaunchKernelGGL(scale_kernel<true>, dim3(grid), dim3(kThreads), 0, s, t, slots, grid, max_norm,
+                         first ? d_norm : nullptr);
+    });
+  else
+    each_table<false>(in, out, sizes, types, count, [&](const Table<false>& t, bool first) {
+      hipLaunchKernelGGL(scale_kernel<false>, dim3(grid), dim3(kThreads), 0, s, t, slots, grid, max_norm,
+                         first ? d_norm : nullptr);
+    });
   HIP_TRY(hipGetLastError());
   return GELIM_OK;
 }

@@ -29,6 +29,8 @@ _ARGS = struct.Struct("=21qd8q")
 def _stored(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """(t, distance of two rows as stored, 1 if stored transposed) of the last
     two dimensions; a copy where neither of them has unit stride."""
+    if t.is_contiguous():
+        return t, t.shape[-1], 0
     rs, cs = t.stride(-2), t.stride(-1)
     rows, cols = t.shape[-2:]
     if cs == 1 or cols == 1:

@@ -24,6 +24,28 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+_PTR, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.numel
+_DTYPE = torch.Tensor.dtype.__get__
+
+
+def _types(tensors: list[torch.Tensor]) -> bytes:
+    try:
+        return bytes(map(TYPES.__getitem__, map(_DTYPE, tensors)))
+    except KeyError as e:
+        raise TypeError(f"clip_global_norm takes float32, bfloat16 and float16, not {e.args[0]}") from None
+
+
+def _check_memory(tensors: list[torch.Tensor], dev: torch.device) -> bool:
+    """Whether all are contiguous; an error where one is elsewhere or not dense."""
+    if set(map(torch.Tensor.get_device, tensors)) != {dev.index}:
+        raise ValueError("all tensors must be on one device")
+    if all(map(torch.Tensor.is_contiguous, tensors)):
+        return True
+    if not all(map(_dense, tensors)):
+        raise ValueError("a tensor has gaps in memory, or overlaps itself")
+    return False
+
+
 def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
                      out: Sequence[torch.Tensor] | None = None) -> torch.Tensor:
     """Scales all tensors by min(1, max_norm / (norm + 1e-6)), norm the 2-norm of
@@ -31,13 +53,14 @@ def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
     the device, nothing waits for it).
 
     tensors: float32, bfloat16 and float16 in any mixture, on one device, each
-    without gaps in memory (any order of dimensions); none twice.
-    out: tensors of the same shapes, types and strides that get the scaled
-    copies, the inputs staying as they are; None: in place.
+    without gaps in memory (any order of dimensions).
+    out: tensors of the same types and shapes (and strides, if they are not
+    contiguous) that get the scaled copies, the inputs staying as they are;
+    None: in place.  What is written must not overlap anything else in the call.
     max_norm = math.inf only measures.  As the factor comes from the norm, a NaN anywhere
     makes all of them NaN, and an infinity makes the finite elements zero.
     Squares and their sum are held in float64, in an order that does not change
-    from run to run.  May be captured into a graph."""
+    from run to run.  Autograd records nothing.  May be captured into a graph."""
     tensors = list(tensors)
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
@@ -47,29 +70,20 @@ def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
     dev = tensors[0].device
     if dev.type != "cuda":
         raise ValueError("clip_global_norm needs CUDA tensors")
-    try:
-        types = bytes([TYPES[t.dtype] for t in tensors])
-    except KeyError as e:
-        raise TypeError(f"clip_global_norm takes float32, bfloat16 and float16, not {e.args[0]}") from None
-    if any(t.device != dev for t in tensors):
-        raise ValueError("all tensors must be on one device")
-    if not all(_dense(t) for t in tensors):
-        raise ValueError("a tensor has gaps in memory, or overlaps itself")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError("clip_global_norm is not recorded by autograd: pass the gradients themselves, or call it "
-                         "under torch.no_grad()")
-    src = array("Q", [t.data_ptr() for t in tensors])
+    types = _types(tensors)
+    sizes = array("q", map(_NUMEL, tensors))
+    contiguous = _check_memory(tensors, dev)
+    src = array("Q", map(_PTR, tensors))
     if out is None:
         dst = src
     else:
         out = list(out)
-        if len(out) != len(tensors):
-            raise ValueError("out must have one tensor per input")
-        for t, o in zip(tensors, out):
-            if o.dtype != t.dtype or o.device != dev or o.shape != t.shape or o.stride() != t.stride():
-                raise ValueError("each out must have the shape, type, strides and device of its input")
-        dst = array("Q", [t.data_ptr() for t in out])
-    sizes = array("q", [t.numel() for t in tensors])
+        if len(out) != len(tensors) or _types(out) != types or array("q", map(_NUMEL, out)) != sizes:
+            raise ValueError("out must have one tensor of the same type and shape per input")
+        if not (_check_memory(out, dev) and contiguous):
+            if any(o.shape != t.shape or o.stride() != t.stride() for t, o in zip(tensors, out)):
+                raise ValueError("each out must have the strides of its input")
+        dst = array("Q", map(_PTR, out))
     norm = torch.empty((), dtype=torch.float32, device=dev)
     lib = _native.lib()
     ws = torch.empty(lib.gelim_clip_workspace(len(tensors)), dtype=torch.uint8, device=dev)

@@ -21,7 +21,8 @@ def stream_handle(device: torch.device | None = None) -> int | None:
     """hipStream_t of torch's current stream on `device` (None on CPU)."""
     if device is not None and device.type != "cuda":
         return None
-    return torch.cuda.current_stream(device).cuda_stream
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    return torch._C._cuda_getCurrentRawStream(index)  # 2 us less than by way of a Stream object
 
 
 _DEDICATED: dict[tuple[int, str], torch.cuda.ExternalStream] = {}
