@@ -111,6 +111,20 @@ __device__ __forceinline__ typename Mma<T>::Frag load_part(const T* p, int64_t h
   return v;
 }
 
+// The same without a branch, for waves of which all lanes are at an edge or may be: kE loads in flight.  The row's
+// last element, have - 1 from p, exists also where have <= 0.
+template <class T>
+__device__ __forceinline__ typename Mma<T>::Frag load_edge(const T* p, int64_t have) {
+  constexpr int E = Mma<T>::kE;
+  typename Mma<T>::Frag v;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const T x = p[min((int64_t)e, have - 1)];
+    v[e] = e < have ? x : (T)0.f;
+  }
+  return v;
+}
+
 // kE rows (along the sum) of kE columns each, in registers, turned: out[j] holds column j's kE values.
 // 16-bit types: 32 byte permutes for 64 elements.
 template <class T>
@@ -161,8 +175,11 @@ struct Few {
   int64_t ldy;
 };
 
+// The first of the kE columns that a lane takes where W's rows run along memory: at the end of a row the lane takes
+// its last kE, some of them a neighbour's as well, who comes to the same sums.
+__device__ __forceinline__ int few_column(int N, int n, int E) { return N >= E ? min(n, N - E) : n; }
 constexpr int kFewFlight = 2;  // steps whose loads a wave has in flight
-constexpr int kFewGroups = 512;
+constexpr int kFewGroups = 256;
 // One wave: 16 kE columns of W, its steps of the sum; W_KC: W's sum runs along its rows in memory.
 // Each 16-byte load of 16 neighbouring lanes covers 256 bytes of a row of W (64 where W_KC: two steps make the line).
 template <class T, bool W_KC, int TT, bool EDGE>
@@ -184,12 +201,15 @@ __device__ __forceinline__ void few_steps(const Few& a, int n0, int s0, int s1, 
         w[q][j] = Frag{};
         if (!in) continue;
         if constexpr (W_KC) {
-          const int n = n0 + j * 16 + l16;
-          if constexpr (EDGE) w[q][j] = load_part(W + (int64_t)min(n, a.N - 1) * a.W.cs + k, a.C - k);
-          else w[q][j] = load16(W + (int64_t)n * a.W.cs + k);
+          const T* col = W + (int64_t)min(n0 + j * 16 + l16, a.N - 1) * a.W.cs;
+          if constexpr (EDGE) w[q][j] = load_edge(col + k, a.C - k);
+          else w[q][j] = load16(col + k);
         } else {
-          const int n = n0 + l16 * E;
-          if constexpr (EDGE) w[q][j] = load_part(W + (int64_t)(k + j) * a.W.rs + n, k + j < a.C ? a.N - n : 0);
+          const int n = few_column(a.N, n0 + l16 * E, E);
+          if constexpr (EDGE) {
+            w[q][j] = load_edge(W + (int64_t)min(k + j, a.C - 1) * a.W.rs + n, a.N - n);
+            if (k + j >= a.C) w[q][j] = Frag{};
+          }
           else w[q][j] = load16(W + (int64_t)(k + j) * a.W.rs + n);
         }
       }
@@ -198,7 +218,7 @@ __device__ __forceinline__ void few_steps(const Few& a, int n0, int s0, int s1, 
         const T* row = U + (int64_t)min(t * 16 + l16, a.rows.T - 1) * a.ldu;
         x[q][t] = Frag{};
         if (!in) continue;
-        if constexpr (EDGE) x[q][t] = load_part(row + k, a.C - k);
+        if constexpr (EDGE) x[q][t] = load_edge(row + k, a.C - k);
         else x[q][t] = load16(row + k);
       }
     }
@@ -219,6 +239,7 @@ __device__ __forceinline__ void few_steps(const Few& a, int n0, int s0, int s1, 
   }
 }
 
+constexpr int kLowPiece = 512;  // values of C: a wave's load of 16 bytes a lane, or two
 // low (T x r) of one row over one piece of C, on the vector units: F_i is read once per row that uses it.
 template <class T>
 __device__ __forceinline__ void few_low(const Few& a, int t, int split, float* lds) {
@@ -226,31 +247,49 @@ __device__ __forceinline__ void few_low(const Few& a, int t, int split, float* l
   constexpr int E = M::kE;
   const int i = adapter_of(a.rows, t);
   if (i < 0 || i >= a.rows.n) return;
-  const int piece = (a.C + a.low_splits - 1) / a.low_splits, c0 = split * piece, c1 = min(a.C, c0 + piece);
+  const int piece = (a.C + a.low_splits * kLowPiece - 1) / (a.low_splits * kLowPiece) * kLowPiece;
+  const int c0 = min(a.C, split * piece), c1 = min(a.C, c0 + piece);
   const T* u = (const T*)a.U + t * a.ldu;
   const T* f = (const T*)a.F.p + i * a.F.as;
   float* out = a.low + ((int64_t)split * a.rows.T + t) * a.r;
   if (a.F.rs != 1) {
-    // r values side by side: thread (c, chunk of E ranks)
+    // r values side by side: thread (c, chunk of E ranks); what a chunk reads behind the last rank is not used
     const int chunks = (a.r + E - 1) / E, lanes = 256 / chunks;
     const int j0 = threadIdx.x % chunks * E, cl = threadIdx.x / chunks;
+    const int64_t last = (int64_t)(a.C - 1) * a.F.rs + a.r - E - j0;  // the last offset that 16 bytes can be read from
+    const int whole = last < 0 ? c0 : a.F.rs == 0 ? c1 : (int)min((int64_t)c1, last / a.F.rs + 1);
     float acc[E] = {};
-    if (cl < lanes)
+    if (cl < lanes) {
+      int c = c0 + cl;
 #pragma unroll 4
-      for (int c = c0 + cl; c < c1; c += lanes) {
-        const auto v = load_part(f + c * a.F.rs + j0, a.r - j0);
+      for (; c < whole; c += lanes) {
+        const auto v = load16(f + c * a.F.rs + j0);
         const float x = (float)u[c];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += x * (float)v[e];
       }
-    // thread layout [cl][chunk][e] is [cl][rank]: sum over cl
+      for (; c < c1; c += lanes) {
+        const auto v = load_edge(f + c * a.F.rs + j0, a.r - j0);
+        const float x = (float)u[c];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += x * (float)v[e];
+      }
+    }
+    // thread layout [cl][chunk][e] is [cl][rank]: sum over cl in two steps
 #pragma unroll
     for (int e = 0; e < E; ++e) lds[threadIdx.x * E + e] = acc[e];
     __syncthreads();
-    const int width = chunks * E;
-    for (int j = threadIdx.x; j < a.r; j += 256) {
-      float s = 0.f;
-      for (int c = 0; c < lanes; ++c) s += lds[c * width + j];
+    const int width = chunks * E, shares = min(256 / width, 16);
+    const int j = threadIdx.x % width, share = threadIdx.x / width;
+    float s = 0.f;
+    if (share < shares)
+      for (int c = share; c < lanes; c += shares) s += lds[c * width + j];
+    __syncthreads();
+    if (share < shares) lds[share * width + j] = s;
+    __syncthreads();
+    if (share == 0 && j < a.r) {
+      s = 0.f;
+      for (int c = 0; c < shares; ++c) s += lds[c * width + j];
       out[j] = s;
     }
   } else {
@@ -291,8 +330,9 @@ __global__ __launch_bounds__(256) void few_kernel(Few a) {
   const int steps = (a.C + M::kStep - 1) / M::kStep, parts = a.splits * 4, part = split * 4 + wave;
   const int s0 = (int)((int64_t)steps * part / parts), s1 = (int)((int64_t)steps * (part + 1) / parts);
   f4 acc[E][TT] = {};
-  if (n0 + kCols <= a.N && s1 * M::kStep <= a.C) few_steps<T, W_KC, TT, false>(a, n0, s0, s1, acc);
-  else few_steps<T, W_KC, TT, true>(a, n0, s0, s1, acc);
+  const int whole = W_KC || a.N >= E ? min(s1, a.C / M::kStep) : s0;  // steps before one that ends behind the sum
+  few_steps<T, W_KC, TT, false>(a, n0, s0, whole, acc);
+  few_steps<T, W_KC, TT, true>(a, n0, max(s0, whole), s1, acc);
   // waves 2 and 3 hand theirs to 0 and 1, then 1 to 0
 #pragma unroll
   for (int half = 2; half >= 1; half /= 2) {
@@ -315,17 +355,17 @@ __global__ __launch_bounds__(256) void few_kernel(Few a) {
   for (int t = 0; t < TT; ++t) {
     const int row = t * 16 + l16;
     if (row >= a.rows.T) continue;
-    float* out = a.part + ((int64_t)split * a.rows.T + row) * a.ldp + n0;
+    float* out = a.part + ((int64_t)split * a.rows.T + row) * a.ldp;
     if constexpr (W_KC) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) *(f4*)(out + j * 16 + g * 4) = acc[j][t];
+      for (int j = 0; j < E; ++j) *(f4*)(out + n0 + j * 16 + g * 4) = acc[j][t];
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < E; j += 4) {
-          const f4 v = {acc[j][t][i], acc[j + 1][t][i], acc[j + 2][t][i], acc[j + 3][t][i]};
-          *(f4*)(out + (g * 4 + i) * E + j) = v;
+          const Four<float> v = {acc[j][t][i], acc[j + 1][t][i], acc[j + 2][t][i], acc[j + 3][t][i]};
+          *(Four<float>*)(out + few_column(a.N, n0 + (g * 4 + i) * E, E) + j) = v;
         }
     }
   }
@@ -382,8 +422,20 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] += s[j] * (float)v.v[e];
       }
+    } else if (a.G.rs == 1) {
+      // ranks side by side: 16 bytes of them at a time
+      constexpr int E = Mma<T>::kE;
+      const int64_t last = (a.N - 1) * a.G.cs + a.r - E;
+      for (int j = part * E; j < a.r; j += kShare * E)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t at = min(n + e, a.N - 1) * a.G.cs + j;
+          const auto v = at <= last ? load16(G + at) : load_edge(G + at, a.r - j);
+#pragma unroll
+          for (int k = 0; k < E; ++k)
+            if (j + k < a.r) acc[e] += s[j + k] * (float)v[k];
+        }
     } else {
-#pragma unroll 2
       for (int j = part; j < a.r; j += kShare)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
