@@ -114,12 +114,12 @@ __device__ __forceinline__ typename Mma<T>::Frag load_part(const T* p, int64_t h
 // The same without a branch, for waves of which all lanes are at an edge or may be: kE loads in flight.  The row's
 // last element, have - 1 from p, exists also where have <= 0.
 template <class T>
-__device__ __forceinline__ typename Mma<T>::Frag load_edge(const T* p, int64_t have) {
+__device__ __forceinline__ typename Mma<T>::Frag load_edge(const T* p, int have) {
   constexpr int E = Mma<T>::kE;
   typename Mma<T>::Frag v;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const T x = p[min((int64_t)e, have - 1)];
+    const T x = p[min(e, have - 1)];
     v[e] = e < have ? x : (T)0.f;
   }
   return v;
@@ -178,10 +178,10 @@ struct Few {
 // The first of the kE columns that a lane takes where W's rows run along memory: at the end of a row the lane takes
 // its last kE, some of them a neighbour's as well, who comes to the same sums.
 __device__ __forceinline__ int few_column(int N, int n, int E) { return N >= E ? min(n, N - E) : n; }
-constexpr int kFewFlight = 2;  // steps whose loads a wave has in flight
 constexpr int kFewGroups = 256;
 // One wave: 16 kE columns of W, its steps of the sum; W_KC: W's sum runs along its rows in memory.
 // Each 16-byte load of 16 neighbouring lanes covers 256 bytes of a row of W (64 where W_KC: two steps make the line).
+// One step's loads in flight: with two, fewer waves fit a SIMD, and 32 rows of 4096 x 4096 took 14.2 instead of 10.9 us.
 template <class T, bool W_KC, int TT, bool EDGE>
 __device__ __forceinline__ void few_steps(const Few& a, int n0, int s0, int s1, f4 (&acc)[Mma<T>::kE][TT]) {
   using M = Mma<T>;
@@ -190,52 +190,41 @@ __device__ __forceinline__ void few_steps(const Few& a, int n0, int s0, int s1, 
   const int l16 = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
   const T* W = (const T*)a.W.p;
   const T* U = (const T*)a.U;
-  for (int s = s0; s < s1; s += kFewFlight) {
-    Frag w[kFewFlight][E], x[kFewFlight][TT];
+  for (int s = s0; s < s1; ++s) {
+    const int k = s * M::kStep + g * E;
+    Frag w[E], x[TT];
 #pragma unroll
-    for (int q = 0; q < kFewFlight; ++q) {
-      const bool in = s + q < s1;  // a step behind the last one: zeros
-      const int k = (in ? s + q : s) * M::kStep + g * E;
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        w[q][j] = Frag{};
-        if (!in) continue;
-        if constexpr (W_KC) {
-          const T* col = W + (int64_t)min(n0 + j * 16 + l16, a.N - 1) * a.W.cs;
-          if constexpr (EDGE) w[q][j] = load_edge(col + k, a.C - k);
-          else w[q][j] = load16(col + k);
+    for (int j = 0; j < E; ++j) {
+      if constexpr (W_KC) {
+        const T* col = W + (int64_t)min(n0 + j * 16 + l16, a.N - 1) * a.W.cs;
+        if constexpr (EDGE) w[j] = load_edge(col + k, a.C - k);
+        else w[j] = load16(col + k);
+      } else {
+        const int n = few_column(a.N, n0 + l16 * E, E);
+        if constexpr (EDGE) {
+          w[j] = load_edge(W + (int64_t)min(k + j, a.C - 1) * a.W.rs + n, a.N - n);
+          if (k + j >= a.C) w[j] = Frag{};
         } else {
-          const int n = few_column(a.N, n0 + l16 * E, E);
-          if constexpr (EDGE) {
-            w[q][j] = load_edge(W + (int64_t)min(k + j, a.C - 1) * a.W.rs + n, a.N - n);
-            if (k + j >= a.C) w[q][j] = Frag{};
-          }
-          else w[q][j] = load16(W + (int64_t)(k + j) * a.W.rs + n);
+          w[j] = load16(W + (int64_t)(k + j) * a.W.rs + n);
         }
       }
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const T* row = U + (int64_t)min(t * 16 + l16, a.rows.T - 1) * a.ldu;
-        x[q][t] = Frag{};
-        if (!in) continue;
-        if constexpr (EDGE) x[q][t] = load_edge(row + k, a.C - k);
-        else x[q][t] = load16(row + k);
-      }
     }
 #pragma unroll
-    for (int q = 0; q < kFewFlight; ++q) {
+    for (int t = 0; t < TT; ++t) {
+      const T* row = U + (int64_t)min(t * 16 + l16, a.rows.T - 1) * a.ldu;
+      if constexpr (EDGE) x[t] = load_edge(row + k, a.C - k);
+      else x[t] = load16(row + k);
+    }
+    if constexpr (!W_KC) {
       Frag v[E];
-      if constexpr (W_KC) {
+      turn<T>(w, v);
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = w[q][j];
-      } else {
-        turn<T>(w[q], v);
-      }
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-#pragma unroll
-        for (int t = 0; t < TT; ++t) acc[j][t] = M::mma(v[j], x[q][t], acc[j][t]);
+      for (int j = 0; j < E; ++j) w[j] = v[j];
     }
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) acc[j][t] = M::mma(w[j], x[t], acc[j][t]);
   }
 }
 
@@ -313,7 +302,7 @@ __device__ __forceinline__ void few_low(const Few& a, int t, int split, float* l
 // The first launch: blocks x splits workgroups of the large product, then T x low_splits of the low one.
 // Four waves share a block of 16 kE columns and cut its steps once more; their sums meet in LDS.
 template <class T, bool W_KC, int TT>
-__global__ __launch_bounds__(256) void few_kernel(Few a) {
+__global__ __launch_bounds__(256, TT <= 2 ? 3 : 2) void few_kernel(Few a) {
   using M = Mma<T>;
   constexpr int E = M::kE, kCols = 16 * E;
   constexpr int kFrags = E * TT;
