@@ -360,7 +360,7 @@ __global__ __launch_bounds__(256, TT <= 2 ? 3 : 2) void few_kernel(Few a) {
   }
 }
 
-// The second launch: sums of the pieces, the product with G_i, the result.
+// The second launch: sums of the pieces, the product with G_i (r = 0: it is in them), the result.
 // A workgroup takes 256 columns of one row, its four waves sharing the pieces and the ranks, or (ONE_ROW false: with
 // enough rows to fill the chip) of four rows, a wave each.
 struct Finish {
@@ -506,52 +506,73 @@ struct Prepare {
   int order_groups;  // n + 1, or 0: the order is not needed
   Copy copy[kCopies];
   int copies;
+  int* counter;  // set to zero for the launches behind this one
+  int counters;
 };
 
 // Adapter i's rows (i = n: those without one), in order, by one workgroup:
-// it counts the rows of lower adapters, then writes its own behind those.
+// it counts the rows of lower adapters, then writes its own behind those.  A thread takes kOrder rows side by side.
+constexpr int kOrder = 16, kPrepare = 256;
 __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
-  __shared__ int lower[16], own[16];
+  __shared__ int sums[2][kPrepare / 64];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = p.rows.n;
-  auto adapter = [&](int t) {
-    const int a = p.rows.index ? p.rows.index[t] : 0;
-    return a < 0 || a >= n ? n : a;
+  int id[kOrder];
+  auto fetch = [&](int64_t t0) {  // adapters of this thread's rows; behind the last row -1
+#pragma unroll
+    for (int q = 0; q < kOrder; ++q) {
+      const int64_t t = t0 + threadIdx.x * kOrder + q;
+      const int a = t < p.rows.T ? p.rows.index[t] : 0;
+      id[q] = t >= p.rows.T ? -1 : a < 0 || a >= n ? n : a;
+    }
   };
   int c = 0;
-  for (int64_t t = threadIdx.x; t < p.rows.T; t += 1024) c += adapter((int)t) < i;
+  for (int64_t t0 = 0; t0 < p.rows.T; t0 += kPrepare * kOrder) {
+    fetch(t0);
+#pragma unroll
+    for (int q = 0; q < kOrder; ++q) c += id[q] >= 0 && id[q] < i;
+  }
 #pragma unroll
   for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
-  if (lane == 0) lower[wave] = c;
+  if (lane == 0) sums[0][wave] = c;
   __syncthreads();
   int at = 0;
-  for (int w = 0; w < 16; ++w) at += lower[w];
+  for (int w = 0; w < kPrepare / 64; ++w) at += sums[0][w];
   if (threadIdx.x == 0) p.start[i] = at;
-  for (int64_t t0 = 0; t0 < p.rows.T; t0 += 1024) {
-    const int64_t t = t0 + threadIdx.x;
-    const bool mine = t < p.rows.T && adapter((int)t) == i;
-    const uint64_t all = __ballot(mine);
-    if (lane == 0) own[wave] = __popcll(all);
-    __syncthreads();
-    int before = at;
-    for (int w = 0; w < 16; ++w) {
-      if (w < wave) before += own[w];
-      at += own[w];
+  for (int64_t t0 = 0; t0 < p.rows.T; t0 += kPrepare * kOrder) {
+    if (p.rows.T > kPrepare * kOrder) fetch(t0);  // otherwise they are still here
+    int mine = 0;
+#pragma unroll
+    for (int q = 0; q < kOrder; ++q) mine += id[q] == i;
+    int upto = mine;  // of this and the lower lanes
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int v = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += v;
     }
-    if (mine) p.perm[before + __popcll(all & ((1ull << lane) - 1))] = (int32_t)t;
     __syncthreads();
+    if (lane == 63) sums[1][wave] = upto;
+    __syncthreads();
+    int place = at + upto - mine;
+    for (int w = 0; w < kPrepare / 64; ++w) {
+      if (w < wave) place += sums[1][w];
+      at += sums[1][w];
+    }
+#pragma unroll
+    for (int q = 0; q < kOrder; ++q)
+      if (id[q] == i) p.perm[place++] = (int32_t)(t0 + threadIdx.x * kOrder + q);
   }
 }
 
-// 64 KB of a copy whose source runs along its rows: 16 bytes a thread, from any element's address.
-constexpr int kStraight = 4096;  // chunks of 16 bytes
+// 16 KB of a copy whose source runs along its rows: 16 bytes a thread, from any element's address.
+constexpr int kStraight = 1024;  // chunks of 16 bytes
 template <class T>
 __device__ __forceinline__ void copy_straight(const Copy& c, int part) {
   constexpr int E = Mma<T>::kE;
   const int across = c.ld / E;
   const int64_t all = (int64_t)c.count * c.rows * across;
 #pragma unroll
-  for (int q = 0; q < kStraight / 1024; ++q) {
-    const int64_t o = (int64_t)part * kStraight + q * 1024 + threadIdx.x;
+  for (int q = 0; q < kStraight / kPrepare; ++q) {
+    const int64_t o = (int64_t)part * kStraight + q * kPrepare + threadIdx.x;
     if (o >= all) return;
     const int64_t row = o / across, m = row / c.rows, i = row % c.rows;
     const int j = (int)(o % across) * E;
@@ -560,45 +581,64 @@ __device__ __forceinline__ void copy_straight(const Copy& c, int part) {
   }
 }
 
-// One 64 x 64 tile of a copy, read along the source's memory and written along the destination's.
+// One 64 x 64 tile of a copy, read along the source's memory and written along the destination's, 16 bytes a thread.
 template <class T>
 __device__ __forceinline__ void copy_tile(const Copy& c, int tile) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int E = M::kE, kAcross = kCopyTile / E, kChunks = kCopyTile * kAcross;
   __shared__ T lds[kCopyTile][kCopyTile + 2];
   const int across = (c.ld + kCopyTile - 1) / kCopyTile, down = (c.rows + kCopyTile - 1) / kCopyTile;
   const int m = tile / (across * down), r0 = tile / across % down * kCopyTile, c0 = tile % across * kCopyTile;
   const T* src = (const T*)c.src.p + m * c.src.as;
   T* dst = (T*)c.dst + (int64_t)m * c.rows * c.ld;
-  const int fast = threadIdx.x % 64, slow = threadIdx.x / 64;
+  const bool along = c.src.cs == 1;
+  Frag v[kChunks / kPrepare];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int a = slow + 16 * k;
-    const int i = c.src.cs == 1 ? a : fast, j = c.src.cs == 1 ? fast : a;
-    lds[i][j] = r0 + i < c.have && c0 + j < c.cols ? src[(r0 + i) * c.src.rs + (c0 + j) * c.src.cs] : (T)0.f;
+  for (int q = 0; q < kChunks / kPrepare; ++q) {
+    const int o = q * kPrepare + threadIdx.x, slow = o / kAcross, fast = o % kAcross * E;
+    const int i = r0 + (along ? slow : fast), j = c0 + (along ? fast : slow);
+    const bool in = i < c.have && j < c.cols;
+    v[q] = load_part(src + i * c.src.rs + j * c.src.cs, !in ? 0 : along ? c.cols - j : c.have - i);
+  }
+#pragma unroll
+  for (int q = 0; q < kChunks / kPrepare; ++q) {
+    const int o = q * kPrepare + threadIdx.x, slow = o / kAcross, fast = o % kAcross * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (along) lds[slow][fast + e] = v[q][e];
+      else lds[fast + e][slow] = v[q][e];
+    }
   }
   __syncthreads();
-  if (c.steps) {
-    using M = Mma<T>;
-    constexpr int kBlock = 64 * M::kE, kInTile = kCopyTile / M::kStep;
-    const int blocks = c.rows / 16, here = min(4, blocks - r0 / 16);  // of 16 rows, in all and in this tile
-    for (int o = threadIdx.x; o < kInTile * here * kBlock; o += 1024) {
-      const int step = o / (here * kBlock), rb = o / kBlock % here, lane = o / M::kE % 64;
-      dst[((int64_t)(c0 / M::kStep + step) * blocks + r0 / 16 + rb) * kBlock + o % kBlock] =
-          lds[rb * 16 + lane % 16][step * M::kStep + lane / 16 * M::kE + o % M::kE];
-    }
-    return;
-  }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int i = slow + 16 * k;
-    if (r0 + i < c.rows && c0 + fast < c.ld) dst[(int64_t)(r0 + i) * c.ld + c0 + fast] = lds[i][fast];
+  for (int q = 0; q < kChunks / kPrepare; ++q) {
+    int o = q * kPrepare + threadIdx.x, i, j;
+    T* to;
+    if (c.steps) {
+      const int blocks = c.rows / 16, here = min(4, blocks - r0 / 16);  // of 16 rows, in all and in this tile
+      const int step = o / (here * 64), rb = o / 64 % here, lane = o % 64;
+      if (step >= kCopyTile / M::kStep) continue;
+      i = rb * 16 + lane % 16, j = step * M::kStep + lane / 16 * E;
+      to = dst + (((int64_t)(c0 / M::kStep + step) * blocks + r0 / 16 + rb) * 64 + lane) * E;
+    } else {
+      i = o / kAcross, j = o % kAcross * E;
+      if (r0 + i >= c.rows || c0 + j >= c.ld) continue;
+      to = dst + (int64_t)(r0 + i) * c.ld + c0 + j;
+    }
+    Frag w;
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = lds[i][j + e];
+    *(Frag*)to = w;
   }
 }
 
-// The first launch: the order, the factors laid out for the matrix units, and
+// The first launch: counters cleared, the order, the factors laid out for the matrix units, and
 // an operand whose rows do not begin at multiples of 16 bytes copied to where they do.
 template <class T>
-__global__ __launch_bounds__(1024) void prepare_kernel(Prepare p) {
+__global__ __launch_bounds__(kPrepare) void prepare_kernel(Prepare p) {
   int b = blockIdx.x;
+  for (int c = b * kPrepare + threadIdx.x; c < p.counters; c += gridDim.x * kPrepare) p.counter[c] = 0;
   if (b < p.order_groups) return order_rows(p, b);
   b -= p.order_groups;
   int k = p.copies - 1;
@@ -609,7 +649,8 @@ __global__ __launch_bounds__(1024) void prepare_kernel(Prepare p) {
 
 // low (place, rank) = U F_i, 32 places of one adapter by a workgroup, whose waves cut the sum.
 // F is laid out in fragments, ldf values along the sum with zeros behind C.  Bound by
-// reading U and, for every 32 rows, F_i: each wave keeps several steps' loads in flight.
+// reading U and, for every 32 rows, F_i: each wave keeps several steps' loads in flight.  With few rows several
+// workgroups cut the sum once more; the last of them to end adds their parts, always in the same order.
 // 16-bit types: also as the sum of two values of the type, 8 ranks' upper and then lower parts side by side, for
 // the matrix units of the large product.  One value's rounding alone would be as large as the
 // result's.  fp16: a row is first brought to below 2^14 by a power of two (`by`), as it may be beyond the type's range.
@@ -618,7 +659,9 @@ struct Low {
   int64_t ldu;
   float *low, *by;
   void* split;
-  int cu, ldf, pieces;  // cu: values in a row of U, a multiple of 16 bytes
+  int cu, ldf, pieces, splits;  // cu: values in a row of U, a multiple of 16 bytes
+  float* part;                  // split, place, rank; with splits > 1
+  int* arrived;                 // of each piece
 };
 struct LowPair {
   Low p[2];
@@ -646,7 +689,9 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
   constexpr int E = M::kE, rp = 16 * RB, kWaves = kLowWaves;
   __shared__ f4 lds[kWaves / 2][RB * 2][64];
   const Low& a = both.p[blockIdx.y];
-  const Piece pc = piece_of(both.order, both.rows, blockIdx.x, kLowRows);
+  const int piece = blockIdx.x % a.pieces, split = blockIdx.x / a.pieces;
+  if (split >= a.splits) return;
+  const Piece pc = piece_of(both.order, both.rows, piece, kLowRows);
   if (pc.count == 0) return;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
   const T* u[2];
@@ -655,7 +700,8 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
     u[t] = (const T*)a.U + row_at(both.order, pc.begin + min(t * 16 + l16, pc.count - 1)) * a.ldu;
   const Frag* f = (const Frag*)((const T*)a.F + (int64_t)pc.adapter * rp * a.ldf) + lane;
   const int steps = (a.cu + M::kStep - 1) / M::kStep;
-  const int s0 = (int)((int64_t)steps * wave / kWaves), s1 = (int)((int64_t)steps * (wave + 1) / kWaves);
+  const int parts = kWaves * a.splits, mine = split * kWaves + wave;
+  const int s0 = (int)((int64_t)steps * mine / parts), s1 = (int)((int64_t)steps * (mine + 1) / parts);
   f4 acc[RB][2] = {};
   constexpr int kFlight = RB <= 2 ? 4 : RB == 4 ? 2 : 1;  // by the registers of two workgroups a CU
   for (int s = s0; s < s1; s += kFlight) {
@@ -698,6 +744,38 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
     __syncthreads();
   }
   if (wave) return;
+  if (a.splits > 1) {
+    // The parts go past the caches (agent-scope relaxed atomics), so that no cache has to be written back or
+    // dropped as by a fence; the count goes up when they have arrived (vmcnt 0).
+    auto part = [&](int p, int t, int j) {
+      const int64_t at = pc.begin + min(t * 16 + l16, pc.count - 1);
+      return a.part + ((int64_t)p * both.rows.T + at) * rp + j * 16 + g * 4;
+    };
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < RB; ++j)
+        if (t * 16 + l16 < pc.count)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            __hip_atomic_store(part(split, t, j) + e, acc[j][t][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    int before = 0;
+    if (lane == 0) before = __hip_atomic_fetch_add(a.arrived + piece, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__builtin_amdgcn_readfirstlane(before) != a.splits - 1) return;
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        f4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < a.splits; ++p)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] += __hip_atomic_load(part(p, t, j) + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        acc[j][t] = v;
+      }
+  }
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const bool in = t * 16 + l16 < pc.count;
@@ -785,7 +863,8 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   constexpr int TT = BT / WT / 32, TN = BN / WN / 32;
   constexpr int kLoadU = BT / (WT * WN * 8), kLoadW = BN / (WT * WN * 8);
   constexpr int kRowChunks = BN / E;  // chunks in a row of W's tile if not W_KC
-  __shared__ __attribute__((aligned(16))) T us0[BT * BK], us1[BT * BK], ws0[BN * BK], ws1[BN * BK];
+  __shared__ __attribute__((aligned(16))) T lds[2 * (BT + BN) * BK];
+  constexpr int us0 = 0, us1 = BT * BK, ws0 = 2 * BT * BK, ws1 = ws0 + BN * BK;  // places in it
 
   // Workgroups go to the 8 XCDs in turn: each XCD gets neighbouring tiles, and those that run at a time (a 256 x
   // 256 tile or two smaller ones on each of 32 CUs) are kGroup tiles high and about as wide, so that its L2 reads few
@@ -826,65 +905,80 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     }
   }
   const int64_t w_step = W_KC ? BK : BK * a.ldw;
+  // W not along the sum: loads whose rows' columns are swapped alike differ by whole rows, so one address serves them
+  constexpr int kLoadRows = W_KC ? 1 : 64 / kRowChunks;
+  auto twin = [](int q) constexpr {
+    if (W_KC) return q;
+    for (int p = 0; p < q; ++p)
+      if (sizeof(T) == 2 ? ((p ^ q) * kLoadRows & 11) == 0 : ((p ^ q) * kLoadRows & 4) == 0) return p;
+    return q;
+  };
   // the q-th load of a tile; guard: with zeros behind the sum's end, also for tiles that nothing uses
-  auto load = [&](auto guard, int kt, T* us, T* ws, int q) {
+  auto load = [&](auto guard, int kt, int us, int ws, int q) {
     const int k = kt * BK;
     const void* from;
     unsigned to;
     if (q < kLoadU) {
       from = up[q] + k;
       if (decltype(guard)::value && k + uk[q] >= a.cu) from = g_zeros;
-      to = lds_address(us + (wave * kLoadU + q) * 64 * E);
+      to = lds_address(lds + us + (wave * kLoadU + q) * 64 * E);
     } else {
       q -= kLoadU;
-      from = wp[q] + kt * w_step;
+      from = wp[twin(q)] + (kt * w_step + (q - twin(q)) * kLoadRows * a.ldw);
       if (decltype(guard)::value && k + wk[q] >= a.cw) from = g_zeros;
-      to = lds_address(ws + (wave * kLoadW + q) * 64 * E);
+      to = lds_address(lds + ws + (wave * kLoadW + q) * 64 * E);
     }
     to_lds(from, __builtin_amdgcn_readfirstlane(to));
   };
 
-  f16 acc[TN][TT] = {};
+  f16 acc[TN][TT] = {}, total[sizeof(T) == 4 ? TN : 1][TT] = {};
   struct Frags {
     Frag x[TT], w[TN];
   };
+  // Where this lane's fragments begin in a tile.  A quarter moves the chunk's number by an exclusive or, which the
+  // swap above leaves alone, or the row; the rest are constant distances.
+  const int u_at = (wt + l32) * BK + (half ^ (l32 >> 1 & 7)) * E;
+  int w_at[W_KC ? 1 : TN];
+  if constexpr (W_KC) {
+    w_at[0] = (wn + l32) * BK + (half ^ (l32 >> 1 & 7)) * E;
+  } else {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = wn + j * 32 + (sizeof(T) == 2 ? l32 / 16 * 16 + lane % 4 * 4 : l32);
+      const int k = sizeof(T) == 2 ? half * 8 + lane % 16 / 4 : half * 4;
+      w_at[j] = k * BN + ((n / E) ^ swap_columns<T, kRowChunks>(k)) * E + n % E;
+    }
+  }
   // the q-th fragment of a quarter
-  auto read = [&](const T* us, const T* ws, int part, Frags& f, int q) {
+  auto read = [&](int us, int ws, int part, Frags& f, int q) {
     if (q < TT) {
-      const int i = wt + q * 32 + l32;
-      f.x[q] = *(const Frag*)&us[i * BK + ((part * 2 + half) ^ (i >> 1 & 7)) * E];
+      f.x[q] = *(const Frag*)&lds[us + (u_at ^ (part * 2 * E)) + q * 32 * BK];
       return;
     }
     const int j = q - TT;
     if constexpr (W_KC) {
-      const int i = wn + j * 32 + l32;
-      f.w[j] = *(const Frag*)&ws[i * BK + ((part * 2 + half) ^ (i >> 1 & 7)) * E];
+      f.w[j] = *(const Frag*)&lds[ws + (w_at[0] ^ (part * 2 * E)) + j * 32 * BK];
     } else if constexpr (sizeof(T) == 2) {
       // 16 lanes read 4 rows (of the sum) x 16 columns, 8 bytes each, and get their column's 4 values
       s8 v;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = part * 16 + half * 8 + h * 4 + lane % 16 / 4;
-        const int chunk = ((wn + j * 32) / 8 + l32 / 16 * 2 + lane % 4 / 2) ^ swap_columns<T, kRowChunks>(k);
         const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s4*)&ws[k * BN + chunk * 8 + lane % 2 * 4]);
+            (__attribute__((address_space(3))) s4*)&lds[ws + w_at[j] + (part * 16 + h * 4) * BN]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[h * 4 + e] = r[e];
       }
       f.w[j] = __builtin_bit_cast(Frag, v);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = part * 8 + half * 4 + e, n = wn + j * 32 + l32;
-        f.w[j][e] = ws[k * BN + ((n / E) ^ swap_columns<T, kRowChunks>(k)) * E + n % E];
-      }
+      for (int e = 0; e < 4; ++e) f.w[j][e] = lds[ws + w_at[j] + (part * 8 + e) * BN];
     }
   };
   // A quarter: `now` is multiplied; in between, in this order, quarter `part` is read into `next` in the first
   // half and, with kLoads, a tile is loaded.
   constexpr int kMma = TT * TN, kReads = TT + TN, kLoads = kLoadU + kLoadW;
-  auto quarter = [&](const Frags& now, const T* us, const T* ws, int part, Frags& next, auto loads, auto guard, int kt,
-                     T* us_to, T* ws_to) {
+  auto quarter = [&](const Frags& now, int us, int ws, int part, Frags& next, auto loads, auto guard, int kt,
+                     int us_to, int ws_to) {
 #pragma unroll
     for (int m = 0; m < kMma; ++m) {
       constexpr int kSpan = (kMma + 1) / 2;
@@ -901,7 +995,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   };
   Frags f0, f1;
   // one tile from its place in LDS; its first quarter is in f0, and the next tile's will be
-  auto step = [&](auto guard, int kt, T* us, T* ws, const T* us_next, const T* ws_next) {
+  auto step = [&](auto guard, int kt, int us, int ws, int us_next, int ws_next) {
     constexpr std::false_type no{};
     quarter(f0, us, ws, 1, f1, no, no, 0, us, ws);
     quarter(f1, us, ws, 2, f0, no, no, 0, us, ws);
@@ -915,51 +1009,110 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   for (int q = 0; q < kLoads; ++q) load(std::true_type{}, k0, us0, ws0, q);
 #pragma unroll
   for (int q = 0; q < kLoads; ++q) load(std::true_type{}, k0 + 1, us1, ws1, q);
-  if constexpr (!SPLIT) {
-    // The accumulators begin with s_i (U F_i) G_i, while the first tiles load: for each adapter among 32 rows the
-    // product of all of them, kept where it is theirs.
+  unsigned wrong = 0;  // rows of this lane whose adapter does not exist
+  {
+  // this lane's rows, and their adapters
+  int row[TT], mine[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) row[t] = (int)row_at(a.order, min(t0 + wt + t * 32 + l32, a.rows.T - 1));
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    mine[t] = adapter_of(a.rows, row[t]);
+    if (t0 + wt + t * 32 + l32 >= a.rows.T) mine[t] = -1;
+    wrong |= (unsigned)(mine[t] < -1 || mine[t] >= a.rows.n) << t;
+  }
+    // The accumulators begin with s_i (U F_i) G_i, while the first tiles load (SPLIT: each part of the sum with some
+    // of the adapters and ranks).  U F_i comes as two values of the type
+    // (fp32: itself), so 8 ranks are one step.  All loads of kBatch steps come before their products.
+    auto has = [&](int t) { return mine[t] >= 0 && mine[t] < a.rows.n; };
+    auto place = [&](int t) { return (int64_t)min(t0 + wt + t * 32 + l32, a.rows.T - 1); };
+    auto x_of = [&](int t, int b) {
+      const Frag* at = sizeof(T) == 2 ? (const Frag*)((const T*)a.split + place(t) * 2 * a.rp) + half
+                                      : (const Frag*)(a.low + place(t) * a.rp) + half;
+      Frag x = {};
+      if (b < a.rp && has(t)) x = at[b / 8 * 2];
+      return x;
+    };
+    auto w_of = [&](int cur, int j, int b) {
+      const int n = min(n0 + wn + j * 32 + l32, a.N - 1);
+      Frag w = {};
+      if (b < a.rp)
+        w = *(const Frag*)((const T*)a.G + ((int64_t)cur * a.N + n) * a.rp + b + (sizeof(T) == 2 ? 0 : half * 4));
+      return w;
+    };
+    auto factor = [&](int t, int cur) {
+      float f = scale_of(a.rows, cur);
+      if constexpr (std::is_same_v<T, _Float16>) f *= has(t) ? a.by[place(t)] : 0.f;
+      return f;
+    };
+    constexpr int kBatch = BT == 256 ? 1 : 2;  // by the registers
+    const int shares = SPLIT ? a.splits : 1, share = SPLIT ? blockIdx.y : 0;
+    uint64_t some[TT], any = 0;
+    int first = -1;
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      const int at = t0 + wt + t * 32 + l32;
-      const int64_t place = min(at, a.rows.T - 1);
-      const int mine = at < a.rows.T ? adapter_of(a.rows, row_at(a.order, place)) : -1;
-      const bool has = mine >= 0 && mine < a.rows.n;
-      // U F_i comes as two values of the type (fp32: itself), so 8 ranks are one step.  All loads of kBatch
-      // steps come before their products: nothing else hides their latency here.
-      constexpr int kBatch = 4;
-      uint64_t left = __ballot(has);
-      const Frag* x_at = sizeof(T) == 2 ? (const Frag*)((const T*)a.split + place * 2 * a.rp) + half
-                                        : (const Frag*)(a.low + place * a.rp) + half;
-      while (left) {
-        const int cur = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-        left &= ~__ballot(mine == cur);
-        f16 d[TN] = {};
-        for (int b = 0; b < a.r; b += 8 * kBatch) {
-          Frag x[kBatch], w[TN][kBatch];
+      some[t] = __ballot(has(t));
+      if (some[t] && !any) first = __builtin_amdgcn_readlane(mine[t], __builtin_ctzll(some[t]));
+      any |= some[t];
+    }
+    bool one = true;
 #pragma unroll
-          for (int q = 0; q < kBatch; ++q) {
-            const bool more = b + q * 8 < a.rp;
-            x[q] = Frag{};
-            if (more && has) x[q] = x_at[(b / 8 + q) * 2];
+    for (int t = 0; t < TT; ++t) one = one && __ballot(has(t) && mine[t] != first) == 0;
+    if (any && one) {
+      // one adapter among all of the wave's rows: straight into the accumulators, zeros again where it is no row's
+      for (int b = share * 8 * kBatch; b < a.r; b += shares * 8 * kBatch) {
+        Frag x[TT][kBatch], w[TN][kBatch];
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-              const int n = min(n0 + wn + j * 32 + l32, a.N - 1);
-              w[j][q] = Frag{};
-              if (more)
-                w[j][q] = *(const Frag*)((const T*)a.G + ((int64_t)cur * a.N + n) * a.rp + b + q * 8 +
-                                         (sizeof(T) == 2 ? 0 : half * 4));
-            }
-          }
+        for (int q = 0; q < kBatch; ++q) {
 #pragma unroll
-          for (int q = 0; q < kBatch; ++q)
+          for (int t = 0; t < TT; ++t) x[t][q] = x_of(t, b + q * 8);
 #pragma unroll
-            for (int j = 0; j < TN; ++j) d[j] = mma32(w[j][q], x[q], d[j]);
+          for (int j = 0; j < TN; ++j) w[j][q] = w_of(first, j, b + q * 8);
         }
-        float f = scale_of(a.rows, cur);
-        if constexpr (std::is_same_v<T, _Float16>) f *= has ? a.by[place] : 0.f;
-        if (mine == cur)
 #pragma unroll
-          for (int j = 0; j < TN; ++j) acc[j][t] = f * d[j];
+        for (int q = 0; q < kBatch; ++q)
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[j][t] = mma32(w[j][q], x[t][q], acc[j][t]);
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const float f = factor(t, first);
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[j][t][r] = has(t) ? f * acc[j][t][r] : 0.f;
+      }
+    } else if (any) {
+      // for each adapter among 32 rows the product of all of them, kept where it is theirs
+      int unit = shares - share;
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        uint64_t left = some[t];
+        while (left) {
+          const int cur = __builtin_amdgcn_readlane(mine[t], __builtin_ctzll(left));
+          left &= ~__ballot(mine[t] == cur);
+          f16 d[TN] = {};
+          for (int b = 0; b < a.r; b += 8 * kBatch) {
+            if (SPLIT && unit++ % shares != 0) continue;
+            Frag x[kBatch], w[TN][kBatch];
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q) {
+              x[q] = x_of(t, b + q * 8);
+#pragma unroll
+              for (int j = 0; j < TN; ++j) w[j][q] = w_of(cur, j, b + q * 8);
+            }
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q)
+#pragma unroll
+              for (int j = 0; j < TN; ++j) d[j] = mma32(w[j][q], x[q], d[j]);
+          }
+          const float f = factor(t, cur);
+          if (mine[t] == cur)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[j][t] = f * d[j];
+        }
       }
     }
   }
@@ -972,54 +1125,74 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   for (; kt + 3 < whole; kt += 2) {
     step(std::false_type{}, kt, us0, ws0, us1, ws1);
     step(std::false_type{}, kt + 1, us1, ws1, us0, ws0);
+    if constexpr (sizeof(T) == 4)
+      // fp32: sums of 512 values, then of those, or the rounding of one long sum would grow with its length
+      if ((kt - k0) % 16 == 14)
+#pragma unroll
+        for (int m = 0; m < kMma; ++m) {
+          total[m / TT][m % TT] += acc[m / TT][m % TT];
+          acc[m / TT][m % TT] = f16{};
+        }
   }
   for (; kt < k1; kt += 2) {
     step(std::true_type{}, kt, us0, ws0, us1, ws1);
     if (kt + 1 < k1) step(std::true_type{}, kt + 1, us1, ws1, us0, ws0);
   }
-  __builtin_amdgcn_s_waitcnt(0x0070);  // no load may land in LDS that is not this workgroup's any more
-
+  if constexpr (sizeof(T) == 4)
+#pragma unroll
+    for (int m = 0; m < kMma; ++m) acc[m / TT][m % TT] += total[m / TT][m % TT];
+  // No load may land in LDS from here on.  Each wave turns its part of the tile there, in chunks of 16 bytes moved by the
+  // row's number, and writes whole rows of it: straight from the accumulators a store would reach 16 bytes
+  // of each of 32 rows.
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  __syncthreads();
+  using Out = std::conditional_t<SPLIT, float, T>;
+  constexpr int EO = 16 / sizeof(Out), kRowOut = BN / WN / EO, kRows = BT / WT;  // chunks of a row, rows
+  static_assert(WT * WN * kRows * kRowOut * 16 <= (int)sizeof(lds), "turned tile");
+  Out* mem = (Out*)lds + wave * kRows * kRowOut * EO;
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
-    const int at = t0 + wt + t * 32 + l32;
+    const int i = t * 32 + l32;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      f16 v = acc[j][t];
+      if (!SPLIT && (wrong >> t & 1)) v = v * __builtin_nanf("");
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int n = j * 32 + r * 2 + half * 4;
+        *(Four<Out>*)(mem + (i * kRowOut + ((n / EO) ^ (i % kRowOut))) * EO + n % EO) =
+            Four<Out>{(Out)v[r], (Out)v[r + 1], (Out)v[r + 2], (Out)v[r + 3]};
+      }
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  constexpr int kAtOnce = 64 / kRowOut;  // rows of a store
+#pragma unroll
+  for (int q = 0; q < kRows / kAtOnce; ++q) {
+    const int i = q * kAtOnce + lane / kRowOut, c = lane % kRowOut;
+    typedef Out Chunk __attribute__((ext_vector_type(EO)));
+    const Chunk v = *(const Chunk*)(mem + (i * kRowOut + (c ^ (i % kRowOut))) * EO);
+    const int at = t0 + wt + i, n = n0 + wn + c * EO;
+    if (at >= a.rows.T) continue;
     if constexpr (SPLIT) {
-      if (at < a.rows.T) {
-        float* out = a.part + ((int64_t)blockIdx.y * a.rows.T + at) * a.ldp + n0 + wn + half * 4;
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; r += 4)
-            *(f4*)(out + j * 32 + r * 2) = f4{acc[j][t][r], acc[j][t][r + 1], acc[j][t][r + 2], acc[j][t][r + 3]};
-      }
+      *(Chunk*)(a.part + ((int64_t)blockIdx.y * a.rows.T + at) * a.ldp + n) = v;
     } else {
-      const bool in = at < a.rows.T;
-      const int64_t row = row_at(a.order, min(at, a.rows.T - 1));
-      const int mine = in ? adapter_of(a.rows, row) : -1;
-      const bool has = mine >= 0 && mine < a.rows.n;
-      if (!in) continue;
-      T* out = (T*)a.Y + row * a.ldy;
+      struct __attribute__((packed, aligned(sizeof(Out)))) Any {
+        Chunk v;
+      };
+      Out* out = (Out*)a.Y + row_at(a.order, at) * a.ldy + n;
+      if (n + EO <= a.N) ((Any*)out)->v = v;
+      else
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        f16 v = acc[j][t];
-        if (!has && mine != -1) v = v * __builtin_nanf("");
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const int n = n0 + wn + j * 32 + r * 2 + half * 4;
-          if (n + 4 <= a.N) {
-            *(Four<T>*)(out + n) = Four<T>{(T)v[r], (T)v[r + 1], (T)v[r + 2], (T)v[r + 3]};
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n + e < a.N) out[n + e] = (T)v[r + e];
-          }
-        }
-      }
+        for (int e = 0; e < EO; ++e)
+          if (n + e < a.N) out[e] = v[e];
     }
   }
 }
 
-// The factors' gradients: sum over the places of an adapter of U_t^T V_t, V = S or D, in pieces of kGradRows
-// places.  A workgroup takes 64 kE columns of U, a wave 16 kE, whose rows it turns in registers.  V is turned on its
+// The factors' gradients: sum over the places of an adapter of U_t^T V_t, V = S or D, in pieces of `size` places
+// (32 to kGradRows: with few rows smaller ones, for enough workgroups, but not so small that the parts, a rank's 4
+// bytes a column each, outweigh U's).  A workgroup takes 64 kE columns of U, a wave 16 kE, whose rows it turns in registers.  V is turned on its
 // way to LDS, as upper and lower part of the type (fp16: brought to below 2^14 by the
 // piece's power of two).  Bound by reading U once: each wave keeps two steps' rows in flight.
 constexpr int kGradRows = 128;
@@ -1034,7 +1207,7 @@ struct OuterPair {
   Outer p[2];
   Rows rows;
   Order order;
-  int rp, pieces;
+  int rp, pieces, size;
 };
 
 template <class T, int RB>
@@ -1048,7 +1221,7 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   const Outer& a = both.p[blockIdx.y];
   const int piece = blockIdx.x % both.pieces, block = blockIdx.x / both.pieces;
   if (block >= a.blocks) return;
-  const Piece pc = piece_of(both.order, both.rows, piece, kGradRows);
+  const Piece pc = piece_of(both.order, both.rows, piece, both.size);
   if (pc.count == 0) return;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
   const int j0 = blockIdx.z * kRanks;
@@ -1150,7 +1323,7 @@ struct SumPair {
   Sum p[2];
   Rows rows;
   Order order;
-  int r, rp;
+  int r, rp, size;
 };
 
 template <class T>
@@ -1162,7 +1335,7 @@ __global__ __launch_bounds__(256) void sum_kernel(SumPair both) {
   const int c = blockIdx.x / fours * 64 + lane, j0 = blockIdx.x % fours * 4;
   for (int i = blockIdx.z; i < both.rows.n; i += gridDim.z) {
     const int count = both.order.start ? both.order.start[i + 1] - both.order.start[i] : both.rows.T;
-    const int first = first_piece(both.order, i, kGradRows), many = (count + kGradRows - 1) / kGradRows;
+    const int first = first_piece(both.order, i, both.size), many = (count + both.size - 1) / both.size;
     f4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int p = wave; p < many; p += 4) {
@@ -1311,6 +1484,7 @@ struct Many {
       order = {prep.perm, prep.start};
     }
     groups = prep.order_groups;
+    prep.counter = ws.template take<int>(2 * pieces(a.T, a.n, a.index != nullptr, kLowRows));
   }
 
   T* copy(View src, int rows, int have, int cols, int ld, int count, bool steps = false) {
@@ -1344,12 +1518,19 @@ struct Many {
     l.U = U.p, l.ldu = U.ld, l.cu = U.cols;
     l.pieces = pieces(a.T, a.n, a.index != nullptr, kLowRows);
     l.low = ws.template take<float>(a.T * rp);
+    const int steps = (C + Mma<T>::kStep - 1) / Mma<T>::kStep;
+    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (2 * kLowWaves), 1, 16));
+    if (l.splits > 1) {
+      l.part = ws.template take<float>(l.splits * a.T * rp);
+      l.arrived = prep.counter + prep.counters;
+      prep.counters += l.pieces;
+    }
     if (sizeof(T) == 2) l.split = ws.template take<T>(a.T * 2 * rp);
     if (std::is_same_v<T, _Float16>) l.by = ws.template take<float>(a.T);
     return l;
   }
   int run_prepare(hipStream_t s) {
-    if (groups) hipLaunchKernelGGL(prepare_kernel<T>, dim3(groups), dim3(1024), 0, s, prep);
+    if (groups) hipLaunchKernelGGL(prepare_kernel<T>, dim3(groups), dim3(kPrepare), 0, s, prep);
     return GELIM_OK;
   }
   void run_low(const Low* l, int count, hipStream_t s) {
@@ -1358,7 +1539,7 @@ struct Many {
     unsigned most = 0;
     for (int k = 0; k < count; ++k) {
       both.p[k] = l[k];
-      most = std::max(most, (unsigned)l[k].pieces);
+      most = std::max(most, (unsigned)(l[k].pieces * l[k].splits));
     }
     const dim3 grid(most, (unsigned)count);
     switch (rb) {
@@ -1402,9 +1583,8 @@ struct Many {
     if (b.splits > 1) {
       b.ldp = b.tiles_n * q.tile;
       b.part = ws.template take<float>((int64_t)b.splits * a.T * b.ldp);
-    } else {
-      b.G = copy(turned(p.G), p.N, p.N, (int)a.r, rp, (int)a.n);
     }
+    b.G = copy(turned(p.G), p.N, p.N, (int)a.r, rp, (int)a.n);
     return q;
   }
   template <bool KC, int BT, int BN, int WT, int WN>
@@ -1430,7 +1610,7 @@ struct Many {
     if (q.kc) shape(std::true_type{});
     else shape(std::false_type{});
     if (b.splits > 1) {
-      Finish e{b.part, l.low, q.p.G, g, order.perm, b.N, (int)a.r, b.ldp, b.splits, 1, rp,
+      Finish e{b.part, nullptr, View{}, g, order.perm, b.N, 0, b.ldp, b.splits, 0, 0,
                (b.N + 255) / 256, b.Y, b.ldy};
       finish<T>(e, s);
     }
@@ -1467,11 +1647,13 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   low[1] = m.low_of(X, view_a(a), K);
   if ((a.dX && a.T) || all) q = m.big_of(back, dY);
   // the sides: dA = X^T D, dB^T = dY^T S
-  const int pcs = pieces(a.T, a.n, a.index != nullptr, kGradRows);
+  int size = kGradRows;
+  while (size > std::max(32, 2 * m.rp) && a.T / size * ((K + N) / (64 * Mma<T>::kE)) < 256) size /= 2;
+  const int pcs = pieces(a.T, a.n, a.index != nullptr, size);
   OuterPair op{};
   SumPair sp{};
   op.rows = sp.rows = m.g, op.order = sp.order = m.order;
-  op.rp = sp.rp = m.rp, sp.r = (int)a.r, op.pieces = pcs;
+  op.rp = sp.rp = m.rp, sp.r = (int)a.r, op.pieces = pcs, op.size = sp.size = size;
   int sides = 0;
   unsigned outer_groups = 0, sum_groups = 0;
   for (int k = 0; k < 2; ++k) {
