@@ -743,7 +743,6 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
         for (int t = 0; t < 2; ++t) acc[j][t] += lds[wave][j * 2 + t][lane];
     __syncthreads();
   }
-  if (wave) return;
   if (a.splits > 1) {
     // The parts go past the caches (agent-scope relaxed atomics), so that no cache has to be written back or
     // dropped as by a fence; the count goes up when they have arrived (vmcnt 0).
@@ -751,31 +750,46 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
       const int64_t at = pc.begin + min(t * 16 + l16, pc.count - 1);
       return a.part + ((int64_t)p * both.rows.T + at) * rp + j * 16 + g * 4;
     };
+    __shared__ int last;
+    if (wave == 0) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < RB; ++j)
+          if (t * 16 + l16 < pc.count)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              __hip_atomic_store(part(split, t, j) + e, acc[j][t][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (lane == 0)
+        last = __hip_atomic_fetch_add(a.arrived + piece, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.splits - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int m = wave; m < RB * 2; m += kWaves) {
+      f4 v = {0.f, 0.f, 0.f, 0.f};
+      for (int p = 0; p < a.splits; p += 4) {
+        f4 w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[q][e] = __hip_atomic_load(part(min(p + q, a.splits - 1), m % 2, m / 2) + e, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (p + q < a.splits) v += w[q];
+      }
+      lds[0][m][lane] = v;
+    }
+    __syncthreads();
+    if (wave == 0)
 #pragma unroll
       for (int j = 0; j < RB; ++j)
-        if (t * 16 + l16 < pc.count)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            __hip_atomic_store(part(split, t, j) + e, acc[j][t][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    int before = 0;
-    if (lane == 0) before = __hip_atomic_fetch_add(a.arrived + piece, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (__builtin_amdgcn_readfirstlane(before) != a.splits - 1) return;
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int j = 0; j < RB; ++j) {
-        f4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int p = 0; p < a.splits; ++p)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] += __hip_atomic_load(part(p, t, j) + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        acc[j][t] = v;
-      }
+        for (int t = 0; t < 2; ++t) acc[j][t] = lds[0][j * 2 + t][lane];
   }
+  if (wave) return;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const bool in = t * 16 + l16 < pc.count;
@@ -852,19 +866,18 @@ __device__ __forceinline__ int swap_columns(int k) {  // in chunks
   else return (k >> 2 & 1) * 8 % kRowChunks;
 }
 
-// WT x WN waves share a tile in blocks of 32 x 32.  Two tiles in
+// WT x WN waves share a tile in blocks of 32 x 32.  S tiles in
 // LDS and two sets of fragments in registers: while one quarter of a tile is
 // multiplied the next is read; when the last quarter is in registers the
-// tile's place is loaded again, a whole tile's time before the barrier that waits for it.
-template <class T, bool W_KC, int BT, int BN, int WT, int WN, bool SPLIT>
+// tile's place is loaded again, S - 1 tiles' time before the barrier that waits for it.
+template <class T, bool W_KC, int BT, int BN, int WT, int WN, int S, bool SPLIT>
 __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   using Frag = typename Mma<T>::Frag;
   constexpr int E = Mma<T>::kE, BK = 8 * E;
   constexpr int TT = BT / WT / 32, TN = BN / WN / 32;
   constexpr int kLoadU = BT / (WT * WN * 8), kLoadW = BN / (WT * WN * 8);
   constexpr int kRowChunks = BN / E;  // chunks in a row of W's tile if not W_KC
-  __shared__ __attribute__((aligned(16))) T lds[2 * (BT + BN) * BK];
-  constexpr int us0 = 0, us1 = BT * BK, ws0 = 2 * BT * BK, ws1 = ws0 + BN * BK;  // places in it
+  __shared__ __attribute__((aligned(16))) T lds[S * (BT + BN) * BK];  // U's tiles, then W's
 
   // Workgroups go to the 8 XCDs in turn: each XCD gets neighbouring tiles, and those that run at a time (a 256 x
   // 256 tile or two smaller ones on each of 32 CUs) are kGroup tiles high and about as wide, so that its L2 reads few
@@ -914,19 +927,19 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     return q;
   };
   // the q-th load of a tile; guard: with zeros behind the sum's end, also for tiles that nothing uses
-  auto load = [&](auto guard, int kt, int us, int ws, int q) {
+  auto load = [&](auto guard, int kt, int stage, int q) {
     const int k = kt * BK;
     const void* from;
     unsigned to;
     if (q < kLoadU) {
       from = up[q] + k;
       if (decltype(guard)::value && k + uk[q] >= a.cu) from = g_zeros;
-      to = lds_address(lds + us + (wave * kLoadU + q) * 64 * E);
+      to = lds_address(lds + stage * BT * BK + (wave * kLoadU + q) * 64 * E);
     } else {
       q -= kLoadU;
       from = wp[twin(q)] + (kt * w_step + (q - twin(q)) * kLoadRows * a.ldw);
       if (decltype(guard)::value && k + wk[q] >= a.cw) from = g_zeros;
-      to = lds_address(lds + ws + (wave * kLoadW + q) * 64 * E);
+      to = lds_address(lds + (S * BT + stage * BN) * BK + (wave * kLoadW + q) * 64 * E);
     }
     to_lds(from, __builtin_amdgcn_readfirstlane(to));
   };
@@ -950,7 +963,8 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     }
   }
   // the q-th fragment of a quarter
-  auto read = [&](int us, int ws, int part, Frags& f, int q) {
+  auto read = [&](int stage, int part, Frags& f, int q) {
+    const int us = stage * BT * BK, ws = (S * BT + stage * BN) * BK;
     if (q < TT) {
       f.x[q] = *(const Frag*)&lds[us + (u_at ^ (part * 2 * E)) + q * 32 * BK];
       return;
@@ -977,38 +991,40 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   // A quarter: `now` is multiplied; in between, in this order, quarter `part` is read into `next` in the first
   // half and, with kLoads, a tile is loaded.
   constexpr int kMma = TT * TN, kReads = TT + TN, kLoads = kLoadU + kLoadW;
-  auto quarter = [&](const Frags& now, int us, int ws, int part, Frags& next, auto loads, auto guard, int kt,
-                     int us_to, int ws_to) {
+  auto quarter = [&](const Frags& now, int stage, int part, Frags& next, auto loads, auto guard, int kt, int to) {
 #pragma unroll
     for (int m = 0; m < kMma; ++m) {
       constexpr int kSpan = (kMma + 1) / 2;
 #pragma unroll
       for (int q = 0; q < kReads; ++q)
-        if (q * kSpan / kReads == m) read(us, ws, part, next, q);
+        if (q * kSpan / kReads == m) read(stage, part, next, q);
       if constexpr (decltype(loads)::value)
 #pragma unroll
         for (int q = 0; q < kLoads; ++q)
-          if (q * kMma / kLoads == m) load(guard, kt, us_to, ws_to, q);
+          if (q * kMma / kLoads == m) load(guard, kt, to, q);
       acc[m / TT][m % TT] = mma32(now.w[m / TT], now.x[m % TT], acc[m / TT][m % TT]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   Frags f0, f1;
   // one tile from its place in LDS; its first quarter is in f0, and the next tile's will be
-  auto step = [&](auto guard, int kt, int us, int ws, int us_next, int ws_next) {
+  auto step = [&](auto guard, int kt, int stage) {
     constexpr std::false_type no{};
-    quarter(f0, us, ws, 1, f1, no, no, 0, us, ws);
-    quarter(f1, us, ws, 2, f0, no, no, 0, us, ws);
-    quarter(f0, us, ws, 3, f1, no, no, 0, us, ws);
-    // this wave's loads have landed (vmcnt 0) and its reads are done, then everybody's
-    __builtin_amdgcn_s_waitcnt(0x0070);
+    quarter(f0, stage, 1, f1, no, no, 0, 0);
+    quarter(f1, stage, 2, f0, no, no, 0, 0);
+    quarter(f0, stage, 3, f1, no, no, 0, 0);
+    // this wave's loads of the next tile have landed (only S - 2 tiles' may be under way) and its reads are done,
+    // then everybody's
+    constexpr int kAway = (S - 2) * kLoads;
+    static_assert(kAway < 64, "vmcnt");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (kAway & 15) | (kAway >> 4) << 14);
     __syncthreads();
-    quarter(f1, us_next, ws_next, 0, f0, std::true_type{}, guard, kt + 2, us, ws);
+    quarter(f1, (stage + 1) % S, 0, f0, std::true_type{}, guard, kt + S, stage);
   };
 #pragma unroll
-  for (int q = 0; q < kLoads; ++q) load(std::true_type{}, k0, us0, ws0, q);
+  for (int st = 0; st < S; ++st)
 #pragma unroll
-  for (int q = 0; q < kLoads; ++q) load(std::true_type{}, k0 + 1, us1, ws1, q);
+    for (int q = 0; q < kLoads; ++q) load(std::true_type{}, k0 + st, st, q);
   unsigned wrong = 0;  // rows of this lane whose adapter does not exist
   {
   // this lane's rows, and their adapters
@@ -1119,25 +1135,25 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   __builtin_amdgcn_s_waitcnt(0x0070);
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < kReads; ++q) read(us0, ws0, 0, f0, q);
+  for (int q = 0; q < kReads; ++q) read(0, 0, f0, q);
   const int whole = min(k1, min(a.cu, a.cw) / BK);  // tiles without a part behind the end
   int kt = k0;
-  for (; kt + 3 < whole; kt += 2) {
-    step(std::false_type{}, kt, us0, ws0, us1, ws1);
-    step(std::false_type{}, kt + 1, us1, ws1, us0, ws0);
+  for (; kt + 2 * S - 1 < whole; kt += S) {
+#pragma unroll
+    for (int st = 0; st < S; ++st) step(std::false_type{}, kt + st, st);
     if constexpr (sizeof(T) == 4)
-      // fp32: sums of 512 values, then of those, or the rounding of one long sum would grow with its length
-      if ((kt - k0) % 16 == 14)
+      // fp32: sums of about 512 values, then of those, or the rounding of one long sum would grow with its length
+      if ((kt - k0) / S % (16 / S) == 16 / S - 1)
 #pragma unroll
         for (int m = 0; m < kMma; ++m) {
           total[m / TT][m % TT] += acc[m / TT][m % TT];
           acc[m / TT][m % TT] = f16{};
         }
   }
-  for (; kt < k1; kt += 2) {
-    step(std::true_type{}, kt, us0, ws0, us1, ws1);
-    if (kt + 1 < k1) step(std::true_type{}, kt + 1, us1, ws1, us0, ws0);
-  }
+  for (; kt < k1; kt += S)
+#pragma unroll
+    for (int st = 0; st < S; ++st)
+      if (kt + st < k1) step(std::true_type{}, kt + st, st);
   if constexpr (sizeof(T) == 4)
 #pragma unroll
     for (int m = 0; m < kMma; ++m) acc[m / TT][m % TT] += total[m / TT][m % TT];
@@ -1555,9 +1571,36 @@ struct Many {
   struct Plan {
     Big b;
     bool kc;
-    int tile;
+    int bt, bn;
     Problem p;
   };
+  // The tile by what it is expected to take: the rounds of workgroups that fit the chip at a time, each of a fixed
+  // part (a launch's share, the first loads, the low-rank part, the end) and the tiles' steps of 128 bytes
+  // along the sum, both as measured (us).
+  void choose(Plan& q, int nk) {
+    struct Shape {
+      int bt, bn, at_once;  // at_once: workgroups
+      double fixed, step;
+    };
+    static constexpr Shape k16[] = {{256, 256, 256, 14, 1.6}, {256, 128, 256, 12, 0.9}, {128, 128, 256, 10, 0.55},
+                                    {64, 64, 512, 8, 0.4}};
+    static constexpr Shape k32[] = {{128, 128, 256, 12, 2.4}, {64, 64, 512, 10, 1.3}};
+    double best = 1e30;
+    auto look = [&](const Shape& h) {
+      const int64_t tiles = ((a.T + h.bt - 1) / h.bt) * ((q.p.N + h.bn - 1) / h.bn);
+      for (int splits = 1; splits <= 16 && (splits == 1 || (h.bn < 256 && nk / splits >= 4)); ++splits) {
+        const double rounds = (double)((tiles * splits + h.at_once - 1) / h.at_once);
+        // joining the parts: a launch, and writing and reading them
+        const double join = splits == 1 ? 0 : 5 + 8e-6 * (double)splits * a.T * q.p.N / 4;
+        const double us = rounds * (h.fixed + h.step * ((nk + splits - 1) / splits)) + join;
+        if (us < best) best = us, q.bt = h.bt, q.bn = h.bn, q.b.splits = splits;
+      }
+    };
+    if (sizeof(T) == 2)
+      for (const Shape& h : k16) look(h);
+    else
+      for (const Shape& h : k32) look(h);
+  }
   Plan big_of(const Problem& p, const Wide& U) {
     Plan q{};
     Big& b = q.b;
@@ -1572,40 +1615,38 @@ struct Many {
       const Wide w = wide(p.W.p, p.W.rs, p.C, p.N);
       b.W = w.p, b.ldw = w.ld, b.cw = p.C, b.nw = w.cols;
     }
-    auto tiles = [&](int tile) { return ((a.T + tile - 1) / tile) * ((p.N + tile - 1) / tile); };
-    if (sizeof(T) == 2 && tiles(256) >= 192) q.tile = 256;
-    else if (tiles(128) >= (sizeof(T) == 2 ? 256 : 512)) q.tile = 128;
-    else q.tile = sizeof(T) == 2 && a.T > 64 ? 128 : 64;
-    b.tiles_t = (int)((a.T + q.tile - 1) / q.tile);
-    b.tiles_n = (p.N + q.tile - 1) / q.tile;
-    const int nk = (std::max(b.cu, b.cw) + 8 * E - 1) / (8 * E), all = std::max(1, b.tiles_t * b.tiles_n);
-    b.splits = q.tile == 256 || all >= 160 ? 1 : std::clamp(512 / all, 1, std::clamp(nk / 4, 1, 16));
+    const int nk = (std::max(b.cu, b.cw) + 8 * E - 1) / (8 * E);
+    choose(q, nk);
+    b.tiles_t = (int)((a.T + q.bt - 1) / q.bt);
+    b.tiles_n = (p.N + q.bn - 1) / q.bn;
     if (b.splits > 1) {
-      b.ldp = b.tiles_n * q.tile;
+      b.ldp = b.tiles_n * q.bn;
       b.part = ws.template take<float>((int64_t)b.splits * a.T * b.ldp);
     }
     b.G = copy(turned(p.G), p.N, p.N, (int)a.r, rp, (int)a.n);
     return q;
   }
-  template <bool KC, int BT, int BN, int WT, int WN>
+  template <bool KC, int BT, int BN, int WT, int WN, int S>
   void launch(const Big& b, hipStream_t s) {
     const dim3 grid((unsigned)(b.tiles_t * b.tiles_n), (unsigned)b.splits);
-    if constexpr (BT < 256) {
+    if constexpr (BN < 256)
       if (b.splits > 1) {
-        hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, true>), grid, dim3(WT * WN * 64), 0, s, b);
+        hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, S, true>), grid, dim3(WT * WN * 64), 0, s, b);
         return;
       }
-    }
-    hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, false>), grid, dim3(WT * WN * 64), 0, s, b);
+    hipLaunchKernelGGL((big_kernel<T, KC, BT, BN, WT, WN, S, false>), grid, dim3(WT * WN * 64), 0, s, b);
   }
   void run_big(Plan& q, const Low& l, hipStream_t s) {
     Big& b = q.b;
     b.low = l.low, b.by = l.by, b.split = l.split;
     auto shape = [&](auto kc) {
       constexpr bool KC = decltype(kc)::value;
-      if (q.tile == 64) launch<KC, 64, 64, 2, 2>(b, s);
-      else if (q.tile == 128) launch<KC, 128, 128, 2, 2>(b, s);
-      else if constexpr (sizeof(T) == 2) launch<KC, 256, 256, 2, 4>(b, s);
+      if (q.bt == 64) launch<KC, 64, 64, 2, 2, 4>(b, s);
+      else if (q.bt == 128) launch<KC, 128, 128, 2, 2, 4>(b, s);
+      else if constexpr (sizeof(T) == 2) {
+        if (q.bn == 128) launch<KC, 256, 128, 4, 2, 3>(b, s);
+        else launch<KC, 256, 256, 2, 4, 2>(b, s);
+      }
     };
     if (q.kc) shape(std::true_type{});
     else shape(std::false_type{});
