@@ -470,21 +470,14 @@ __device__ __forceinline__ int64_t row_at(const Order& o, int64_t at) { return o
 // Pieces of at most `size` places, each within one adapter.  Adapter i's
 // pieces have the numbers from start[i] / size + i on: distinct for different adapters, as
 // floor((s + c) / size) - floor(s / size) + 1 >= ceil(c / size), and without a
-// table.  Numbers in between stay empty (count 0).
+// sum over the adapters.  Numbers in between stay empty (count 0).
 struct Piece {
-  int adapter, begin, count;
+  int adapter, begin, count, unused;
 };
 __device__ __forceinline__ int first_piece(const Order& o, int i, int size) { return o.start ? o.start[i] / size + i : 0; }
-__device__ __forceinline__ Piece piece_of(const Order& o, const Rows& g, int number, int size) {
-  if (!o.start) return {0, number * size, max(0, min(size, g.T - number * size))};
-  int lo = 0, hi = g.n - 1;  // the last adapter whose pieces begin at or before the number
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (first_piece(o, mid, size) <= number) lo = mid;
-    else hi = mid - 1;
-  }
-  const int begin = o.start[lo] + (number - first_piece(o, lo, size)) * size;
-  return {lo, begin, max(0, min(size, o.start[lo + 1] - begin))};
+__device__ __forceinline__ Piece piece_of(const Piece* table, const Rows& g, int number, int size) {
+  if (!table) return {0, number * size, max(0, min(size, g.T - number * size)), 0};
+  return table[number];
 }
 int pieces(int64_t T, int64_t n, bool ordered, int size) { return (int)(T / size + (ordered ? n : 1)); }
 
@@ -504,6 +497,10 @@ struct Prepare {
   Rows rows;
   int32_t *perm, *start;
   int order_groups;  // n + 1, or 0: the order is not needed
+  struct Pieces {
+    Piece* table;
+    int size;
+  } pieces[2];
   Copy copy[kCopies];
   int copies;
   int* counter;  // set to zero for the launches behind this one
@@ -512,17 +509,23 @@ struct Prepare {
 
 // Adapter i's rows (i = n: those without one), in order, by one workgroup:
 // it counts the rows of lower adapters, then writes its own behind those.  A thread takes kOrder rows side by side.
-constexpr int kOrder = 16, kPrepare = 256;
+constexpr int kOrder = 32, kPrepare = 256;
 __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
   __shared__ int sums[2][kPrepare / 64];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n = p.rows.n;
   int id[kOrder];
   auto fetch = [&](int64_t t0) {  // adapters of this thread's rows; behind the last row -1
 #pragma unroll
-    for (int q = 0; q < kOrder; ++q) {
+    for (int q = 0; q < kOrder; q += 4) {
       const int64_t t = t0 + threadIdx.x * kOrder + q;
-      const int a = t < p.rows.T ? p.rows.index[t] : 0;
-      id[q] = t >= p.rows.T ? -1 : a < 0 || a >= n ? n : a;
+      Four<int> a = {{0, 0, 0, 0}};
+      if (t + 4 <= p.rows.T) a = *(const Four<int>*)(p.rows.index + t);
+      else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (t + e < p.rows.T) a.v[e] = p.rows.index[t + e];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) id[q + e] = t + e >= p.rows.T ? -1 : a.v[e] < 0 || a.v[e] >= n ? n : a.v[e];
     }
   };
   int c = 0;
@@ -537,6 +540,7 @@ __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
   __syncthreads();
   int at = 0;
   for (int w = 0; w < kPrepare / 64; ++w) at += sums[0][w];
+  const int begin = at;
   if (threadIdx.x == 0) p.start[i] = at;
   for (int64_t t0 = 0; t0 < p.rows.T; t0 += kPrepare * kOrder) {
     if (p.rows.T > kPrepare * kOrder) fetch(t0);  // otherwise they are still here
@@ -560,6 +564,17 @@ __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
 #pragma unroll
     for (int q = 0; q < kOrder; ++q)
       if (id[q] == i) p.perm[place++] = (int32_t)(t0 + threadIdx.x * kOrder + q);
+  }
+  // this adapter's pieces, and empty ones up to the next adapter's; behind the last adapter empty ones to the table's end
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int size = p.pieces[k].size;
+    if (!p.pieces[k].table) continue;
+    const int first = begin / size + i, end = i < n ? at / size + i + 1 : p.rows.T / size + n;
+    for (int q = first + threadIdx.x; q < end; q += kPrepare) {
+      const int from = begin + (q - first) * size;
+      p.pieces[k].table[q] = {i, from, i < n ? max(0, min(size, at - from)) : 0, 0};
+    }
   }
 }
 
@@ -667,6 +682,7 @@ struct LowPair {
   Low p[2];
   Rows rows;
   Order order;
+  const Piece* table;
 };
 constexpr int kLowRows = 32;
 constexpr int kLowWaves = 8;
@@ -691,7 +707,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
   const Low& a = both.p[blockIdx.y];
   const int piece = blockIdx.x % a.pieces, split = blockIdx.x / a.pieces;
   if (split >= a.splits) return;
-  const Piece pc = piece_of(both.order, both.rows, piece, kLowRows);
+  const Piece pc = piece_of(both.table, both.rows, piece, kLowRows);
   if (pc.count == 0) return;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
   const T* u[2];
@@ -1223,6 +1239,7 @@ struct OuterPair {
   Outer p[2];
   Rows rows;
   Order order;
+  const Piece* table;
   int rp, pieces, size;
 };
 
@@ -1237,7 +1254,7 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   const Outer& a = both.p[blockIdx.y];
   const int piece = blockIdx.x % both.pieces, block = blockIdx.x / both.pieces;
   if (block >= a.blocks) return;
-  const Piece pc = piece_of(both.order, both.rows, piece, both.size);
+  const Piece pc = piece_of(both.table, both.rows, piece, both.size);
   if (pc.count == 0) return;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
   const int j0 = blockIdx.z * kRanks;
@@ -1327,8 +1344,8 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   }
 }
 
-// Last their sums, times s_i, in the factor's layout: 64 columns x 4 ranks of one adapter by a workgroup, whose four
-// waves share the pieces.
+// Last their sums, times s_i, in the factor's layout: 64 columns of one adapter by a workgroup, whose four waves share
+// the pieces of 4 ranks or, where the adapters have few pieces, take 4 ranks each.
 struct Sum {
   const float* part;
   void* out;
@@ -1342,29 +1359,34 @@ struct SumPair {
   int r, rp, size;
 };
 
-template <class T>
+template <class T, bool SHARE>
 __global__ __launch_bounds__(256) void sum_kernel(SumPair both) {
   __shared__ f4 lds[3][64];
   const Sum& a = both.p[blockIdx.y];
   if ((int)blockIdx.x >= a.blocks) return;
-  const int fours = (both.r + 3) / 4, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int c = blockIdx.x / fours * 64 + lane, j0 = blockIdx.x % fours * 4;
+  constexpr int kRanks = SHARE ? 4 : 16;
+  const int groups = (both.r + kRanks - 1) / kRanks, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int c = blockIdx.x / groups * 64 + lane, j0 = blockIdx.x % groups * kRanks + (SHARE ? 0 : wave * 4);
   for (int i = blockIdx.z; i < both.rows.n; i += gridDim.z) {
     const int count = both.order.start ? both.order.start[i + 1] - both.order.start[i] : both.rows.T;
     const int first = first_piece(both.order, i, both.size), many = (count + both.size - 1) / both.size;
     f4 s = {0.f, 0.f, 0.f, 0.f};
+    if (j0 < both.rp)
 #pragma unroll 4
-    for (int p = wave; p < many; p += 4) {
-      const float* from = a.part + ((int64_t)(first + p) * both.rp + j0) * a.ldp + c;
-      f4 v;
+      for (int p = SHARE ? wave : 0; p < many; p += SHARE ? 4 : 1) {
+        const float* from = a.part + ((int64_t)(first + p) * both.rp + j0) * a.ldp + c;
+        f4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = from[e * (int64_t)a.ldp];
-      s += v;
+        for (int e = 0; e < 4; ++e) v[e] = from[e * (int64_t)a.ldp];
+        s += v;
+      }
+    if constexpr (SHARE) {
+      if (wave) lds[wave - 1][lane] = s;
+      __syncthreads();
+      s += lds[0][lane] + lds[1][lane] + lds[2][lane];
     }
-    if (wave) lds[wave - 1][lane] = s;
-    __syncthreads();
-    if (wave == 0 && c < a.cols) {
-      s = (s + lds[0][lane] + lds[1][lane] + lds[2][lane]) * scale_of(both.rows, i);
+    if ((!SHARE || wave == 0) && c < a.cols) {
+      s = s * scale_of(both.rows, i);
       T* out = (T*)a.out + i * a.as + c * a.cs + j0 * a.rs;
       if (a.rs == 1 && j0 + 4 <= both.r) {
         *(Four<T>*)out = Four<T>{(T)s[0], (T)s[1], (T)s[2], (T)s[3]};
@@ -1374,7 +1396,7 @@ __global__ __launch_bounds__(256) void sum_kernel(SumPair both) {
           if (j0 + e < both.r) out[e * a.rs] = (T)s[e];
       }
     }
-    __syncthreads();
+    if constexpr (SHARE) __syncthreads();
   }
 }
 
@@ -1498,11 +1520,16 @@ struct Many {
       prep.start = ws.template take<int32_t>(a.n + 1);
       prep.order_groups = (int)a.n + 1;
       order = {prep.perm, prep.start};
+      set_pieces(0, kLowRows);
     }
     groups = prep.order_groups;
     prep.counter = ws.template take<int>(2 * pieces(a.T, a.n, a.index != nullptr, kLowRows));
   }
 
+  // a table of pieces of that size, if there is an order at all
+  void set_pieces(int k, int size) {
+    if (a.index) prep.pieces[k] = {ws.template take<Piece>(pieces(a.T, a.n, true, size)), size};
+  }
   T* copy(View src, int rows, int have, int cols, int ld, int count, bool steps = false) {
     Copy& c = prep.copy[prep.copies++];
     c = {src, ws.template take<T>((int64_t)count * rows * ld), rows, cols, ld, count, have, steps,
@@ -1535,7 +1562,9 @@ struct Many {
     l.pieces = pieces(a.T, a.n, a.index != nullptr, kLowRows);
     l.low = ws.template take<float>(a.T * rp);
     const int steps = (C + Mma<T>::kStep - 1) / Mma<T>::kStep;
-    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (2 * kLowWaves), 1, 16));
+    // cut the sum where that leaves a wave four rounds of loads or more
+    const int flight = rb <= 2 ? 4 : rb == 4 ? 2 : 1;
+    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (kLowWaves * flight * 4), 1, 16));
     if (l.splits > 1) {
       l.part = ws.template take<float>(l.splits * a.T * rp);
       l.arrived = prep.counter + prep.counters;
@@ -1551,7 +1580,7 @@ struct Many {
   }
   void run_low(const Low* l, int count, hipStream_t s) {
     LowPair both{};
-    both.rows = g, both.order = order;
+    both.rows = g, both.order = order, both.table = prep.pieces[0].table;
     unsigned most = 0;
     for (int k = 0; k < count; ++k) {
       both.p[k] = l[k];
@@ -1582,16 +1611,16 @@ struct Many {
       int bt, bn, at_once;  // at_once: workgroups
       double fixed, step;
     };
-    static constexpr Shape k16[] = {{256, 256, 256, 14, 1.6}, {256, 128, 256, 12, 0.9}, {128, 128, 256, 10, 0.55},
-                                    {64, 64, 512, 8, 0.4}};
-    static constexpr Shape k32[] = {{128, 128, 256, 12, 2.4}, {64, 64, 512, 10, 1.3}};
+    static constexpr Shape k16[] = {{256, 256, 256, 16.7, 1.61}, {256, 128, 256, 11.9, 0.90},
+                                    {128, 128, 256, 9.4, 0.50}, {64, 64, 512, 5.3, 0.39}};
+    static constexpr Shape k32[] = {{128, 128, 256, 12.3, 2.26}, {64, 64, 512, 6.4, 1.37}};
     double best = 1e30;
     auto look = [&](const Shape& h) {
       const int64_t tiles = ((a.T + h.bt - 1) / h.bt) * ((q.p.N + h.bn - 1) / h.bn);
       for (int splits = 1; splits <= 16 && (splits == 1 || (h.bn < 256 && nk / splits >= 4)); ++splits) {
         const double rounds = (double)((tiles * splits + h.at_once - 1) / h.at_once);
-        // joining the parts: a launch, and writing and reading them
-        const double join = splits == 1 ? 0 : 5 + 8e-6 * (double)splits * a.T * q.p.N / 4;
+        // joining the parts: a launch, and reading them
+        const double join = splits == 1 ? 0 : 3 + 0.6e-6 * (double)splits * a.T * q.p.N;
         const double us = rounds * (h.fixed + h.step * ((nk + splits - 1) / splits)) + join;
         if (us < best) best = us, q.bt = h.bt, q.bn = h.bn, q.b.splits = splits;
       }
@@ -1691,10 +1720,13 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   int size = kGradRows;
   while (size > std::max(32, 2 * m.rp) && a.T / size * ((K + N) / (64 * Mma<T>::kE)) < 256) size /= 2;
   const int pcs = pieces(a.T, a.n, a.index != nullptr, size);
+  m.set_pieces(1, size);
   OuterPair op{};
   SumPair sp{};
   op.rows = sp.rows = m.g, op.order = sp.order = m.order;
   op.rp = sp.rp = m.rp, sp.r = (int)a.r, op.pieces = pcs, op.size = sp.size = size;
+  op.table = m.prep.pieces[1].table;
+  const bool share = pcs >= 4 * a.n;
   int sides = 0;
   unsigned outer_groups = 0, sum_groups = 0;
   for (int k = 0; k < 2; ++k) {
@@ -1712,7 +1744,7 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
     u.as = (int64_t)a.r * cols;
     const bool along = k ? !a.b_trans : a.a_trans;  // columns side by side
     u.cs = along ? 1 : a.r, u.rs = along ? cols : 1;
-    u.blocks = (int)((cols + 63) / 64 * ((a.r + 3) / 4));
+    u.blocks = (int)((cols + 63) / 64 * ((a.r + (share ? 3 : 15)) / (share ? 4 : 16)));
     outer_groups = std::max(outer_groups, (unsigned)(pcs * o.blocks));
     sum_groups = std::max(sum_groups, (unsigned)u.blocks);
   }
@@ -1731,8 +1763,9 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
       else if (per == 2) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, dim3(256), 0, s, op);
       else hipLaunchKernelGGL((outer_kernel<T, 4>), grid, dim3(256), 0, s, op);
     }
-    hipLaunchKernelGGL(sum_kernel<T>, dim3(sum_groups, (unsigned)sides, (unsigned)std::min<int64_t>(a.n, 4096)),
-                       dim3(256), 0, s, sp);
+    const dim3 grid(sum_groups, (unsigned)sides, (unsigned)std::min<int64_t>(a.n, 4096));
+    if (share) hipLaunchKernelGGL((sum_kernel<T, true>), grid, dim3(256), 0, s, sp);
+    else hipLaunchKernelGGL((sum_kernel<T, false>), grid, dim3(256), 0, s, sp);
   }
   HIP_TRY(hipGetLastError());
   return GELIM_OK;
