@@ -481,15 +481,17 @@ __device__ __forceinline__ Piece piece_of(const Piece* table, const Rows& g, int
 }
 int pieces(int64_t T, int64_t n, bool ordered, int size) { return (int)(T / size + (ordered ? n : 1)); }
 
-// A matrix (one per adapter) copied as rows x ld values, zeros behind the source's rows and columns; `steps`: as the
-// matrix instruction's fragments, so that a wave's load of one is 1 KB without gaps: step along ld, block of 16
-// rows, lane, kE values.
+// A matrix (one per adapter) copied as rows x ld values, zeros behind the source's rows and columns; or in a matrix
+// instruction's fragments, so that a wave's load of one is 1 KB without gaps: kFrag16 by steps along ld, blocks of 16
+// rows, lanes, kE values; kFrag32 by blocks of 32 rows, 8 values along ld, lanes, kE values.
+enum { kRows, kFrag16, kFrag32 };
 struct Copy {
   View src;
   void* dst;
   int rows, cols, ld, count;  // of the copy (rows, ld) and how many matrices
   int have;                   // rows of the source; the others are zeros
-  bool steps, straight;
+  int order;  // kRows, or in fragments
+  bool straight;
   int first;                  // workgroups before this copy's
 };
 constexpr int kCopies = 6, kCopyTile = 64;
@@ -630,7 +632,7 @@ __device__ __forceinline__ void copy_tile(const Copy& c, int tile) {
   for (int q = 0; q < kChunks / kPrepare; ++q) {
     int o = q * kPrepare + threadIdx.x, i, j;
     T* to;
-    if (c.steps) {
+    if (c.order == kFrag16) {
       const int blocks = c.rows / 16, here = min(4, blocks - r0 / 16);  // of 16 rows, in all and in this tile
       const int step = o / (here * 64), rb = o / 64 % here, lane = o % 64;
       if (step >= kCopyTile / M::kStep) continue;
@@ -640,6 +642,8 @@ __device__ __forceinline__ void copy_tile(const Copy& c, int tile) {
       i = o / kAcross, j = o % kAcross * E;
       if (r0 + i >= c.rows || c0 + j >= c.ld) continue;
       to = dst + (int64_t)(r0 + i) * c.ld + c0 + j;
+      if (c.order == kFrag32)
+        to = dst + (((int64_t)(r0 + i) / 32 * (c.ld / 8) + (c0 + j) / 8) * (32 * 8 / E) + j % 8 / E * 32 + i % 32) * E;
     }
     Frag w;
 #pragma unroll
@@ -666,8 +670,8 @@ __global__ __launch_bounds__(kPrepare) void prepare_kernel(Prepare p) {
 // F is laid out in fragments, ldf values along the sum with zeros behind C.  Bound by
 // reading U and, for every 32 rows, F_i: each wave keeps several steps' loads in flight.  With few rows several
 // workgroups cut the sum once more; the last of them to end adds their parts, always in the same order.
-// 16-bit types: also as the sum of two values of the type, 8 ranks' upper and then lower parts side by side, for
-// the matrix units of the large product.  One value's rounding alone would be as large as the
+// Also in fragments of 32 places and 8 ranks for the matrix units of the large product, with 16-bit types as the sum
+// of two values of the type, the upper parts for the lower half of the lanes.  One value's rounding alone would be as large as the
 // result's.  fp16: a row is first brought to below 2^14 by a power of two (`by`), as it may be beyond the type's range.
 struct Low {
   const void *U, *F;
@@ -677,6 +681,7 @@ struct Low {
   int cu, ldf, pieces, splits;  // cu: values in a row of U, a multiple of 16 bytes
   float* part;                  // split, place, rank; with splits > 1
   int* arrived;                 // of each piece
+  bool many;
 };
 struct LowPair {
   Low p[2];
@@ -685,7 +690,7 @@ struct LowPair {
   const Piece* table;
 };
 constexpr int kLowRows = 32;
-constexpr int kLowWaves = 8;
+constexpr int low_waves(int rank_blocks, bool many) { return many && rank_blocks <= 8 ? 16 : 8; }  // MANY: with few pieces
 
 // v as upper and lower part of the type; the lower is 0 beside an infinity or NaN
 template <class T>
@@ -698,11 +703,11 @@ __device__ __forceinline__ int to_fp16_range(float most) {
   return most > 0.f ? min(max(13 - ilogbf(most), -100), 100) : 0;
 }
 
-template <class T, int RB>
-__global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
+template <class T, int RB, bool MANY>
+__global__ __launch_bounds__(low_waves(RB, MANY) * 64) void low_kernel(LowPair both) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int E = M::kE, rp = 16 * RB, kWaves = kLowWaves;
+  constexpr int E = M::kE, rp = 16 * RB, kWaves = low_waves(RB, MANY);
   __shared__ f4 lds[kWaves / 2][RB * 2][64];
   const Low& a = both.p[blockIdx.y];
   const int piece = blockIdx.x % a.pieces, split = blockIdx.x / a.pieces;
@@ -830,13 +835,16 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
 #pragma unroll
     for (int j = 0; j < RB; ++j) {
       *(f4*)(a.low + at * rp + j * 16 + g * 4) = acc[j][t];
+      // in fragments of 8 ranks (j * 2 + g / 2) and 32 places: two halves of 32 lanes
+      T* out = (T*)a.split + ((at / 32 * (rp / 8) + j * 2 + g / 2) * 64 + at % 32) * E;
       if constexpr (sizeof(T) == 2) {
         Four<T> hi, lo;
 #pragma unroll
         for (int i = 0; i < 4; ++i) two_parts(acc[j][t][i] * by, hi.v[i], lo.v[i]);
-        T* out = (T*)a.split + at * 2 * rp + (j * 2 + g / 2) * 16 + g % 2 * 4;
-        *(Four<T>*)out = hi;
-        *(Four<T>*)(out + 8) = lo;
+        *(Four<T>*)(out + g % 2 * 4) = hi;
+        *(Four<T>*)(out + 32 * E + g % 2 * 4) = lo;
+      } else {
+        *(f4*)(out + g % 2 * 32 * E) = acc[j][t];
       }
     }
   }
@@ -1055,29 +1063,25 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   }
     // The accumulators begin with s_i (U F_i) G_i, while the first tiles load (SPLIT: each part of the sum with some
     // of the adapters and ranks).  U F_i comes as two values of the type
-    // (fp32: itself), so 8 ranks are one step.  All loads of kBatch steps come before their products.
+    // (fp32: itself), so 8 ranks are one step; the loads of kSets steps are under way at a time.  A row without this adapter loads its own garbage, which reaches
+    // that row's accumulators alone, and these are set afterwards.
     auto has = [&](int t) { return mine[t] >= 0 && mine[t] < a.rows.n; };
     auto place = [&](int t) { return (int64_t)min(t0 + wt + t * 32 + l32, a.rows.T - 1); };
     auto x_of = [&](int t, int b) {
-      const Frag* at = sizeof(T) == 2 ? (const Frag*)((const T*)a.split + place(t) * 2 * a.rp) + half
-                                      : (const Frag*)(a.low + place(t) * a.rp) + half;
-      Frag x = {};
-      if (b < a.rp && has(t)) x = at[b / 8 * 2];
-      return x;
+      const int64_t block = min((t0 + wt) / 32 + t, (a.rows.T - 1) / 32);
+      return ((const Frag*)a.split)[(block * (a.rp / 8) + b / 8) * 64 + lane];
     };
+    constexpr int kG = 32 * 8 / E;  // fragments' chunks of 8 ranks and 32 columns: 16-bit types' halves share them
     auto w_of = [&](int cur, int j, int b) {
-      const int n = min(n0 + wn + j * 32 + l32, a.N - 1);
-      Frag w = {};
-      if (b < a.rp)
-        w = *(const Frag*)((const T*)a.G + ((int64_t)cur * a.N + n) * a.rp + b + (sizeof(T) == 2 ? 0 : half * 4));
-      return w;
+      const int64_t blocks = (a.N + 31) / 32, block = min((int64_t)(n0 + wn) / 32 + j, blocks - 1);
+      return ((const Frag*)a.G)[((cur * blocks + block) * (a.rp / 8) + b / 8) * kG + lane % kG];
     };
     auto factor = [&](int t, int cur) {
       float f = scale_of(a.rows, cur);
       if constexpr (std::is_same_v<T, _Float16>) f *= has(t) ? a.by[place(t)] : 0.f;
       return f;
     };
-    constexpr int kBatch = BT == 256 ? 1 : 2;  // by the registers
+    constexpr int kSets = TT * TN >= 8 ? 2 : TT * TN >= 4 ? 2 : 4;  // by the registers
     const int shares = SPLIT ? a.splits : 1, share = SPLIT ? blockIdx.y : 0;
     uint64_t some[TT], any = 0;
     int first = -1;
@@ -1092,22 +1096,26 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     for (int t = 0; t < TT; ++t) one = one && __ballot(has(t) && mine[t] != first) == 0;
     if (any && one) {
       // one adapter among all of the wave's rows: straight into the accumulators, zeros again where it is no row's
-      for (int b = share * 8 * kBatch; b < a.r; b += shares * 8 * kBatch) {
-        Frag x[TT][kBatch], w[TN][kBatch];
+      Frag x[kSets][TT], w[kSets][TN];
+      auto fetch = [&](int q, int b) {
+        if (b >= a.r) return;
 #pragma unroll
-        for (int q = 0; q < kBatch; ++q) {
+        for (int t = 0; t < TT; ++t) x[q][t] = x_of(t, b);
 #pragma unroll
-          for (int t = 0; t < TT; ++t) x[t][q] = x_of(t, b + q * 8);
+        for (int j = 0; j < TN; ++j) w[q][j] = w_of(first, j, b);
+      };
 #pragma unroll
-          for (int j = 0; j < TN; ++j) w[j][q] = w_of(first, j, b + q * 8);
+      for (int q = 0; q < kSets; ++q) fetch(q, (share + q * shares) * 8);
+      for (int b = share * 8; b < a.r; b += kSets * shares * 8)
+#pragma unroll
+        for (int q = 0; q < kSets; ++q) {
+          if (b + q * shares * 8 < a.r)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+              for (int t = 0; t < TT; ++t) acc[j][t] = mma32(w[q][j], x[q][t], acc[j][t]);
+          fetch(q, b + (kSets + q) * shares * 8);
         }
-#pragma unroll
-        for (int q = 0; q < kBatch; ++q)
-#pragma unroll
-          for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int t = 0; t < TT; ++t) acc[j][t] = mma32(w[j][q], x[t][q], acc[j][t]);
-      }
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
         const float f = factor(t, first);
@@ -1126,19 +1134,21 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
           const int cur = __builtin_amdgcn_readlane(mine[t], __builtin_ctzll(left));
           left &= ~__ballot(mine[t] == cur);
           f16 d[TN] = {};
-          for (int b = 0; b < a.r; b += 8 * kBatch) {
+          for (int b = 0; b < a.r; b += 8 * kSets) {
             if (SPLIT && unit++ % shares != 0) continue;
-            Frag x[kBatch], w[TN][kBatch];
+            Frag x[kSets], w[TN][kSets];
 #pragma unroll
-            for (int q = 0; q < kBatch; ++q) {
+            for (int q = 0; q < kSets; ++q) {
+              if (b + q * 8 >= a.r) continue;
               x[q] = x_of(t, b + q * 8);
 #pragma unroll
               for (int j = 0; j < TN; ++j) w[j][q] = w_of(cur, j, b + q * 8);
             }
 #pragma unroll
-            for (int q = 0; q < kBatch; ++q)
+            for (int q = 0; q < kSets; ++q)
+              if (b + q * 8 < a.r)
 #pragma unroll
-              for (int j = 0; j < TN; ++j) d[j] = mma32(w[j][q], x[q], d[j]);
+                for (int j = 0; j < TN; ++j) d[j] = mma32(w[j][q], x[q], d[j]);
           }
           const float f = factor(t, cur);
           if (mine[t] == cur)
@@ -1179,9 +1189,9 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   __builtin_amdgcn_s_waitcnt(0x0070);
   __syncthreads();
   using Out = std::conditional_t<SPLIT, float, T>;
-  constexpr int EO = 16 / sizeof(Out), kRowOut = BN / WN / EO, kRows = BT / WT;  // chunks of a row, rows
-  static_assert(WT * WN * kRows * kRowOut * 16 <= (int)sizeof(lds), "turned tile");
-  Out* mem = (Out*)lds + wave * kRows * kRowOut * EO;
+  constexpr int EO = 16 / sizeof(Out), kRowOut = BN / WN / EO, kHigh = BT / WT;  // chunks of a row, rows
+  static_assert(WT * WN * kHigh * kRowOut * 16 <= (int)sizeof(lds), "turned tile");
+  Out* mem = (Out*)lds + wave * kHigh * kRowOut * EO;
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
     const int i = t * 32 + l32;
@@ -1200,7 +1210,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   __builtin_amdgcn_wave_barrier();
   constexpr int kAtOnce = 64 / kRowOut;  // rows of a store
 #pragma unroll
-  for (int q = 0; q < kRows / kAtOnce; ++q) {
+  for (int q = 0; q < kHigh / kAtOnce; ++q) {
     const int i = q * kAtOnce + lane / kRowOut, c = lane % kRowOut;
     typedef Out Chunk __attribute__((ext_vector_type(EO)));
     const Chunk v = *(const Chunk*)(mem + (i * kRowOut + (c ^ (i % kRowOut))) * EO);
@@ -1530,10 +1540,10 @@ struct Many {
   void set_pieces(int k, int size) {
     if (a.index) prep.pieces[k] = {ws.template take<Piece>(pieces(a.T, a.n, true, size)), size};
   }
-  T* copy(View src, int rows, int have, int cols, int ld, int count, bool steps = false) {
+  T* copy(View src, int rows, int have, int cols, int ld, int count, int order = kRows) {
     Copy& c = prep.copy[prep.copies++];
-    c = {src, ws.template take<T>((int64_t)count * rows * ld), rows, cols, ld, count, have, steps,
-         !steps && src.cs == 1, (int)groups - prep.order_groups};
+    c = {src, ws.template take<T>((int64_t)count * rows * ld), rows, cols, ld, count, have, order,
+         order == kRows && src.cs == 1, (int)groups - prep.order_groups};
     groups += c.straight ? (unsigned)(((int64_t)count * rows * (ld / E) + kStraight - 1) / kStraight)
                          : (unsigned)(count * ((rows + kCopyTile - 1) / kCopyTile) * ((ld + kCopyTile - 1) / kCopyTile));
     return (T*)c.dst;
@@ -1557,20 +1567,21 @@ struct Many {
   Low low_of(const Wide& U, View F, int C) {
     Low l{};
     l.ldf = (int)up(C, 64);
-    l.F = copy(turned(F), rp, (int)a.r, C, l.ldf, (int)a.n, true);
+    l.F = copy(turned(F), rp, (int)a.r, C, l.ldf, (int)a.n, kFrag16);
     l.U = U.p, l.ldu = U.ld, l.cu = U.cols;
     l.pieces = pieces(a.T, a.n, a.index != nullptr, kLowRows);
     l.low = ws.template take<float>(a.T * rp);
     const int steps = (C + Mma<T>::kStep - 1) / Mma<T>::kStep;
     // cut the sum where that leaves a wave four rounds of loads or more
     const int flight = rb <= 2 ? 4 : rb == 4 ? 2 : 1;
-    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (kLowWaves * flight * 4), 1, 16));
+    l.many = l.pieces <= 144;
+    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (low_waves(rb, l.many) * flight * 4), 1, 16));
     if (l.splits > 1) {
       l.part = ws.template take<float>(l.splits * a.T * rp);
       l.arrived = prep.counter + prep.counters;
       prep.counters += l.pieces;
     }
-    if (sizeof(T) == 2) l.split = ws.template take<T>(a.T * 2 * rp);
+    l.split = ws.template take<T>(up(a.T, 32) * rp * (sizeof(T) == 2 ? 2 : 1));
     if (std::is_same_v<T, _Float16>) l.by = ws.template take<float>(a.T);
     return l;
   }
@@ -1587,13 +1598,16 @@ struct Many {
       most = std::max(most, (unsigned)(l[k].pieces * l[k].splits));
     }
     const dim3 grid(most, (unsigned)count);
-    switch (rb) {
-      case 1: hipLaunchKernelGGL((low_kernel<T, 1>), grid, dim3(kLowWaves * 64), 0, s, both); break;
-      case 2: hipLaunchKernelGGL((low_kernel<T, 2>), grid, dim3(kLowWaves * 64), 0, s, both); break;
-      case 4: hipLaunchKernelGGL((low_kernel<T, 4>), grid, dim3(kLowWaves * 64), 0, s, both); break;
-      case 8: hipLaunchKernelGGL((low_kernel<T, 8>), grid, dim3(kLowWaves * 64), 0, s, both); break;
-      default: hipLaunchKernelGGL((low_kernel<T, 16>), grid, dim3(kLowWaves * 64), 0, s, both);
-    }
+    auto launch = [&](auto blocks) {
+      constexpr int RB = decltype(blocks)::value;
+      if (l[0].many) hipLaunchKernelGGL((low_kernel<T, RB, true>), grid, dim3(low_waves(RB, true) * 64), 0, s, both);
+      else hipLaunchKernelGGL((low_kernel<T, RB, false>), grid, dim3(low_waves(RB, false) * 64), 0, s, both);
+    };
+    if (rb == 1) launch(std::integral_constant<int, 1>{});
+    else if (rb == 2) launch(std::integral_constant<int, 2>{});
+    else if (rb == 4) launch(std::integral_constant<int, 4>{});
+    else if (rb == 8) launch(std::integral_constant<int, 8>{});
+    else launch(std::integral_constant<int, 16>{});
   }
 
   // the large product
@@ -1652,7 +1666,7 @@ struct Many {
       b.ldp = b.tiles_n * q.bn;
       b.part = ws.template take<float>((int64_t)b.splits * a.T * b.ldp);
     }
-    b.G = copy(turned(p.G), p.N, p.N, (int)a.r, rp, (int)a.n);
+    b.G = copy(turned(p.G), (int)up(p.N, 32), p.N, (int)a.r, rp, (int)a.n, kFrag32);
     return q;
   }
   template <bool KC, int BT, int BN, int WT, int WN, int S>
