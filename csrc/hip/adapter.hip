@@ -1572,10 +1572,10 @@ struct Many {
     l.pieces = pieces(a.T, a.n, a.index != nullptr, kLowRows);
     l.low = ws.template take<float>(a.T * rp);
     const int steps = (C + Mma<T>::kStep - 1) / Mma<T>::kStep;
-    // cut the sum where that leaves a wave four rounds of loads or more
+    // cut the sum where that leaves a wave a round of loads or more
     const int flight = rb <= 2 ? 4 : rb == 4 ? 2 : 1;
     l.many = l.pieces <= 144;
-    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (low_waves(rb, l.many) * flight * 4), 1, 16));
+    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (low_waves(rb, l.many) * flight), 1, 16));
     if (l.splits > 1) {
       l.part = ws.template take<float>(l.splits * a.T * rp);
       l.arrived = prep.counter + prep.counters;
@@ -1771,7 +1771,8 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   }
   if (sides) {
     if (a.T) {
-      const int per = std::min(m.rb, 4);
+      int per = std::min(m.rb, 4);  // blocks of 16 ranks a workgroup, fewer where that fills the chip
+      while (per > 1 && (int64_t)outer_groups * sides * (m.rb / per) < 384) per /= 2;
       const dim3 grid(outer_groups, (unsigned)sides, (unsigned)(m.rb / per));
       if (per == 1) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, dim3(256), 0, s, op);
       else if (per == 2) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, dim3(256), 0, s, op);
