@@ -472,11 +472,11 @@ __device__ __forceinline__ int64_t row_at(const Order& o, int64_t at) { return o
 // floor((s + c) / size) - floor(s / size) + 1 >= ceil(c / size), and without a
 // sum over the adapters.  Numbers in between stay empty (count 0).
 struct Piece {
-  int adapter, begin, count, unused;
+  int adapter, begin, count, first;  // first: its adapter's first, also with count 0
 };
 __device__ __forceinline__ int first_piece(const Order& o, int i, int size) { return o.start ? o.start[i] / size + i : 0; }
 __device__ __forceinline__ Piece piece_of(const Piece* table, const Rows& g, int number, int size) {
-  if (!table) return {0, number * size, max(0, min(size, g.T - number * size)), 0};
+  if (!table) return {0, number * size, max(0, min(size, g.T - number * size)), number == 0};
   return table[number];
 }
 int pieces(int64_t T, int64_t n, bool ordered, int size) { return (int)(T / size + (ordered ? n : 1)); }
@@ -575,7 +575,7 @@ __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
     const int first = begin / size + i, end = i < n ? at / size + i + 1 : p.rows.T / size + n;
     for (int q = first + threadIdx.x; q < end; q += kPrepare) {
       const int from = begin + (q - first) * size;
-      p.pieces[k].table[q] = {i, from, i < n ? max(0, min(size, at - from)) : 0, 0};
+      p.pieces[k].table[q] = {i, from, i < n ? max(0, min(size, at - from)) : 0, i < n && q == first};
     }
   }
 }
@@ -1244,16 +1244,20 @@ struct Outer {
   const float* low;  // V
   float* part;       // piece, rank, column
   int cu, ldp, blocks;
+  // with at most one piece an adapter: the gradient itself, at adapter as + column cs + rank rs
+  void* out;
+  int64_t as, cs, rs;
+  int cols;
 };
 struct OuterPair {
   Outer p[2];
   Rows rows;
   Order order;
   const Piece* table;
-  int rp, pieces, size;
+  int rp, pieces, size, r;
 };
 
-template <class T, int RB>
+template <class T, int RB, bool DIRECT>
 __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
@@ -1265,10 +1269,11 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   const int piece = blockIdx.x % both.pieces, block = blockIdx.x / both.pieces;
   if (block >= a.blocks) return;
   const Piece pc = piece_of(both.table, both.rows, piece, both.size);
-  if (pc.count == 0) return;
+  if (DIRECT ? !pc.first : pc.count == 0) return;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
   const int j0 = blockIdx.z * kRanks;
-  if (threadIdx.x < kGradRows) row[threadIdx.x] = (int32_t)row_at(both.order, pc.begin + min((int)threadIdx.x, pc.count - 1));
+  if (threadIdx.x < kGradRows)
+    row[threadIdx.x] = pc.count ? (int32_t)row_at(both.order, pc.begin + min((int)threadIdx.x, pc.count - 1)) : 0;
   __syncthreads();
   const int n0 = (block * 4 + wave) * 16 * E, n = n0 + l16 * E;
   const T* U = (const T*)a.U + n;
@@ -1341,6 +1346,28 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
     s += kFlight;
     if (s * M::kStep >= pc.count) break;
     fetch(s);
+  }
+  if constexpr (DIRECT) {
+    const float f = scale_of(both.rows, pc.adapter) * back;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      const int j = j0 + b * 16 + l16;
+      if (j >= both.r) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = n0 + (g * 4 + i) * E;
+        T* out = (T*)a.out + pc.adapter * a.as + c * a.cs + j * a.rs;
+        Unaligned<T> v;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v.v[e] = (T)(f * acc[e][b][i]);
+        if (a.cs == 1 && c + E <= a.cols) *(Unaligned<T>*)out = v;
+        else
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (c + e < a.cols) out[e * a.cs] = v.v[e];
+      }
+    }
+    return;
   }
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -1732,13 +1759,14 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   if ((a.dX && a.T) || all) q = m.big_of(back, dY);
   // the sides: dA = X^T D, dB^T = dY^T S
   int size = kGradRows;
-  while (size > std::max(32, 2 * m.rp) && a.T / size * ((K + N) / (64 * Mma<T>::kE)) < 256) size /= 2;
+  const bool direct = a.T > 0 && a.T <= size;  // no adapter has more than one piece: no parts to add up
+  while (!direct && size > std::max(32, 2 * m.rp) && a.T / size * ((K + N) / (64 * Mma<T>::kE)) < 256) size /= 2;
   const int pcs = pieces(a.T, a.n, a.index != nullptr, size);
   m.set_pieces(1, size);
   OuterPair op{};
   SumPair sp{};
   op.rows = sp.rows = m.g, op.order = sp.order = m.order;
-  op.rp = sp.rp = m.rp, sp.r = (int)a.r, op.pieces = pcs, op.size = sp.size = size;
+  op.rp = sp.rp = m.rp, sp.r = (int)a.r, op.pieces = pcs, op.size = sp.size = size, op.r = (int)a.r;
   op.table = m.prep.pieces[1].table;
   const bool share = pcs >= 4 * a.n;
   int sides = 0;
@@ -1759,6 +1787,7 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
     const bool along = k ? !a.b_trans : a.a_trans;  // columns side by side
     u.cs = along ? 1 : a.r, u.rs = along ? cols : 1;
     u.blocks = (int)((cols + 63) / 64 * ((a.r + (share ? 3 : 15)) / (share ? 4 : 16)));
+    o.out = u.out, o.as = u.as, o.cs = u.cs, o.rs = u.rs, o.cols = cols;
     outer_groups = std::max(outer_groups, (unsigned)(pcs * o.blocks));
     sum_groups = std::max(sum_groups, (unsigned)u.blocks);
   }
@@ -1774,9 +1803,18 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
       int per = std::min(m.rb, 4);  // blocks of 16 ranks a workgroup, fewer where that fills the chip
       while (per > 1 && (int64_t)outer_groups * sides * (m.rb / per) < 384) per /= 2;
       const dim3 grid(outer_groups, (unsigned)sides, (unsigned)(m.rb / per));
-      if (per == 1) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, dim3(256), 0, s, op);
-      else if (per == 2) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, dim3(256), 0, s, op);
-      else hipLaunchKernelGGL((outer_kernel<T, 4>), grid, dim3(256), 0, s, op);
+      auto launch = [&](auto direct) {
+        constexpr bool D = decltype(direct)::value;
+        if (per == 1) hipLaunchKernelGGL((outer_kernel<T, 1, D>), grid, dim3(256), 0, s, op);
+        else if (per == 2) hipLaunchKernelGGL((outer_kernel<T, 2, D>), grid, dim3(256), 0, s, op);
+        else hipLaunchKernelGGL((outer_kernel<T, 4, D>), grid, dim3(256), 0, s, op);
+      };
+      if (direct) launch(std::true_type{});
+      else launch(std::false_type{});
+    }
+    if (direct) {
+      HIP_TRY(hipGetLastError());
+      return GELIM_OK;
     }
     const dim3 grid(sum_groups, (unsigned)sides, (unsigned)std::min<int64_t>(a.n, 4096));
     if (share) hipLaunchKernelGGL((sum_kernel<T, true>), grid, dim3(256), 0, s, sp);

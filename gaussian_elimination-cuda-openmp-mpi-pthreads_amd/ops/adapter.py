@@ -55,9 +55,10 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _check(X, W, A, B, index, scale):
-    if X.dtype not in TYPES:
-        raise TypeError(f"adapter_matmul takes float32, bfloat16 and float16, not {X.dtype}")
-    if not (W.dtype == A.dtype == B.dtype == X.dtype):
+    dtype = X.dtype
+    if dtype not in TYPES:
+        raise TypeError(f"adapter_matmul takes float32, bfloat16 and float16, not {dtype}")
+    if not (W.dtype == A.dtype == B.dtype == dtype):
         raise TypeError("X, W, A and B must have one type")
     dev = X.device
     if dev.type != "cuda" or not (W.device == A.device == B.device == dev):
@@ -67,7 +68,7 @@ def _check(X, W, A, B, index, scale):
     T, K = X.shape
     N = W.shape[1]
     n, _, r = A.shape
-    if W.shape[0] != K or A.shape[1] != K or B.shape != (n, r, N):
+    if W.shape[0] != K or A.shape[1] != K or tuple(B.shape) != (n, r, N):
         raise ValueError(f"shape mismatch: X {tuple(X.shape)}, W {tuple(W.shape)}, A {tuple(A.shape)}, "
                          f"B {tuple(B.shape)}")
     if min(K, N, n, r) < 1:
@@ -152,7 +153,7 @@ def adapter_matmul(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.T
     Runs on the current stream; may be captured into a graph."""
     dev, T, K, N, n, r = _check(X, W, A, B, index, scale)
     if out is None:
-        out = torch.empty((T, N), dtype=X.dtype, device=dev)
+        out = X.new_empty((T, N))
     else:
         if out.dtype != X.dtype or out.device != dev:
             raise ValueError("out must have the type and device of X")

@@ -39,13 +39,13 @@ def make(dev, T, K, N, r, n, dtype, layout="kn", rows="mixed", seed=0):
     return X, W, A, B, index.int().to(dev), scale
 
 
-def ref_product(X, W, A, B, index, scale):
-    """(result, tolerance) in 64 bits, on the CPU."""
+def ref_product(X, W, A, B, index, scale, device="cpu"):
+    """(result, tolerance) in 64 bits."""
     dtype = X.dtype
-    X, W, A, B, index = (v.detach().cpu() for v in (X, W, A, B, index))
+    X, W, A, B, index = (v.detach().to(device) for v in (X, W, A, B, index))
     X, W, A, B = (v.double() for v in (X, W, A, B))
     scale = torch.full((len(A),), float(scale), dtype=torch.float64) if not isinstance(scale, torch.Tensor) \
-        else scale.cpu().double()
+        else scale.to(device).double()
     Y, total = X @ W, X.abs() @ W.abs()
     low = torch.zeros_like(Y)
     for i in range(len(A)):
@@ -59,7 +59,7 @@ def ref_product(X, W, A, B, index, scale):
 
 
 def check(got, ref, tol, scale=1.0):
-    got = got.detach().cpu().double()
+    got = got.detach().to(ref.device).double()
     assert got.shape == ref.shape
     assert torch.isfinite(got).all()
     off = ((got - ref).abs() / tol).max().item() if got.numel() else 0.0
@@ -71,6 +71,36 @@ def check(got, ref, tol, scale=1.0):
 @pytest.mark.parametrize("shape", SHAPES)
 def test_product(gelim, cuda, shape, layout, dtype):
     args = make(cuda, *shape, dtype, layout)
+    check(gelim.ops.adapter_matmul(*args), *ref_product(*args))
+
+
+# sizes for which each tile shape is chosen, whole and with the sum cut, with tails in every dimension; a sum of fewer
+# tiles than are kept in LDS, and of a number of them that is no multiple of that
+TILES = [(2050, 72, 4104, 40, 3), (2050, 264, 4104, 16, 9), (2303, 520, 4104, 8, 1), (2050, 72, 2056, 33, 5),
+         (1030, 136, 4104, 16, 4), (1500, 200, 4104, 64, 2), (2050, 4104, 1032, 16, 3), (1030, 4104, 2056, 24, 7),
+         (513, 72, 4104, 16, 3), (1030, 392, 2056, 9, 5), (513, 4104, 2056, 64, 3), (257, 4104, 4104, 16, 20),
+         (130, 1032, 264, 128, 4), (70, 2056, 520, 256, 3)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("rows", ["mixed", "runs"])
+@pytest.mark.parametrize("shape", TILES)
+def test_tiles(gelim, cuda, shape, rows, layout, dtype):
+    args = make(cuda, *shape, dtype, layout, rows)
+    check(gelim.ops.adapter_matmul(*args), *ref_product(*args, device=cuda))
+    T, K, N, r, n = shape
+    dY = torch.randn(T, N, generator=torch.Generator().manual_seed(2)).to(dtype).to(cuda)
+    for v, t in zip(gelim.ops.adapter_matmul_grad(dY, *args), ref_grad(dY, *args, device=cuda)):
+        check(v, *t)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 17, 40, 64])
+@pytest.mark.parametrize("K, N", [(1, 1), (3, 7), (7, 3), (8, 8), (31, 9), (33, 127), (511, 129), (4097, 130)])
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+def test_few_rows_of_odd_sizes(gelim, cuda, T, K, N, layout, dtype):
+    args = make(cuda, T, K, N, 5, 3, dtype, layout)
     check(gelim.ops.adapter_matmul(*args), *ref_product(*args))
 
 
@@ -200,15 +230,15 @@ def test_large_and_small_low_rank_parts(gelim, cuda, T, dtype):
     check(gelim.ops.adapter_matmul(*args), ref, tol + 2.0 ** -25)  # half a step of fp16's subnormal numbers
 
 
-def ref_grad(dY, X, W, A, B, index, scale):
+def ref_grad(dY, X, W, A, B, index, scale, device="cpu"):
     dtype = X.dtype
-    dY, X, W, A, B, index = (v.detach().cpu() for v in (dY, X, W, A, B, index))
+    dY, X, W, A, B, index = (v.detach().to(device) for v in (dY, X, W, A, B, index))
     dY, X, W, A, B = (v.double() for v in (dY, X, W, A, B))
     T, K = X.shape
     n, _, r = A.shape
     N = W.shape[1]
     scale = torch.full((n,), float(scale), dtype=torch.float64) if not isinstance(scale, torch.Tensor) \
-        else scale.cpu().double()
+        else scale.to(device).double()
     eps, u = torch.finfo(dtype).eps / 2, 2.0 ** -23
     split = 0.0 if dtype == torch.float32 else 2.0 ** -16
     tiny = torch.finfo(dtype).smallest_normal
@@ -242,6 +272,7 @@ def test_gradient(gelim, cuda, shape, layout, dtype):
     got = gelim.ops.adapter_matmul_grad(dY, *args)
     for v, t, like in zip(got, ref_grad(dY, *args), (args[0], args[2], args[3])):
         check(v, *t)
+        assert like is args[0] or v.stride() == like.stride() or 1 in like.shape
         assert v.shape == like.shape and v.dtype == dtype
 
 
