@@ -449,11 +449,13 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish a) {
   }
 }
 
+bool one_row(const Finish& e) { return (int64_t)e.rows.T * e.blocks < 2048; }
+int64_t finish_groups(const Finish& e) { return (int64_t)(one_row(e) ? e.rows.T : (e.rows.T + 3) / 4) * e.blocks; }
 template <class T>
 void finish(const Finish& e, hipStream_t s) {
-  const int64_t groups = (int64_t)e.rows.T * e.blocks;
-  if (groups < 2048) hipLaunchKernelGGL((finish_kernel<T, true>), dim3((unsigned)groups), dim3(256), 0, s, e);
-  else hipLaunchKernelGGL((finish_kernel<T, false>), dim3((unsigned)((e.rows.T + 3) / 4 * e.blocks)), dim3(256), 0, s, e);
+  const dim3 grid((unsigned)finish_groups(e));
+  if (one_row(e)) hipLaunchKernelGGL((finish_kernel<T, true>), grid, dim3(256), 0, s, e);
+  else hipLaunchKernelGGL((finish_kernel<T, false>), grid, dim3(256), 0, s, e);
 }
 
 // ---- many rows ------------------------------------------------------------
@@ -1455,14 +1457,20 @@ int check(const gelim_adapter_args& a, bool grad) {
   if (!a.index && a.n != 1 && a.T)
     return GELIM_FAIL(GELIM_E_ARG, "adapter: an index is needed with more than one adapter");
   if (!a.W || !a.A || !a.B || (a.T && (!a.X || !a.Y))) return GELIM_FAIL(GELIM_E_ARG, "adapter: null matrix");
-  if (a.ws_bytes < gelim_adapter_workspace(&a, grad)) return GELIM_FAIL(GELIM_E_ARG, "adapter: workspace too small");
+  const int64_t need = gelim_adapter_workspace(&a, grad);
+  if (need < 0) return (int)need;
+  if (a.ws_bytes < need) return GELIM_FAIL(GELIM_E_ARG, "adapter: workspace too small");
   return GELIM_OK;
 }
 
 // Hands out the workspace; with a null base it only counts.
 struct Space {
   char* base;
-  int64_t used = 0;
+  int64_t used = 0, threads = 0;  // threads: of the largest launch
+  unsigned launch(int64_t groups, int64_t block, int64_t across = 1) {
+    threads = std::max(threads, groups * block * across);
+    return (unsigned)groups;
+  }
   template <class P>
   P* take(int64_t count) {
     P* p = (P*)(base + used);
@@ -1517,8 +1525,11 @@ int few_product(const Problem& p, const Rows& g, int r, Space& ws, hipStream_t s
   f.ldp = f.blocks * 16 * M::kE;
   f.part = ws.take<float>((int64_t)f.splits * g.T * f.ldp);
   f.low = ws.take<float>((int64_t)f.low_splits * g.T * r);
+  const dim3 grid(ws.launch((int64_t)f.blocks * f.splits + g.T * f.low_splits, 256));
+  Finish e{f.part, f.low, p.G, g, nullptr, p.N, r, f.ldp, f.splits, f.low_splits, r, (p.N + 255) / 256,
+           p.Y, p.ldy};
+  ws.launch(finish_groups(e), 256);
   if (!run) return GELIM_OK;
-  const dim3 grid((unsigned)(f.blocks * f.splits + g.T * f.low_splits));
   const int tt = (g.T + 15) / 16;
   auto launch = [&](auto kc) {
     constexpr bool KC = decltype(kc)::value;
@@ -1528,8 +1539,6 @@ int few_product(const Problem& p, const Rows& g, int r, Space& ws, hipStream_t s
   };
   if (p.w_kc) launch(std::true_type{});
   else launch(std::false_type{});
-  Finish e{f.part, f.low, p.G, g, nullptr, p.N, r, f.ldp, f.splits, f.low_splits, r, (p.N + 255) / 256,
-           p.Y, p.ldy};
   finish<T>(e, s);
   HIP_TRY(hipGetLastError());
   return GELIM_OK;
@@ -1545,7 +1554,7 @@ struct Many {
   int rb, rp;
   Prepare prep{};
   Order order{};
-  unsigned groups = 0;
+  int64_t groups = 0;
   Space& ws;
 
   Many(const gelim_adapter_args& args, Space& space) : a(args), g(rows_of(args)), ws(space) {
@@ -1571,8 +1580,9 @@ struct Many {
     Copy& c = prep.copy[prep.copies++];
     c = {src, ws.template take<T>((int64_t)count * rows * ld), rows, cols, ld, count, have, order,
          order == kRows && src.cs == 1, (int)groups - prep.order_groups};
-    groups += c.straight ? (unsigned)(((int64_t)count * rows * (ld / E) + kStraight - 1) / kStraight)
-                         : (unsigned)(count * ((rows + kCopyTile - 1) / kCopyTile) * ((ld + kCopyTile - 1) / kCopyTile));
+    groups += c.straight ? ((int64_t)count * rows * (ld / E) + kStraight - 1) / kStraight
+                         : (int64_t)count * ((rows + kCopyTile - 1) / kCopyTile) * ((ld + kCopyTile - 1) / kCopyTile);
+    ws.launch(groups, kPrepare);
     return (T*)c.dst;
   }
   static bool aligned(const void* p, int64_t ld, int64_t len) {
@@ -1603,6 +1613,7 @@ struct Many {
     const int flight = rb <= 2 ? 4 : rb == 4 ? 2 : 1;
     l.many = l.pieces <= 144;
     l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (low_waves(rb, l.many) * flight), 1, 16));
+    ws.launch((int64_t)l.pieces * l.splits, low_waves(rb, l.many) * 64);
     if (l.splits > 1) {
       l.part = ws.template take<float>(l.splits * a.T * rp);
       l.arrived = prep.counter + prep.counters;
@@ -1613,7 +1624,7 @@ struct Many {
     return l;
   }
   int run_prepare(hipStream_t s) {
-    if (groups) hipLaunchKernelGGL(prepare_kernel<T>, dim3(groups), dim3(kPrepare), 0, s, prep);
+    if (groups) hipLaunchKernelGGL(prepare_kernel<T>, dim3((unsigned)groups), dim3(kPrepare), 0, s, prep);
     return GELIM_OK;
   }
   void run_low(const Low* l, int count, hipStream_t s) {
@@ -1671,6 +1682,10 @@ struct Many {
     else
       for (const Shape& h : k32) look(h);
   }
+  Finish joined(const Plan& q) const {
+    const Big& b = q.b;
+    return {b.part, nullptr, View{}, g, order.perm, b.N, 0, b.ldp, b.splits, 0, 0, (b.N + 255) / 256, b.Y, b.ldy};
+  }
   Plan big_of(const Problem& p, const Wide& U) {
     Plan q{};
     Big& b = q.b;
@@ -1693,6 +1708,8 @@ struct Many {
       b.ldp = b.tiles_n * q.bn;
       b.part = ws.template take<float>((int64_t)b.splits * a.T * b.ldp);
     }
+    ws.launch((int64_t)b.tiles_t * b.tiles_n, q.bt * q.bn >= 256 * 128 ? 512 : 256, b.splits);
+    if (b.splits > 1) ws.launch(finish_groups(joined(q)), 256);
     b.G = copy(turned(p.G), (int)up(p.N, 32), p.N, (int)a.r, rp, (int)a.n, kFrag32);
     return q;
   }
@@ -1720,11 +1737,7 @@ struct Many {
     };
     if (q.kc) shape(std::true_type{});
     else shape(std::false_type{});
-    if (b.splits > 1) {
-      Finish e{b.part, nullptr, View{}, g, order.perm, b.N, 0, b.ldp, b.splits, 0, 0,
-               (b.N + 255) / 256, b.Y, b.ldy};
-      finish<T>(e, s);
-    }
+    if (b.splits > 1) finish<T>(joined(q), s);
   }
 };
 
@@ -1770,7 +1783,7 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   op.table = m.prep.pieces[1].table;
   const bool share = pcs >= 4 * a.n;
   int sides = 0;
-  unsigned outer_groups = 0, sum_groups = 0;
+  int64_t outer_groups = 0, sum_groups = 0;
   for (int k = 0; k < 2; ++k) {
     if (!(k ? a.dB : a.dA) && !all) continue;
     const auto& U = k ? dY : X;
@@ -1786,11 +1799,15 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
     u.as = (int64_t)a.r * cols;
     const bool along = k ? !a.b_trans : a.a_trans;  // columns side by side
     u.cs = along ? 1 : a.r, u.rs = along ? cols : 1;
-    u.blocks = (int)((cols + 63) / 64 * ((a.r + (share ? 3 : 15)) / (share ? 4 : 16)));
+    const int64_t blocks = (cols + 63) / 64 * ((a.r + (share ? 3 : 15)) / (share ? 4 : 16));
+    u.blocks = (int)blocks;
     o.out = u.out, o.as = u.as, o.cs = u.cs, o.rs = u.rs, o.cols = cols;
-    outer_groups = std::max(outer_groups, (unsigned)(pcs * o.blocks));
-    sum_groups = std::max(sum_groups, (unsigned)u.blocks);
+    outer_groups = std::max(outer_groups, (int64_t)pcs * o.blocks);
+    sum_groups = std::max(sum_groups, blocks);
   }
+  const unsigned sum_depth = (unsigned)std::min<int64_t>(a.n, 4096);
+  ws.launch(outer_groups, 256, 2 * m.rb);
+  ws.launch(sum_groups, 256, 2);
   if (!run) return GELIM_OK;
   m.run_prepare(s);
   if (a.T) {
@@ -1801,8 +1818,8 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   if (sides) {
     if (a.T) {
       int per = std::min(m.rb, 4);  // blocks of 16 ranks a workgroup, fewer where that fills the chip
-      while (per > 1 && (int64_t)outer_groups * sides * (m.rb / per) < 384) per /= 2;
-      const dim3 grid(outer_groups, (unsigned)sides, (unsigned)(m.rb / per));
+      while (per > 1 && outer_groups * sides * (m.rb / per) < 384) per /= 2;
+      const dim3 grid((unsigned)outer_groups, (unsigned)sides, (unsigned)(m.rb / per));
       auto launch = [&](auto direct) {
         constexpr bool D = decltype(direct)::value;
         if (per == 1) hipLaunchKernelGGL((outer_kernel<T, 1, D>), grid, dim3(256), 0, s, op);
@@ -1816,7 +1833,7 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
       HIP_TRY(hipGetLastError());
       return GELIM_OK;
     }
-    const dim3 grid(sum_groups, (unsigned)sides, (unsigned)std::min<int64_t>(a.n, 4096));
+    const dim3 grid((unsigned)sum_groups, (unsigned)sides, sum_depth);
     if (share) hipLaunchKernelGGL((sum_kernel<T, true>), grid, dim3(256), 0, s, sp);
     else hipLaunchKernelGGL((sum_kernel<T, false>), grid, dim3(256), 0, s, sp);
   }
@@ -1852,6 +1869,8 @@ extern "C" int64_t gelim_adapter_workspace(const gelim_adapter_args* a, int grad
   GELIM_TRY(gelim::check_shape(*a));
   gelim::Space ws{nullptr};
   gelim::run_or_count(*a, grad != 0, ws, nullptr, false);
+  // a workgroup's number times its threads is an int in the kernels
+  if (ws.threads > INT32_MAX) return GELIM_FAIL(GELIM_E_ARG, "adapter: too large for one launch");
   return ws.used;
 }
 

@@ -96,11 +96,14 @@ def _check(X, W, A, B, index, scale):
 @lru_cache(maxsize=4096)
 def _workspace_bytes(grad: bool, *layout) -> int:
     """What a call of these sizes and layouts needs."""
-    dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, ldy, odd, indexed = layout
-    # the addresses' low bits choose between aligned and unaligned loads, so they take the place of the addresses
-    args = _ARGS.pack(dtype, T, K, N, r, n, odd, ldx, odd, ldw, wt, 0, 0, lda, at, 0, 0, ldb, bt, indexed, 0, 0.0,
-                      odd, ldy, 0, 0, 0, 0, 0, 0)
-    return _native.lib().gelim_adapter_workspace(args, grad)
+    dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, ldy, x, w, y, indexed = layout
+    # an address's low bits choose between reading in place and copying, so they take the place of the addresses
+    args = _ARGS.pack(dtype, T, K, N, r, n, x, ldx, w, ldw, wt, 0, 0, lda, at, 0, 0, ldb, bt, indexed, 0, 0.0,
+                      y, ldy, 0, 0, 0, 0, 0, 0)
+    need = _native.lib().gelim_adapter_workspace(args, grad)
+    if need < 0:
+        _native.check(need, "adapter_matmul")
+    return need
 
 
 def _call(grad, dev, T, K, N, n, r, X, W, A, B, index, scale, Y, dX=None, dA=None, dB=None):
@@ -119,7 +122,7 @@ def _call(grad, dev, T, K, N, n, r, X, W, A, B, index, scale, Y, dX=None, dA=Non
     dtype = TYPES[X.dtype]
     xp, wp, yp = X.data_ptr(), W.data_ptr(), Y.data_ptr()
     ws_bytes = _workspace_bytes(grad, dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, ldy,
-                                (xp | wp | yp) & 15, index is not None)
+                                xp & 15, wp & 15, yp & 15, index is not None)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     args = _ARGS.pack(dtype, T, K, N, r, n, xp, ldx, wp, ldw, wt, A.data_ptr(), A.stride(0), lda, at, B.data_ptr(),
                       B.stride(0), ldb, bt, 0 if index is None else index.data_ptr(),
@@ -144,12 +147,13 @@ def adapter_matmul(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.T
     X (T, K), W (K, N), A (n, K, r), B (n, r, N): float32, bfloat16 or float16,
     all of one type.  Any strides; W, A and B are read in place if one of their
     last two dimensions has unit stride, so weights kept as (out, in) are
-    passed as transposed views.  T may be 0; r is at most 256.
+    passed as transposed views.  T may be 0; r is at most 256, n at most 65535.
     index (T,) int32: the adapter of each row, in any order; -1: the row has
     none; any other value outside [0, n) makes the row NaN.  None: n is 1 and
     every row has that adapter.
     scale: a number, or (n,) float32 on the device.
-    out: (T, N) with unit column stride, overlapping no input.
+    out: (T, N) with unit column stride; no input begins or ends between its
+    first and last element.
     Runs on the current stream; may be captured into a graph."""
     dev, T, K, N, n, r = _check(X, W, A, B, index, scale)
     if out is None:
@@ -159,6 +163,8 @@ def adapter_matmul(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.T
             raise ValueError("out must have the type and device of X")
         if out.shape != (T, N) or (N > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < N):
             raise ValueError("out must be a (T, N) tensor with unit column stride")
+        if torch.is_grad_enabled() and out.requires_grad:
+            raise ValueError("out is not recorded by autograd: call under torch.no_grad()")
         if any(_overlap(out, t) for t in (X, W, A, B, index, scale) if isinstance(t, torch.Tensor)):
             raise ValueError("out overlaps an input")
     if T:

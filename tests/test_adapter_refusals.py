@@ -49,3 +49,18 @@ def test_native_entry_refuses(gelim, field, value, grad):
     fn = lib.gelim_adapter_matmul_grad if grad else lib.gelim_adapter_matmul
     assert fn(adapter._ARGS.pack(*[vals[k] for k in names]), None) == _native.E_ARG
     assert "adapter" in _native.last_error()
+
+
+@pytest.mark.parametrize("sizes", [dict(T=2 ** 30 - 64, K=8, N=8, n=1), dict(T=64, K=1, N=2 ** 30 - 64, n=1),
+                                   dict(T=100, K=2 ** 19, N=64, n=65535)])
+def test_sizes_beyond_one_launch(gelim, sizes):
+    from gelim import _native
+    from gelim.ops import adapter
+
+    v = dict(r=16) | sizes
+    grad = v["T"] == 100
+    with pytest.raises(_native.GelimError, match="one launch"):
+        adapter._workspace_bytes(grad, 1, v["T"], v["K"], v["N"], v["r"], v["n"], v["K"], v["N"], 0, v["r"], 0, v["N"], 0,
+                                 v["N"], 0, 0, 0, True)
+    # as many rows as one launch takes
+    assert adapter._workspace_bytes(False, 1, 2 ** 26, 64, 64, 16, 1, 64, 64, 0, 16, 0, 64, 0, 64, 0, 0, 0, False) > 0

@@ -95,6 +95,32 @@ def test_tiles(gelim, cuda, shape, rows, layout, dtype):
         check(v, *t)
 
 
+def shifted(v):
+    """v one element behind a multiple of 16 bytes."""
+    return torch.cat([v.new_zeros(1), v.reshape(-1)])[1:].view(v.shape)
+
+
+# one operand of three at another address than the others: the tile is chosen by what is copied, and so is the workspace
+@pytest.mark.parametrize("grad, which, T, K, N, layout", [
+    (False, "W", 2973, 852, 680, "kn"), (False, "W", 943, 1120, 732, "kn"), (False, "Y", 630, 1092, 1136, "kn"),
+    (False, "Y", 1013, 1112, 664, "kn"), (True, "X", 2983, 448, 852, "nk"), (True, "X", 1551, 796, 856, "nk"),
+    (True, "W", 2099, 1200, 852, "nk"), (True, "Y", 2686, 860, 832, "nk")])
+def test_addresses(gelim, cuda, grad, which, T, K, N, layout):
+    X, W, A, B, index, scale = make(cuda, T, K, N, 16, 2, torch.float32, layout)
+    X = shifted(X) if which == "X" else X
+    if which == "W":
+        W = shifted(W) if layout == "kn" else shifted(W.t()).t()
+    args = X, W, A, B, index, scale
+    if not grad:
+        out = shifted(X.new_zeros(T, N)) if which == "Y" else None
+        check(gelim.ops.adapter_matmul(*args, out=out), *ref_product(*args, device=cuda))
+        return
+    dY = torch.randn(T, N, generator=torch.Generator().manual_seed(2)).to(cuda)
+    dY = shifted(dY) if which == "Y" else dY
+    for v, t in zip(gelim.ops.adapter_matmul_grad(dY, *args), ref_grad(dY, *args, device=cuda)):
+        check(v, *t)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [1, 17, 40, 64])
 @pytest.mark.parametrize("K, N", [(1, 1), (3, 7), (7, 3), (8, 8), (31, 9), (33, 127), (511, 129), (4097, 130)])
