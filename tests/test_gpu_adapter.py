@@ -190,6 +190,42 @@ def test_what_a_row_does_not_use_does_not_reach_it(gelim, cuda, T, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T, K, N", [(2050, 264, 4104), (1030, 136, 4104), (513, 72, 4104), (257, 4104, 1032)])
+def test_rows_of_large_tiles_stay_apart(gelim, cuda, T, K, N, dtype):
+    """NaN and infinities in a row or in an adapter, where a wave's rows have one adapter, several, and none."""
+    X, W, A, B, index, scale = make(cuda, T, K, N, 16, 4, dtype, rows="runs")
+    index[40:70] = torch.arange(30, device=cuda).int() % 4
+    want = gelim.ops.adapter_matmul(X, W, A, B, index, scale)
+    dY = torch.randn(T, N, generator=torch.Generator().manual_seed(5)).to(dtype).to(cuda)
+    grads = gelim.ops.adapter_matmul_grad(dY, X, W, A, B, index, scale)
+    rows = torch.tensor([0, 41, 63, 64, T // 2, T - 1], device=cuda)
+    clean = torch.ones(T, dtype=torch.bool, device=cuda)
+    clean[rows] = False
+    X2, dY2 = X.clone(), dY.clone()
+    X2[rows[::2]], X2[rows[1::2], 3] = float("nan"), float("inf")
+    dY2[rows] = float("nan")
+    Y = gelim.ops.adapter_matmul(X2, W, A, B, index, scale)
+    assert torch.equal(Y[clean], want[clean]) and not torch.isfinite(Y[rows]).any()
+    dX = gelim.ops.adapter_matmul_grad(dY2, X, W, A, B, index, scale)[0]
+    assert torch.equal(dX[clean], grads[0][clean]) and torch.isnan(dX[rows]).all()
+    A2, B2 = A.clone(), B.clone()
+    A2[2], B2[2] = float("nan"), float("inf")
+    Y = gelim.ops.adapter_matmul(X, W, A2, B2, index, scale)
+    other = index != 2
+    assert torch.equal(Y[other], want[other]) and torch.isnan(Y[~other]).all()
+    got = gelim.ops.adapter_matmul_grad(dY, X, W, A2, B2, index, scale)
+    assert torch.equal(got[0][other], grads[0][other])
+    for a, b in zip(got[1:], grads[1:]):
+        assert torch.equal(a[[0, 1, 3]], b[[0, 1, 3]]) and torch.isnan(a[2]).all()
+    # rows with no adapter, whatever they hold, add nothing to the gradients
+    index[rows] = -1
+    fine = gelim.ops.adapter_matmul_grad(torch.where(clean[:, None], dY, 0), X, W, A, B, index, scale)
+    got = gelim.ops.adapter_matmul_grad(dY2, X2, W, A, B, index, scale)
+    for a, b in zip(got[1:], fine[1:]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [6, 150])
 def test_strides(gelim, cuda, T, dtype):
     """Slices of larger matrices, transposed X, a repeated row, adapters picked with a step, a strided index."""
@@ -391,6 +427,52 @@ def test_other_stream(gelim, cuda):
     s.synchronize()
     for v in got:
         assert torch.equal(v, want)
+
+
+def test_two_at_a_time(gelim, cuda):
+    """Calls and replays on two streams, from two threads: sums cut over workgroups that wait for each other's parts."""
+    from threading import Thread
+
+    sizes = [(70, 2056, 520, 64, 3), (20, 1024, 512, 8, 2), (257, 4104, 1032, 16, 5)]
+    sets = [[make(cuda, *z, torch.bfloat16, seed=s) for z in sizes] for s in range(2)]
+
+    def work(args):
+        Y = gelim.ops.adapter_matmul(*args)
+        return [Y, *gelim.ops.adapter_matmul_grad(Y, *args)]
+
+    want = [[work(a) for a in mine] for mine in sets]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for mine in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append([work(a) for a in mine])
+        graphs.append(graph)
+    got, failed = [[], []], []
+
+    def thread(k):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    got[k].append([work(a) for a in sets[k]])
+                    graphs[k].replay()
+                    got[k].append([[v.clone() for v in vs] for vs in outs[k]])
+            s.synchronize()
+        except Exception as e:
+            failed.append(e)
+
+    threads = [Thread(target=thread, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for k in range(2):
+        for once in got[k]:
+            for a, b in zip(once, want[k]):
+                for v, w in zip(a, b):
+                    assert torch.equal(v, w)
 
 
 @pytest.mark.parametrize("T", [2, 70])
