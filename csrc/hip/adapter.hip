@@ -1169,14 +1169,16 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   for (; kt + 2 * S - 1 < whole; kt += S) {
 #pragma unroll
     for (int st = 0; st < S; ++st) step(std::false_type{}, kt + st, st);
-    if constexpr (sizeof(T) == 4)
+    if constexpr (sizeof(T) == 4) {
       // fp32: sums of about 512 values, then of those, or the rounding of one long sum would grow with its length
-      if ((kt - k0) / S % (16 / S) == 16 / S - 1)
+      constexpr int kLong = 512 / (S * BK);
+      if ((kt - k0) / S % kLong == kLong - 1)
 #pragma unroll
         for (int m = 0; m < kMma; ++m) {
           total[m / TT][m % TT] += acc[m / TT][m % TT];
           acc[m / TT][m % TT] = f16{};
         }
+    }
   }
   for (; kt < k1; kt += S)
 #pragma unroll
@@ -1655,25 +1657,31 @@ struct Many {
     int bt, bn;
     Problem p;
   };
-  // The tile by what it is expected to take: the rounds of workgroups that fit the chip at a time, each of a fixed
+  // The tile by what it is expected to take: the rounds of 256 workgroups, or of 512 where two fit a CU, each of a fixed
   // part (a launch's share, the first loads, the low-rank part, the end) and the tiles' steps of 128 bytes
-  // along the sum, both as measured (us).
+  // along the sum, both as measured (us) with one workgroup a CU and with two.
   void choose(Plan& q, int nk) {
     struct Shape {
-      int bt, bn, at_once;  // at_once: workgroups
-      double fixed, step;
+      int bt, bn;
+      double fixed, step, fixed2, step2;  // step2 0: one fits
     };
-    static constexpr Shape k16[] = {{256, 256, 256, 16.7, 1.61}, {256, 128, 256, 11.9, 0.90},
-                                    {128, 128, 256, 9.4, 0.50}, {64, 64, 512, 5.3, 0.39}};
-    static constexpr Shape k32[] = {{128, 128, 256, 12.3, 2.26}, {64, 64, 512, 6.4, 1.37}};
+    static constexpr Shape k16[] = {{256, 256, 16.7, 1.61, 0, 0}, {256, 128, 11.9, 0.90, 0, 0},
+                                    {128, 128, 9.4, 0.50, 0, 0}, {64, 64, 5.6, 0.26, 5.2, 0.39}};
+    static constexpr Shape k32[] = {{128, 128, 12.3, 2.26, 0, 0}, {128, 64, 9.7, 1.17, 10.0, 2.37},
+                                    {64, 64, 6.5, 0.65, 6.0, 1.30}};
     double best = 1e30;
     auto look = [&](const Shape& h) {
       const int64_t tiles = ((a.T + h.bt - 1) / h.bt) * ((q.p.N + h.bn - 1) / h.bn);
       for (int splits = 1; splits <= 16 && (splits == 1 || (h.bn < 256 && nk / splits >= 4)); ++splits) {
-        const double rounds = (double)((tiles * splits + h.at_once - 1) / h.at_once);
+        const int64_t groups = tiles * splits, steps = (nk + splits - 1) / splits;
+        const double one = h.fixed + h.step * steps, two = h.fixed2 + h.step2 * steps;
+        const int64_t rest = groups % 512;
+        double us = (double)((groups + 255) / 256) * one;
+        // a last round of less than a workgroup a CU: some CUs get two of them all the same, unless it is the only one
+        const double last = rest > 256 ? two : rest ? (groups < 512 ? one : (one + two) / 2) : 0;
+        if (h.step2 > 0) us = (double)(groups / 512) * two + last;
         // joining the parts: a launch, and reading them
-        const double join = splits == 1 ? 0 : 3 + 0.6e-6 * (double)splits * a.T * q.p.N;
-        const double us = rounds * (h.fixed + h.step * ((nk + splits - 1) / splits)) + join;
+        if (splits > 1) us += 3 + 0.6e-6 * (double)splits * a.T * q.p.N;
         if (us < best) best = us, q.bt = h.bt, q.bn = h.bn, q.b.splits = splits;
       }
     };
@@ -1729,7 +1737,8 @@ struct Many {
     auto shape = [&](auto kc) {
       constexpr bool KC = decltype(kc)::value;
       if (q.bt == 64) launch<KC, 64, 64, 2, 2, 4>(b, s);
-      else if (q.bt == 128) launch<KC, 128, 128, 2, 2, 4>(b, s);
+      else if (q.bt == 128 && q.bn == 128) launch<KC, 128, 128, 2, 2, 4>(b, s);
+      else if constexpr (sizeof(T) == 4) launch<KC, 128, 64, 2, 2, 3>(b, s);
       else if constexpr (sizeof(T) == 2) {
         if (q.bn == 128) launch<KC, 256, 128, 4, 2, 3>(b, s);
         else launch<KC, 256, 256, 2, 4, 2>(b, s);
