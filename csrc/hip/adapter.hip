@@ -681,7 +681,7 @@ struct Low {
   float *low, *by;
   void* split;
   int cu, ldf, pieces, splits;  // cu: values in a row of U, a multiple of 16 bytes
-  float* part;                  // split, place, rank; with splits > 1
+  float* part;                  // piece, split, fragment, lane, 4 values; with splits > 1
   int* arrived;                 // of each piece
   bool many;
 };
@@ -723,8 +723,8 @@ __global__ __launch_bounds__(low_waves(RB, MANY) * 64) void low_kernel(LowPair b
     u[t] = (const T*)a.U + row_at(both.order, pc.begin + min(t * 16 + l16, pc.count - 1)) * a.ldu;
   const Frag* f = (const Frag*)((const T*)a.F + (int64_t)pc.adapter * rp * a.ldf) + lane;
   const int steps = (a.cu + M::kStep - 1) / M::kStep;
-  const int parts = kWaves * a.splits, mine = split * kWaves + wave;
-  const int s0 = (int)((int64_t)steps * mine / parts), s1 = (int)((int64_t)steps * (mine + 1) / parts);
+  const int shares = kWaves * a.splits, share = split * kWaves + wave;
+  const int s0 = (int)((int64_t)steps * share / shares), s1 = (int)((int64_t)steps * (share + 1) / shares);
   f4 acc[RB][2] = {};
   constexpr int kFlight = RB <= 2 ? 4 : RB == 4 ? 2 : 1;  // by the registers of two workgroups a CU
   for (int s = s0; s < s1; s += kFlight) {
@@ -767,22 +767,20 @@ __global__ __launch_bounds__(low_waves(RB, MANY) * 64) void low_kernel(LowPair b
     __syncthreads();
   }
   if (a.splits > 1) {
-    // The parts go past the caches (agent-scope relaxed atomics), so that no cache has to be written back or
-    // dropped as by a fence; the count goes up when they have arrived (vmcnt 0).
-    auto part = [&](int p, int t, int j) {
-      const int64_t at = pc.begin + min(t * 16 + l16, pc.count - 1);
-      return a.part + ((int64_t)p * both.rows.T + at) * rp + j * 16 + g * 4;
-    };
+    // The parts go past the caches that other XCDs do not see (sc1: the scope of the whole device), so that none has to
+    // be written back or dropped as by a fence; the count goes up when they have arrived (vmcnt 0).
+    constexpr int kDevice = 16;
+    typedef int i4 __attribute__((ext_vector_type(4)));
+    float* mine = a.part + (int64_t)piece * a.splits * (RB * 2 * 64 * 4);
+    auto parts = __builtin_amdgcn_make_buffer_rsrc(mine, 0, a.splits * RB * 2 * 1024, 0x00027000);
     __shared__ int last;
     if (wave == 0) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int j = 0; j < RB; ++j)
 #pragma unroll
-        for (int j = 0; j < RB; ++j)
-          if (t * 16 + l16 < pc.count)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              __hip_atomic_store(part(split, t, j) + e, acc[j][t][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int t = 0; t < 2; ++t)
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i4, acc[j][t]), parts,
+                                                 ((split * RB + j) * 2 + t) * 1024 + lane * 16, 0, kDevice);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (lane == 0)
         last = __hip_atomic_fetch_add(a.arrived + piece, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.splits - 1;
@@ -795,10 +793,8 @@ __global__ __launch_bounds__(low_waves(RB, MANY) * 64) void low_kernel(LowPair b
         f4 w[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[q][e] = __hip_atomic_load(part(min(p + q, a.splits - 1), m % 2, m / 2) + e, __ATOMIC_RELAXED,
-                                        __HIP_MEMORY_SCOPE_AGENT);
+          w[q] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(
+                     parts, (min(p + q, a.splits - 1) * RB * 2 + m) * 1024 + lane * 16, 0, kDevice));
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (p + q < a.splits) v += w[q];
@@ -1617,7 +1613,7 @@ struct Many {
     l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (low_waves(rb, l.many) * flight), 1, 16));
     ws.launch((int64_t)l.pieces * l.splits, low_waves(rb, l.many) * 64);
     if (l.splits > 1) {
-      l.part = ws.template take<float>(l.splits * a.T * rp);
+      l.part = ws.template take<float>((int64_t)l.pieces * l.splits * kLowRows * rp);
       l.arrived = prep.counter + prep.counters;
       prep.counters += l.pieces;
     }
