@@ -683,7 +683,6 @@ struct Low {
   int cu, ldf, pieces, splits;  // cu: values in a row of U, a multiple of 16 bytes
   float* part;                  // piece, split, fragment, lane, 4 values; with splits > 1
   int* arrived;                 // of each piece
-  bool many;
 };
 struct LowPair {
   Low p[2];
@@ -692,7 +691,7 @@ struct LowPair {
   const Piece* table;
 };
 constexpr int kLowRows = 32;
-constexpr int low_waves(int rank_blocks, bool many) { return many && rank_blocks <= 8 ? 16 : 8; }  // MANY: with few pieces
+constexpr int kLowWaves = 8;
 
 // v as upper and lower part of the type; the lower is 0 beside an infinity or NaN
 template <class T>
@@ -705,11 +704,11 @@ __device__ __forceinline__ int to_fp16_range(float most) {
   return most > 0.f ? min(max(13 - ilogbf(most), -100), 100) : 0;
 }
 
-template <class T, int RB, bool MANY>
-__global__ __launch_bounds__(low_waves(RB, MANY) * 64) void low_kernel(LowPair both) {
+template <class T, int RB>
+__global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int E = M::kE, rp = 16 * RB, kWaves = low_waves(RB, MANY);
+  constexpr int E = M::kE, rp = 16 * RB, kWaves = kLowWaves;
   __shared__ f4 lds[kWaves / 2][RB * 2][64];
   const Low& a = both.p[blockIdx.y];
   const int piece = blockIdx.x % a.pieces, split = blockIdx.x / a.pieces;
@@ -1609,9 +1608,8 @@ struct Many {
     const int steps = (C + Mma<T>::kStep - 1) / Mma<T>::kStep;
     // cut the sum where that leaves a wave a round of loads or more
     const int flight = rb <= 2 ? 4 : rb == 4 ? 2 : 1;
-    l.many = l.pieces <= 144;
-    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (low_waves(rb, l.many) * flight), 1, 16));
-    ws.launch((int64_t)l.pieces * l.splits, low_waves(rb, l.many) * 64);
+    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (kLowWaves * flight), 1, 16));
+    ws.launch((int64_t)l.pieces * l.splits, kLowWaves * 64);
     if (l.splits > 1) {
       l.part = ws.template take<float>((int64_t)l.pieces * l.splits * kLowRows * rp);
       l.arrived = prep.counter + prep.counters;
@@ -1636,8 +1634,7 @@ struct Many {
     const dim3 grid(most, (unsigned)count);
     auto launch = [&](auto blocks) {
       constexpr int RB = decltype(blocks)::value;
-      if (l[0].many) hipLaunchKernelGGL((low_kernel<T, RB, true>), grid, dim3(low_waves(RB, true) * 64), 0, s, both);
-      else hipLaunchKernelGGL((low_kernel<T, RB, false>), grid, dim3(low_waves(RB, false) * 64), 0, s, both);
+      hipLaunchKernelGGL((low_kernel<T, RB>), grid, dim3(kLowWaves * 64), 0, s, both);
     };
     if (rb == 1) launch(std::integral_constant<int, 1>{});
     else if (rb == 2) launch(std::integral_constant<int, 2>{});
