@@ -692,6 +692,7 @@ struct LowPair {
 };
 constexpr int kLowRows = 32;
 constexpr int kLowWaves = 8;
+constexpr int low_flight(int rank_blocks) { return rank_blocks <= 4 ? 4 : rank_blocks == 8 ? 2 : 1; }  // steps whose loads are under way
 
 // v as upper and lower part of the type; the lower is 0 beside an infinity or NaN
 template <class T>
@@ -725,7 +726,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
   const int shares = kWaves * a.splits, share = split * kWaves + wave;
   const int s0 = (int)((int64_t)steps * share / shares), s1 = (int)((int64_t)steps * (share + 1) / shares);
   f4 acc[RB][2] = {};
-  constexpr int kFlight = RB <= 2 ? 4 : RB == 4 ? 2 : 1;  // by the registers of two workgroups a CU
+  constexpr int kFlight = low_flight(RB);
   for (int s = s0; s < s1; s += kFlight) {
     Frag x[kFlight][2], w[kFlight][RB];
 #pragma unroll
@@ -1607,8 +1608,7 @@ struct Many {
     l.low = ws.template take<float>(a.T * rp);
     const int steps = (C + Mma<T>::kStep - 1) / Mma<T>::kStep;
     // cut the sum where that leaves a wave a round of loads or more
-    const int flight = rb <= 2 ? 4 : rb == 4 ? 2 : 1;
-    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (kLowWaves * flight), 1, 16));
+    l.splits = std::clamp(256 / std::max(1, l.pieces), 1, std::clamp(steps / (kLowWaves * low_flight(rb)), 1, 16));
     ws.launch((int64_t)l.pieces * l.splits, kLowWaves * 64);
     if (l.splits > 1) {
       l.part = ws.template take<float>((int64_t)l.pieces * l.splits * kLowRows * rp);
