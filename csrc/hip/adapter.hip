@@ -178,7 +178,6 @@ struct Few {
 // The first of the kE columns that a lane takes where W's rows run along memory: at the end of a row the lane takes
 // its last kE, some of them a neighbour's as well, who comes to the same sums.
 __device__ __forceinline__ int few_column(int N, int n, int E) { return N >= E ? min(n, N - E) : n; }
-constexpr int kFewGroups = 256;
 // One wave: 16 kE columns of W, its steps of the sum; W_KC: W's sum runs along its rows in memory.
 // Each 16-byte load of 16 neighbouring lanes covers 256 bytes of a row of W (64 where W_KC: two steps make the line).
 // One step's loads in flight: with two, fewer waves fit a SIMD, and 32 rows of 4096 x 4096 took 14.2 instead of 10.9 us.
@@ -1518,7 +1517,11 @@ int few_product(const Problem& p, const Rows& g, int r, Space& ws, hipStream_t s
   f.U = p.U, f.ldu = p.ldu, f.W = p.W, f.F = p.F, f.G = p.G, f.rows = g, f.C = p.C, f.N = p.N, f.r = r;
   f.blocks = (int)((p.N + 16 * M::kE - 1) / (16 * M::kE));
   const int steps = (p.C + M::kStep - 1) / M::kStep;
-  f.splits = std::clamp(kFewGroups / f.blocks, 1, std::max(1, std::min(64, steps / 4)));
+  // workgroups: one a CU, as more cost the second launch what they save (32 rows of bf16 4096 x 4096: 16.2 us with 256,
+  // 17.8 with 512); two for fp32 in rows of N, where a wave has half as many loads under way (8 x 2048 x 7168: 22.5 us with
+  // 256, 17.9 with 512; with W along the sum 60 x 1000 x 2000 takes 14.8 and 17.4)
+  const int groups = sizeof(T) == 4 && !p.w_kc ? 512 : 256;
+  f.splits = std::clamp(groups / f.blocks, 1, std::max(1, std::min(64, steps / 4)));
   f.low_splits = std::clamp(256 / g.T, 1, std::max(1, std::min(16, p.C / 256)));
   f.ldp = f.blocks * 16 * M::kE;
   f.part = ws.take<float>((int64_t)f.splits * g.T * f.ldp);
