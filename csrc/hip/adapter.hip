@@ -8,13 +8,16 @@
 // brings it down to r columns, G_i the factor that brings those up again, so
 // that dX is the same product as Y with the operands turned.
 //
-// Few rows (a decoding step): bound by reading W once.  Two launches: partial
-// sums of U W over pieces of C and of U F_i beside them, then their sums and
-// the product with G_i.
+// Few rows (up to 64, a decoding step): bound by reading W once.  Two launches:
+// partial sums of U W over pieces of C and of U F_i beside them, then their sums
+// and the product with G_i.  32 rows, 64 adapters of rank 16, bf16 4096 x 4096:
+// 10.9 + 5.2 us, W read at 3.1 TB/s (a large copy on this card: 4.95).
 // Many rows: bound by the matrix units.  The rows are ordered by adapter, so a
 // tile of the large product has few adapters; the factors are laid out for the
-// matrix units once per call; U F_i is one pass over U; the large product adds
-// s_i (U F_i) G_i to its accumulators at the end.
+// matrix units once per call; U F_i is one pass over U; the accumulators of the
+// large product begin with s_i (U F_i) G_i.  8192 rows, bf16 8192 x 8192, rank 64:
+// 9 + 60 + 880 us, the large product at 1.25 PFLOP/s (a plain library product of
+// that size: 1.27 to 1.56 by its layout).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -178,9 +181,9 @@ struct Few {
 // The first of the kE columns that a lane takes where W's rows run along memory: at the end of a row the lane takes
 // its last kE, some of them a neighbour's as well, who comes to the same sums.
 __device__ __forceinline__ int few_column(int N, int n, int E) { return N >= E ? min(n, N - E) : n; }
-// One wave: 16 kE columns of W, its steps of the sum; W_KC: W's sum runs along its rows in memory.
-// Each 16-byte load of 16 neighbouring lanes covers 256 bytes of a row of W (64 where W_KC: two steps make the line).
-// One step's loads in flight: with two, fewer waves fit a SIMD, and 32 rows of 4096 x 4096 took 14.2 instead of 10.9 us.
+// One wave: 16 kE columns of W, its steps of the sum; W_KC: W's sum runs along its rows in memory. Each 16-byte
+// load of 16 neighbouring lanes covers 256 bytes of a row of W (64 where W_KC: two steps make the line). One step's
+// loads in flight: with two, fewer waves fit a SIMD, and 32 rows of 4096 x 4096 took 14.2 instead of 10.9 us.
 template <class T, bool W_KC, int TT, bool EDGE>
 __device__ __forceinline__ void few_steps(const Few& a, int n0, int s0, int s1, f4 (&acc)[Mma<T>::kE][TT]) {
   using M = Mma<T>;
@@ -475,7 +478,9 @@ __device__ __forceinline__ int64_t row_at(const Order& o, int64_t at) { return o
 struct Piece {
   int adapter, begin, count, first;  // first: its adapter's first, also with count 0
 };
-__device__ __forceinline__ int first_piece(const Order& o, int i, int size) { return o.start ? o.start[i] / size + i : 0; }
+__device__ __forceinline__ int first_piece(const Order& o, int i, int size) {
+  return o.start ? o.start[i] / size + i : 0;
+}
 __device__ __forceinline__ Piece piece_of(const Piece* table, const Rows& g, int number, int size) {
   if (!table) return {0, number * size, max(0, min(size, g.T - number * size)), number == 0};
   return table[number];
@@ -568,7 +573,8 @@ __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
     for (int q = 0; q < kOrder; ++q)
       if (id[q] == i) p.perm[place++] = (int32_t)(t0 + threadIdx.x * kOrder + q);
   }
-  // this adapter's pieces, and empty ones up to the next adapter's; behind the last adapter empty ones to the table's end
+  // this adapter's pieces, and empty ones up to the next adapter's; behind the last adapter empty ones to the
+  // table's end
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int size = p.pieces[k].size;
@@ -654,7 +660,10 @@ __device__ __forceinline__ void copy_tile(const Copy& c, int tile) {
 }
 
 // The first launch: counters cleared, the order, the factors laid out for the matrix units, and
-// an operand whose rows do not begin at multiples of 16 bytes copied to where they do.
+// an operand whose rows do not begin at multiples of 16 bytes copied to where they do.  All parts run beside each
+// other: 6 us where there is little to copy, X and W of 4096 x 4095 in bf16 26 us (5.1 TB/s).  Read in place by
+// unaligned loads the rows would cost the low-rank pass alone 20 us there (12.5 -> 32.5), as each lane's 16 bytes and
+// its neighbours' then lie in two lines.
 template <class T>
 __global__ __launch_bounds__(kPrepare) void prepare_kernel(Prepare p) {
   int b = blockIdx.x;
@@ -667,13 +676,16 @@ __global__ __launch_bounds__(kPrepare) void prepare_kernel(Prepare p) {
   else copy_tile<T>(p.copy[k], b - p.copy[k].first);
 }
 
-// low (place, rank) = U F_i, 32 places of one adapter by a workgroup, whose waves cut the sum.
-// F is laid out in fragments, ldf values along the sum with zeros behind C.  Bound by
-// reading U and, for every 32 rows, F_i: each wave keeps several steps' loads in flight.  With few rows several
-// workgroups cut the sum once more; the last of them to end adds their parts, always in the same order.
-// Also in fragments of 32 places and 8 ranks for the matrix units of the large product, with 16-bit types as the sum
-// of two values of the type, the upper parts for the lower half of the lanes.  One value's rounding alone would be as large as the
-// result's.  fp16: a row is first brought to below 2^14 by a power of two (`by`), as it may be beyond the type's range.
+// low (place, rank) = U F_i, 32 places of one adapter by a workgroup, whose 8 waves cut the sum (16 waves were no
+// faster at any size, 10.2 instead of 8.3 us for 150 rows of K 2048, rank 64). F is laid out in fragments, ldf
+// values along the sum with zeros behind C.  Bound by reading U and, for every 32 rows, F_i: each wave keeps
+// several steps' loads in flight.  With few rows several workgroups cut the sum once more; the last of them to end
+// adds their parts, always in the same order. Measured, bf16: 2048 x 4096, rank 16, 8.8 us; 8192 x 8192, rank 64,
+// 60 us (U at 2.2 TB/s; more loads under way, waves side by side along a row, or the pieces of an adapter on one
+// XCD changed that by less than the noise). Also in fragments of 32 places and 8 ranks for the matrix units of the
+// large product, with 16-bit types as the sum of two values of the type, the upper parts for the lower half of the
+// lanes.  One value's rounding alone would be as large as the result's.  fp16: a row is first brought to below 2^14
+// by a power of two (`by`), as it may be beyond the type's range.
 struct Low {
   const void *U, *F;
   int64_t ldu;
@@ -691,7 +703,9 @@ struct LowPair {
 };
 constexpr int kLowRows = 32;
 constexpr int kLowWaves = 8;
-constexpr int low_flight(int rank_blocks) { return rank_blocks <= 4 ? 4 : rank_blocks == 8 ? 2 : 1; }  // steps whose loads are under way
+// steps whose loads are under way, by the registers of two workgroups a CU (rank 120, 4096 rows of 4096: 25 us, with
+// one step 29)
+constexpr int low_flight(int rank_blocks) { return rank_blocks <= 4 ? 4 : rank_blocks == 8 ? 2 : 1; }
 
 // v as upper and lower part of the type; the lower is 0 beside an infinity or NaN
 template <class T>
@@ -847,7 +861,10 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
   }
 }
 
-// The large product: (U W) of BT places x BN columns, sum in steps of 128 bytes.
+// The large product: (U W) of BT places x BN columns, sum in steps of 128 bytes.  Bound by the matrix units at the
+// clock that the card holds under them, and by the waits at the barriers: 8192^3 in bf16 keeps them busy 64% of the
+// time at 1.75 to 1.85 GHz.  Against 8 waves of 128 x 64 on 256 x 256, 4 waves of 128 x 128 took 26% longer there,
+// 256 x 128 tiles alone 11%, and half steps with four or five tiles in LDS 3 to 6%.
 struct Big {
   const void *U, *W, *G;
   int64_t ldu, ldw;
@@ -1048,20 +1065,20 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     for (int q = 0; q < kLoads; ++q) load(std::true_type{}, k0 + st, st, q);
   unsigned wrong = 0;  // rows of this lane whose adapter does not exist
   {
-  // this lane's rows, and their adapters
-  int row[TT], mine[TT];
+    // this lane's rows, and their adapters
+    int row[TT], mine[TT];
 #pragma unroll
-  for (int t = 0; t < TT; ++t) row[t] = (int)row_at(a.order, min(t0 + wt + t * 32 + l32, a.rows.T - 1));
+    for (int t = 0; t < TT; ++t) row[t] = (int)row_at(a.order, min(t0 + wt + t * 32 + l32, a.rows.T - 1));
 #pragma unroll
-  for (int t = 0; t < TT; ++t) {
-    mine[t] = adapter_of(a.rows, row[t]);
-    if (t0 + wt + t * 32 + l32 >= a.rows.T) mine[t] = -1;
-    wrong |= (unsigned)(mine[t] < -1 || mine[t] >= a.rows.n) << t;
-  }
-    // The accumulators begin with s_i (U F_i) G_i, while the first tiles load (SPLIT: each part of the sum with some
-    // of the adapters and ranks).  U F_i comes as two values of the type
-    // (fp32: itself), so 8 ranks are one step; the loads of kSets steps are under way at a time.  A row without this adapter loads its own garbage, which reaches
-    // that row's accumulators alone, and these are set afterwards.
+    for (int t = 0; t < TT; ++t) {
+      mine[t] = adapter_of(a.rows, row[t]);
+      if (t0 + wt + t * 32 + l32 >= a.rows.T) mine[t] = -1;
+      wrong |= (unsigned)(mine[t] < -1 || mine[t] >= a.rows.n) << t;
+    }
+    // The accumulators begin with s_i (U F_i) G_i, while the first tiles load (SPLIT: each part of the sum with
+    // some of the adapters and ranks).  U F_i comes as two values of the type (fp32: itself), so 8 ranks are
+    // one step; the loads of kSets steps are under way at a time.  A row without this adapter loads its own
+    // garbage, which reaches that row's accumulators alone, and these are set afterwards.
     auto has = [&](int t) { return mine[t] >= 0 && mine[t] < a.rows.n; };
     auto place = [&](int t) { return (int64_t)min(t0 + wt + t * 32 + l32, a.rows.T - 1); };
     auto x_of = [&](int t, int b) {
@@ -1078,7 +1095,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
       if constexpr (std::is_same_v<T, _Float16>) f *= has(t) ? a.by[place(t)] : 0.f;
       return f;
     };
-    constexpr int kSets = TT * TN >= 8 ? 2 : TT * TN >= 4 ? 2 : 4;  // by the registers
+    constexpr int kSets = TT * TN >= 4 ? 2 : 4;  // by the registers
     const int shares = SPLIT ? a.splits : 1, share = SPLIT ? blockIdx.y : 0;
     uint64_t some[TT], any = 0;
     int first = -1;
@@ -1182,9 +1199,9 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   if constexpr (sizeof(T) == 4)
 #pragma unroll
     for (int m = 0; m < kMma; ++m) acc[m / TT][m % TT] += total[m / TT][m % TT];
-  // No load may land in LDS from here on.  Each wave turns its part of the tile there, in chunks of 16 bytes moved by the
-  // row's number, and writes whole rows of it: straight from the accumulators a store would reach 16 bytes
-  // of each of 32 rows.
+  // No load may land in LDS from here on.  Each wave turns its part of the tile there, in chunks of 16 bytes
+  // moved by the row's number, and writes whole rows of it: straight from the accumulators a store would reach 16
+  // bytes of each of 32 rows.
   __builtin_amdgcn_s_waitcnt(0x0070);
   __syncthreads();
   using Out = std::conditional_t<SPLIT, float, T>;
@@ -1231,11 +1248,12 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   }
 }
 
-// The factors' gradients: sum over the places of an adapter of U_t^T V_t, V = S or D, in pieces of `size` places
-// (32 to kGradRows: with few rows smaller ones, for enough workgroups, but not so small that the parts, a rank's 4
-// bytes a column each, outweigh U's).  A workgroup takes 64 kE columns of U, a wave 16 kE, whose rows it turns in registers.  V is turned on its
-// way to LDS, as upper and lower part of the type (fp16: brought to below 2^14 by the
-// piece's power of two).  Bound by reading U once: each wave keeps two steps' rows in flight.
+// The factors' gradients (4096 rows, 4096 + 4096 columns, rank 16, bf16: 20.6 us, U at 3.3 TB/s): sum over the
+// places of an adapter of U_t^T V_t, V = S or D, in pieces of `size` places (32 to kGradRows: with few rows smaller
+// ones, for enough workgroups, but not so small that the parts, a rank's 4 bytes a column each, outweigh U's).  A
+// workgroup takes 64 kE columns of U, a wave 16 kE, whose rows it turns in registers.  V is turned on its way to
+// LDS, as upper and lower part of the type (fp16: brought to below 2^14 by the piece's power of two).  Bound by
+// reading U once: each wave keeps two steps' rows in flight.
 constexpr int kGradRows = 128;
 struct Outer {
   const void* U;
@@ -1517,9 +1535,9 @@ int few_product(const Problem& p, const Rows& g, int r, Space& ws, hipStream_t s
   f.U = p.U, f.ldu = p.ldu, f.W = p.W, f.F = p.F, f.G = p.G, f.rows = g, f.C = p.C, f.N = p.N, f.r = r;
   f.blocks = (int)((p.N + 16 * M::kE - 1) / (16 * M::kE));
   const int steps = (p.C + M::kStep - 1) / M::kStep;
-  // workgroups: one a CU, as more cost the second launch what they save (32 rows of bf16 4096 x 4096: 16.2 us with 256,
-  // 17.8 with 512); two for fp32 in rows of N, where a wave has half as many loads under way (8 x 2048 x 7168: 22.5 us with
-  // 256, 17.9 with 512; with W along the sum 60 x 1000 x 2000 takes 14.8 and 17.4)
+  // workgroups: one a CU, as more cost the second launch what they save (32 rows of bf16 4096 x 4096: 16.2 us
+  // with 256, 17.8 with 512); two for fp32 in rows of N, where a wave has half as many loads under way (8 x 2048
+  // x 7168: 22.5 us with 256, 17.9 with 512; with W along the sum 60 x 1000 x 2000 takes 14.8 and 17.4)
   const int groups = sizeof(T) == 4 && !p.w_kc ? 512 : 256;
   f.splits = std::clamp(groups / f.blocks, 1, std::max(1, std::min(64, steps / 4)));
   f.low_splits = std::clamp(256 / g.T, 1, std::max(1, std::min(16, p.C / 256)));
@@ -1653,9 +1671,9 @@ struct Many {
     int bt, bn;
     Problem p;
   };
-  // The tile by what it is expected to take: the rounds of 256 workgroups, or of 512 where two fit a CU, each of a fixed
-  // part (a launch's share, the first loads, the low-rank part, the end) and the tiles' steps of 128 bytes
-  // along the sum, both as measured (us) with one workgroup a CU and with two.
+  // The tile by what it is expected to take: the rounds of 256 workgroups, or of 512 where two fit a CU, each of
+  // a fixed part (a launch's share, the first loads, the low-rank part, the end) and the tiles' steps of 128
+  // bytes along the sum, both as measured (us) with one workgroup a CU and with two.
   void choose(Plan& q, int nk) {
     struct Shape {
       int bt, bn;

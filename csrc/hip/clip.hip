@@ -10,7 +10,10 @@
 // atomics, the same bits every time.
 // Squares are summed in fp64: bf16 and fp32 values above 1.8e19 have squares
 // beyond fp32's range, and at 4 converted elements per clock and CU the fp64
-// units keep up with the memory.
+// units keep up with the memory.  The factor is rounded to fp32
+// (off by 2^-24 at most), the product once more to the tensor's type.
+// Measured: 290 tensors of together 1e9 bf16 values 1110 to 1170 us, 6 GB at 5.1 to 5.4 TB/s (a large copy: 4.95); 448
+// tensors of 29e6 fp32 values, outputs apart, 65 us on the GPU under 230 us of the caller's time to name them all.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -53,7 +56,8 @@ struct Pack {
 template <bool APART, class F>
 __device__ __forceinline__ void each_chunk(const Table<APART>& tb, F f) {
   const int all = tb.first[tb.count];
-  const int begin = (int)((int64_t)all * blockIdx.x / gridDim.x), end = (int)((int64_t)all * (blockIdx.x + 1) / gridDim.x);
+  const int begin = (int)((int64_t)all * blockIdx.x / gridDim.x);
+  const int end = (int)((int64_t)all * (blockIdx.x + 1) / gridDim.x);
   if (begin == end) return;
   int lo = 0, hi = tb.count - 1;  // the last tensor that begins at or before `begin`
   while (lo < hi) {

@@ -55,23 +55,23 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _check(X, W, A, B, index, scale):
+    # called for single tokens as well, so short of anything that takes a microsecond
     dtype = X.dtype
     if dtype not in TYPES:
         raise TypeError(f"adapter_matmul takes float32, bfloat16 and float16, not {dtype}")
     if not (W.dtype == A.dtype == B.dtype == dtype):
         raise TypeError("X, W, A and B must have one type")
-    dev = X.device
-    if dev.type != "cuda" or not (W.device == A.device == B.device == dev):
+    at = X.get_device()
+    if not X.is_cuda or not (W.get_device() == A.get_device() == B.get_device() == at):
         raise ValueError("adapter_matmul needs CUDA tensors on one device")
-    if X.dim() != 2 or W.dim() != 2 or A.dim() != 3 or B.dim() != 3:
+    dev = X.device
+    xs, ws, as_, bs = X.shape, W.shape, A.shape, B.shape
+    if len(xs) != 2 or len(ws) != 2 or len(as_) != 3 or len(bs) != 3:
         raise ValueError("X and W must be 2-D, A and B 3-D")
-    T, K = X.shape
-    N = W.shape[1]
-    n, _, r = A.shape
-    if W.shape[0] != K or A.shape[1] != K or tuple(B.shape) != (n, r, N):
-        raise ValueError(f"shape mismatch: X {tuple(X.shape)}, W {tuple(W.shape)}, A {tuple(A.shape)}, "
-                         f"B {tuple(B.shape)}")
-    if min(K, N, n, r) < 1:
+    (T, K), (KW, N), (n, KA, r) = xs, ws, as_
+    if KW != K or KA != K or bs != (n, r, N):
+        raise ValueError(f"shape mismatch: X {tuple(xs)}, W {tuple(ws)}, A {tuple(as_)}, B {tuple(bs)}")
+    if K < 1 or N < 1 or n < 1 or r < 1:
         raise ValueError("K, N, the rank and the number of adapters must be at least 1")
     if r > MAX_RANK:
         raise ValueError(f"rank {r} is above {MAX_RANK}")
@@ -80,12 +80,12 @@ def _check(X, W, A, B, index, scale):
             raise ValueError("index may be left out with one adapter only")
     elif index.dtype != torch.int32:
         raise TypeError("index must be int32")
-    elif index.shape != (T,) or index.device != dev:
+    elif index.shape != (T,) or index.get_device() != at:
         raise ValueError("index must have one entry per row of X, on its device")
     if isinstance(scale, torch.Tensor):
         if scale.dtype != torch.float32:
             raise TypeError("scale must be a number or float32")
-        if scale.shape != (n,) or scale.device != dev:
+        if scale.shape != (n,) or scale.get_device() != at:
             raise ValueError("scale must have one entry per adapter, on the device of X")
     if torch.is_grad_enabled() and (X.requires_grad or W.requires_grad or A.requires_grad or B.requires_grad):
         raise ValueError("adapter_matmul is not recorded by autograd: call it under torch.no_grad() and take the "
