@@ -499,6 +499,7 @@ struct Copy {
   int order;  // kRows, or in fragments
   bool straight;
   int first;                  // workgroups before this copy's
+  int tiles, per;             // of a matrix that is not straight, and of a workgroup
 };
 constexpr int kCopies = 6, kCopyTile = 64;
 struct Prepare {
@@ -607,13 +608,13 @@ __device__ __forceinline__ void copy_straight(const Copy& c, int part) {
 
 // One 64 x 64 tile of a copy, read along the source's memory and written along the destination's, 16 bytes a thread.
 template <class T>
-__device__ __forceinline__ void copy_tile(const Copy& c, int tile) {
+__device__ __forceinline__ void copy_tile(const Copy& c, int m, int tile) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
   constexpr int E = M::kE, kAcross = kCopyTile / E, kChunks = kCopyTile * kAcross;
   __shared__ T lds[kCopyTile][kCopyTile + 2];
-  const int across = (c.ld + kCopyTile - 1) / kCopyTile, down = (c.rows + kCopyTile - 1) / kCopyTile;
-  const int m = tile / (across * down), r0 = tile / across % down * kCopyTile, c0 = tile % across * kCopyTile;
+  const int across = (c.ld + kCopyTile - 1) / kCopyTile;
+  const int r0 = tile / across * kCopyTile, c0 = tile % across * kCopyTile;
   const T* src = (const T*)c.src.p + m * c.src.as;
   T* dst = (T*)c.dst + (int64_t)m * c.rows * c.ld;
   const bool along = c.src.cs == 1;
@@ -659,6 +660,36 @@ __device__ __forceinline__ void copy_tile(const Copy& c, int tile) {
   }
 }
 
+// A workgroup's tiles of one matrix.  With more than a few adapters those that no row has are left out, as resident
+// adapters may be many more than a batch uses (500 of rank 16, 7 of them in use, 4096 x 4096: 149 -> 29 us for this launch); beyond
+// kScanRows rows looking for that would cost more than a tile's copy.
+constexpr int kScanAdapters = 8, kScanRows = 8192;
+template <class T>
+__device__ __forceinline__ void copy_tiles(const Copy& c, int part, const Rows& rows) {
+  const int parts = (c.tiles + c.per - 1) / c.per, m = part / parts, first = part % parts * c.per;
+  if (c.count > kScanAdapters && rows.T <= kScanRows) {
+    constexpr int kLoads = kScanRows / (kPrepare * 4);  // all under way at once
+    Four<int> id[kLoads];
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+      const int t = (q * kPrepare + threadIdx.x) * 4;
+      id[q] = {{-1, -1, -1, -1}};
+      if (t + 4 <= rows.T) id[q] = *(const Four<int>*)(rows.index + t);
+    }
+    const int rest = rows.T / 4 * 4 + threadIdx.x;
+    bool used = rest < rows.T && rows.index[rest] == m;
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) used |= id[q].v[e] == m;
+    if (!__syncthreads_or(used)) return;
+  }
+  for (int tile = first; tile < min(c.tiles, first + c.per); ++tile) {
+    if (tile != first) __syncthreads();
+    copy_tile<T>(c, m, tile);
+  }
+}
+
 // The first launch: counters cleared, the order, the factors laid out for the matrix units, and
 // an operand whose rows do not begin at multiples of 16 bytes copied to where they do.  All parts run beside each
 // other: 6 us where there is little to copy, X and W of 4096 x 4095 in bf16 26 us (5.1 TB/s).  Read in place by
@@ -673,7 +704,7 @@ __global__ __launch_bounds__(kPrepare) void prepare_kernel(Prepare p) {
   int k = p.copies - 1;
   while (k > 0 && b < p.copy[k].first) --k;
   if (p.copy[k].straight) copy_straight<T>(p.copy[k], b - p.copy[k].first);
-  else copy_tile<T>(p.copy[k], b - p.copy[k].first);
+  else copy_tiles<T>(p.copy[k], b - p.copy[k].first, p.rows);
 }
 
 // low (place, rank) = U F_i, 32 places of one adapter by a workgroup, whose 8 waves cut the sum (16 waves were no
@@ -1597,10 +1628,12 @@ struct Many {
   }
   T* copy(View src, int rows, int have, int cols, int ld, int count, int order = kRows) {
     Copy& c = prep.copy[prep.copies++];
+    const int64_t tiles = (int64_t)((rows + kCopyTile - 1) / kCopyTile) * ((ld + kCopyTile - 1) / kCopyTile);
+    const int64_t per = std::clamp<int64_t>(count * tiles / 4096, 1, tiles);  // tiles of a workgroup: 16 of them a CU
     c = {src, ws.template take<T>((int64_t)count * rows * ld), rows, cols, ld, count, have, order,
-         order == kRows && src.cs == 1, (int)groups - prep.order_groups};
+         order == kRows && src.cs == 1, (int)groups - prep.order_groups, (int)tiles, (int)per};
     groups += c.straight ? ((int64_t)count * rows * (ld / E) + kStraight - 1) / kStraight
-                         : (int64_t)count * ((rows + kCopyTile - 1) / kCopyTile) * ((ld + kCopyTile - 1) / kCopyTile);
+                         : count * ((tiles + per - 1) / per);
     ws.launch(groups, kPrepare);
     return (T*)c.dst;
   }

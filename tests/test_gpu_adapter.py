@@ -429,6 +429,48 @@ def test_other_stream(gelim, cuda):
         assert torch.equal(v, want)
 
 
+@pytest.mark.parametrize("seed", range(60))
+def test_any_sizes_and_places(gelim, cuda, seed):
+    """Sizes, layouts and wanted gradients as they come; operands between NaN, or at an address of their type's size only."""
+    import math
+    import random
+
+    rng = random.Random(seed)
+
+    def size(most, step=1):
+        return max(1, int(round(math.exp(rng.uniform(0.0, math.log(most))))) // step * step)
+
+    def put(v):
+        v, how = v.contiguous(), rng.randrange(3)
+        if how == 1:
+            first = rng.choice([1, 2, 3, 4, 8])
+            return torch.cat([v.new_zeros(first), v.reshape(-1)])[first:].view(v.shape)
+        if how == 2:
+            more = rng.choice([1, 4, 8, 13])
+            at = rng.randint(0, more)
+            room = v.new_full((*v.shape[:-2], v.shape[-2] + 2, v.shape[-1] + more), float("nan"))
+            room[..., 1:1 + v.shape[-2], at:at + v.shape[-1]] = v
+            return room[..., 1:1 + v.shape[-2], at:at + v.shape[-1]]
+        return v
+
+    dtype, layout = rng.choice(DTYPES), rng.choice(["kn", "nk"])
+    step = rng.choice([1, 8, 64])
+    T, K, N, n = size(3000), size(2000, step), size(2000, step), size(40)
+    r = rng.choice([1, 2, 7, 8, 16, 17, 33, 64, 100, 129, 256])
+    X, W, A, B, index, scale = make(cuda, T, K, N, r, n, dtype, layout, rng.choice(["mixed", "runs", "none", "all"]), seed)
+    W, A, B = (put(v) if layout == "kn" else put(v.transpose(-1, -2)).transpose(-1, -2) for v in (W, A, B))
+    args = (put(X), W, A, B, index, scale)
+    out = put(X.new_zeros(T, N))
+    gelim.ops.adapter_matmul(*args, out=out)
+    check(out, *ref_product(*args, device=cuda))
+    dY = put(torch.randn(T, N, generator=torch.Generator().manual_seed(seed)).to(dtype).to(cuda))
+    need = rng.choice([(True, True, True), (True, False, False), (False, True, False), (False, False, True)])
+    for v, t, wanted in zip(gelim.ops.adapter_matmul_grad(dY, *args, need=need), ref_grad(dY, *args, device=cuda), need):
+        assert (v is not None) == wanted
+        if wanted:
+            check(v, *t)
+
+
 def test_two_at_a_time(gelim, cuda):
     """Calls and replays on two streams, from two threads: sums cut over workgroups that wait for each other's parts."""
     from threading import Thread
@@ -517,6 +559,23 @@ def test_more_adapters_than_rows(gelim, cuda):
         dY = torch.randn(T, 64, device=cuda).half()
         for v, t in zip(gelim.ops.adapter_matmul_grad(dY, *args), ref_grad(dY, *args)):
             check(v, *t)
+
+
+@pytest.mark.parametrize("T", [66, 257, 5000, 9000])
+def test_many_resident_adapters_of_which_few_are_used(gelim, cuda, T):
+    """What the adapters that no row has hold does not matter, and their gradients are zeros."""
+    X, W, A, B, index, scale = make(cuda, T, 136, 72, 12, 30, torch.bfloat16)
+    index = torch.where(index % 7 == 3, index, -1)
+    index[T - 1] = 29
+    unused = torch.ones(30, dtype=torch.bool, device=cuda)
+    unused[index[index >= 0].long()] = False
+    ref = ref_product(X, W, A, B, index, scale)
+    dY = torch.randn(T, 72, generator=torch.Generator().manual_seed(T)).bfloat16().to(cuda)
+    grads = ref_grad(dY, X, W, A, B, index, scale)
+    A[unused], B[unused] = float("nan"), float("inf")
+    check(gelim.ops.adapter_matmul(X, W, A, B, index, scale), *ref)
+    for v, t in zip(gelim.ops.adapter_matmul_grad(dY, X, W, A, B, index, scale), grads):
+        check(v, *t)
 
 
 def test_refusals(gelim, cuda):
