@@ -75,20 +75,28 @@ struct Mma<float> {
   }
 };
 
-// The same over 32 rows and columns: lane l has row (column) l % 32 and, of a step of 2 kE values along the
-// sum, those from (l / 32) kE on.  In D it has column l % 32 and the rows 8 (r / 4) + 4 (l / 32) + r % 4.
-typedef float f16 __attribute__((ext_vector_type(16)));
-__device__ __forceinline__ f16 mma32(bf8 a, bf8 b, f16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f16 mma32(h8 a, h8 b, f16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f16 mma32(f4 a, f4 b, f16 c) {
+// The blocks of the large product: kB rows and columns; lane l has row (column) l % kB and, of a step along the sum, the
+// kE values from (l / kB) kE on.  16-bit types as above: 32 x 32 x 16 instructions alone, from registers, reach 1670
+// TFLOP/s at the clock that the card holds under them, 16 x 16 x 32 1830.
+template <class T>
+struct Block {
+  static constexpr int kB = 16;
+  using Acc = f4;
+  static __device__ __forceinline__ f4 mma(typename Mma<T>::Frag a, typename Mma<T>::Frag b, f4 c) {
+    return Mma<T>::mma(a, b, c);
+  }
+};
+// fp32: in D lane l has column l % 32 and the rows 8 (r / 4) + 4 (l / 32) + r % 4
+template <>
+struct Block<float> {
+  static constexpr int kB = 32;
+  typedef float Acc __attribute__((ext_vector_type(16)));
+  static __device__ __forceinline__ Acc mma(f4 a, f4 b, Acc c) {
 #pragma unroll
-  for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], c, 0, 0, 0);
-  return c;
-}
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], c, 0, 0, 0);
+    return c;
+  }
+};
 
 template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) Four {
@@ -661,8 +669,8 @@ __device__ __forceinline__ void copy_tile(const Copy& c, int m, int tile) {
 }
 
 // A workgroup's tiles of one matrix.  With more than a few adapters those that no row has are left out, as resident
-// adapters may be many more than a batch uses (500 of rank 16, 7 of them in use, 4096 x 4096: 149 -> 29 us for this launch); beyond
-// kScanRows rows looking for that would cost more than a tile's copy.
+// adapters may be many more than a batch uses (500 of rank 16, 7 of them in use, 4096 x 4096: 149 -> 29 us for this
+// launch); beyond kScanRows rows looking for that would cost more than a tile's copy.
 constexpr int kScanAdapters = 8, kScanRows = 8192;
 template <class T>
 __device__ __forceinline__ void copy_tiles(const Copy& c, int part, const Rows& rows) {
@@ -943,7 +951,9 @@ template <class T, bool W_KC, int BT, int BN, int WT, int WN, int S, bool SPLIT>
 __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   using Frag = typename Mma<T>::Frag;
   constexpr int E = Mma<T>::kE, BK = 8 * E;
-  constexpr int TT = BT / WT / 32, TN = BN / WN / 32;
+  using Acc = typename Block<T>::Acc;
+  constexpr int kB = Block<T>::kB, kLanes = 64 / kB, kParts = 8 / kLanes, kAcc = kB * kB / 64;
+  constexpr int TT = BT / WT / kB, TN = BN / WN / kB;
   constexpr int kLoadU = BT / (WT * WN * 8), kLoadW = BN / (WT * WN * 8);
   constexpr int kRowChunks = BN / E;  // chunks in a row of W's tile if not W_KC
   __shared__ __attribute__((aligned(16))) T lds[S * (BT + BN) * BK];  // U's tiles, then W's
@@ -957,7 +967,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   const int band = number / (kGroup * a.tiles_n), in_band = number % (kGroup * a.tiles_n);
   const int high = min(kGroup, a.tiles_t - band * kGroup);
   const int t0 = (band * kGroup + in_band % high) * BT, n0 = in_band / high * BN;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l32 = lane % 32, half = lane / 32;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, lb = lane % kB, g = lane / kB;
   const int wt = wave / WN * (BT / WT), wn = wave % WN * (BN / WN);
 
   const int nk = (max(a.cu, a.cw) + BK - 1) / BK;
@@ -1013,82 +1023,88 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     to_lds(from, __builtin_amdgcn_readfirstlane(to));
   };
 
-  f16 acc[TN][TT] = {}, total[sizeof(T) == 4 ? TN : 1][TT] = {};
-  struct Frags {
-    Frag x[TT], w[TN];
-  };
-  // Where this lane's fragments begin in a tile.  A quarter moves the chunk's number by an exclusive or, which the
-  // swap above leaves alone, or the row; the rest are constant distances.
-  const int u_at = (wt + l32) * BK + (half ^ (l32 >> 1 & 7)) * E;
+  Acc acc[TN][TT] = {}, total[sizeof(T) == 4 ? TN : 1][TT] = {};
+  // Where this lane's fragments begin in a tile.  A step along the sum (of kParts) moves the chunk's number by an
+  // exclusive or, which the swap above leaves alone, or the row; the rest are constant distances.
+  const int u_at = (wt + lb) * BK + (g ^ (lb >> 1 & 7)) * E;
   int w_at[W_KC ? 1 : TN];
   if constexpr (W_KC) {
-    w_at[0] = (wn + l32) * BK + (half ^ (l32 >> 1 & 7)) * E;
+    w_at[0] = (wn + lb) * BK + (g ^ (lb >> 1 & 7)) * E;
   } else {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int n = wn + j * 32 + (sizeof(T) == 2 ? l32 / 16 * 16 + lane % 4 * 4 : l32);
-      const int k = sizeof(T) == 2 ? half * 8 + lane % 16 / 4 : half * 4;
+      const int n = wn + j * kB + (sizeof(T) == 2 ? lane % 4 * 4 : lb);
+      const int k = sizeof(T) == 2 ? g * 8 + lane % 16 / 4 : g * 4;
       w_at[j] = k * BN + ((n / E) ^ swap_columns<T, kRowChunks>(k)) * E + n % E;
     }
   }
-  // the q-th fragment of a quarter
-  auto read = [&](int stage, int part, Frags& f, int q) {
-    const int us = stage * BT * BK, ws = (S * BT + stage * BN) * BK;
-    if (q < TT) {
-      f.x[q] = *(const Frag*)&lds[us + (u_at ^ (part * 2 * E)) + q * 32 * BK];
-      return;
-    }
-    const int j = q - TT;
+  auto read_x = [&](int stage, int part, int t) {
+    return *(const Frag*)&lds[stage * BT * BK + (u_at ^ (part * kLanes * E)) + t * kB * BK];
+  };
+  auto read_w = [&](int stage, int part, int j) {
+    const int ws = (S * BT + stage * BN) * BK;
     if constexpr (W_KC) {
-      f.w[j] = *(const Frag*)&lds[ws + (w_at[0] ^ (part * 2 * E)) + j * 32 * BK];
+      return *(const Frag*)&lds[ws + (w_at[0] ^ (part * kLanes * E)) + j * kB * BK];
     } else if constexpr (sizeof(T) == 2) {
       // 16 lanes read 4 rows (of the sum) x 16 columns, 8 bytes each, and get their column's 4 values
       s8 v;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s4*)&lds[ws + w_at[j] + (part * 16 + h * 4) * BN]);
+            (__attribute__((address_space(3))) s4*)&lds[ws + w_at[j] + (part * kLanes * E + h * 4) * BN]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[h * 4 + e] = r[e];
       }
-      f.w[j] = __builtin_bit_cast(Frag, v);
+      return __builtin_bit_cast(Frag, v);
     } else {
+      Frag v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f.w[j][e] = lds[ws + w_at[j] + (part * 8 + e) * BN];
+      for (int e = 0; e < 4; ++e) v[e] = lds[ws + w_at[j] + (part * kLanes * E + e) * BN];
+      return v;
     }
   };
-  // A quarter: `now` is multiplied; in between, in this order, quarter `part` is read into `next` in the first
-  // half and, with kLoads, a tile is loaded.
-  constexpr int kMma = TT * TN, kReads = TT + TN, kLoads = kLoadU + kLoadW;
-  auto quarter = [&](const Frags& now, int stage, int part, Frags& next, auto loads, auto guard, int kt, int to) {
+  // A step along the sum in one or two halves of the wave's rows, x[0] and x[1] in turn.  While one half is multiplied
+  // the next is read; with the last half of a step each fragment of W is read for the next step right after its last
+  // use (one half: into the other of two sets), so that it has as long to arrive.
+  constexpr int kMma = TT * TN, kLoads = kLoadU + kLoadW;
+  constexpr int TH = TT > 1 ? TT / 2 : 1, kHalves = TT / TH, kSetsW = kHalves == 1 ? 2 : 1, kSubs = kParts * kHalves;
+  Frag x[2][TH], w[kSetsW][TN];
+  // the sub-th half of a tile's; then, in this order, what follows is read, and with `loads` a tile is loaded
+  auto half = [&](int sub, int stage, auto loads, auto guard, int kt, int to) {
+    const int h = sub % kHalves, next = (sub + 1) % kSubs, part = next / kHalves;
+    const int set = sub / kHalves % kSetsW, set_next = part % kSetsW;
 #pragma unroll
-    for (int m = 0; m < kMma; ++m) {
-      constexpr int kSpan = (kMma + 1) / 2;
+    for (int m = 0; m < TN * TH; ++m) {
+      constexpr int kAll = TN * TH, kSpan = (kAll + 1) / 2;
+      const int j = m / TH, i = m % TH;
 #pragma unroll
-      for (int q = 0; q < kReads; ++q)
-        if (q * kSpan / kReads == m) read(stage, part, next, q);
+      for (int q = 0; q < TH; ++q)
+        if (q * kSpan / TH == m) x[(sub + 1) % 2][q] = read_x(stage, part, next % kHalves * TH + q);
+      if (kSetsW == 2)
+#pragma unroll
+        for (int q = 0; q < TN; ++q)
+          if (q * kSpan / TN == m) w[set_next][q] = read_w(stage, part, q);
       if constexpr (decltype(loads)::value)
 #pragma unroll
         for (int q = 0; q < kLoads; ++q)
-          if (q * kMma / kLoads == m) load(guard, kt, to, q);
-      acc[m / TT][m % TT] = mma32(now.w[m / TT], now.x[m % TT], acc[m / TT][m % TT]);
+          if (q * kAll / kLoads == m) load(guard, kt, to, q);
+      acc[j][h * TH + i] = Block<T>::mma(w[set][j], x[sub % 2][i], acc[j][h * TH + i]);
+      if (kSetsW == 1 && h == kHalves - 1 && i == TH - 1) w[0][j] = read_w(stage, part, j);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  Frags f0, f1;
-  // one tile from its place in LDS; its first quarter is in f0, and the next tile's will be
+  // one tile from its place in LDS; its first half and W are in registers, and the next tile's will be
   auto step = [&](auto guard, int kt, int stage) {
     constexpr std::false_type no{};
-    quarter(f0, stage, 1, f1, no, no, 0, 0);
-    quarter(f1, stage, 2, f0, no, no, 0, 0);
-    quarter(f0, stage, 3, f1, no, no, 0, 0);
+#pragma unroll
+    for (int sub = 0; sub < kSubs - 1; ++sub) half(sub, stage, no, no, 0, 0);
     // this wave's loads of the next tile have landed (only S - 2 tiles' may be under way) and its reads are done,
     // then everybody's
     constexpr int kAway = (S - 2) * kLoads;
     static_assert(kAway < 64, "vmcnt");
     __builtin_amdgcn_s_waitcnt(0x0070 | (kAway & 15) | (kAway >> 4) << 14);
     __syncthreads();
-    quarter(f1, (stage + 1) % S, 0, f0, std::true_type{}, guard, kt + S, stage);
+    half(kSubs - 1, (stage + 1) % S, std::true_type{}, guard, kt + S, stage);
   };
 #pragma unroll
   for (int st = 0; st < S; ++st)
@@ -1099,11 +1115,11 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     // this lane's rows, and their adapters
     int row[TT], mine[TT];
 #pragma unroll
-    for (int t = 0; t < TT; ++t) row[t] = (int)row_at(a.order, min(t0 + wt + t * 32 + l32, a.rows.T - 1));
+    for (int t = 0; t < TT; ++t) row[t] = (int)row_at(a.order, min(t0 + wt + t * kB + lb, a.rows.T - 1));
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       mine[t] = adapter_of(a.rows, row[t]);
-      if (t0 + wt + t * 32 + l32 >= a.rows.T) mine[t] = -1;
+      if (t0 + wt + t * kB + lb >= a.rows.T) mine[t] = -1;
       wrong |= (unsigned)(mine[t] < -1 || mine[t] >= a.rows.n) << t;
     }
     // The accumulators begin with s_i (U F_i) G_i, while the first tiles load (SPLIT: each part of the sum with
@@ -1111,22 +1127,30 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     // one step; the loads of kSets steps are under way at a time.  A row without this adapter loads its own
     // garbage, which reaches that row's accumulators alone, and these are set afterwards.
     auto has = [&](int t) { return mine[t] >= 0 && mine[t] < a.rows.n; };
-    auto place = [&](int t) { return (int64_t)min(t0 + wt + t * 32 + l32, a.rows.T - 1); };
+    auto place = [&](int t) { return (int64_t)min(t0 + wt + t * kB + lb, a.rows.T - 1); };
+    // the fragments that the low-rank pass and the first launch wrote, of 32 places or columns and 8 ranks; with 16-bit
+    // types the lanes' four groups take the upper and the lower parts of two such blocks
+    constexpr int kRanks = sizeof(T) == 2 ? 16 : 8;  // of an instruction
     auto x_of = [&](int t, int b) {
-      const int64_t block = min((t0 + wt) / 32 + t, (a.rows.T - 1) / 32);
-      return ((const Frag*)a.split)[(block * (a.rp / 8) + b / 8) * 64 + lane];
+      const int at = t0 + wt + t * kB;
+      const int64_t block = min(at / 32, (a.rows.T - 1) / 32);
+      if constexpr (sizeof(T) == 2)
+        return ((const Frag*)a.split)[(block * (a.rp / 8) + b / 8 + g % 2) * 64 + g / 2 * 32 + at % 32 + lb];
+      else return ((const Frag*)a.split)[(block * (a.rp / 8) + b / 8) * 64 + lane];
     };
-    constexpr int kG = 32 * 8 / E;  // fragments' chunks of 8 ranks and 32 columns: 16-bit types' halves share them
     auto w_of = [&](int cur, int j, int b) {
-      const int64_t blocks = (a.N + 31) / 32, block = min((int64_t)(n0 + wn) / 32 + j, blocks - 1);
-      return ((const Frag*)a.G)[((cur * blocks + block) * (a.rp / 8) + b / 8) * kG + lane % kG];
+      const int n = n0 + wn + j * kB;
+      const int64_t blocks = (a.N + 31) / 32, block = min((int64_t)n / 32, blocks - 1);
+      const int64_t at = (cur * blocks + block) * (a.rp / 8) + b / 8;
+      if constexpr (sizeof(T) == 2) return ((const Frag*)a.G)[(at + g % 2) * 32 + n % 32 + lb];
+      else return ((const Frag*)a.G)[at * 64 + lane];
     };
     auto factor = [&](int t, int cur) {
       float f = scale_of(a.rows, cur);
       if constexpr (std::is_same_v<T, _Float16>) f *= has(t) ? a.by[place(t)] : 0.f;
       return f;
     };
-    constexpr int kSets = TT * TN >= 4 ? 2 : 4;  // by the registers
+    constexpr int kSets = (sizeof(T) == 2 ? 1 : 2) * (TT * TN * kB * kB <= 1024 ? 2 : 1);  // by the registers
     const int shares = SPLIT ? a.splits : 1, share = SPLIT ? blockIdx.y : 0;
     uint64_t some[TT], any = 0;
     int first = -1;
@@ -1150,16 +1174,16 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
         for (int j = 0; j < TN; ++j) w[q][j] = w_of(first, j, b);
       };
 #pragma unroll
-      for (int q = 0; q < kSets; ++q) fetch(q, (share + q * shares) * 8);
-      for (int b = share * 8; b < a.r; b += kSets * shares * 8)
+      for (int q = 0; q < kSets; ++q) fetch(q, (share + q * shares) * kRanks);
+      for (int b = share * kRanks; b < a.r; b += kSets * shares * kRanks)
 #pragma unroll
         for (int q = 0; q < kSets; ++q) {
-          if (b + q * shares * 8 < a.r)
+          if (b + q * shares * kRanks < a.r)
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
-              for (int t = 0; t < TT; ++t) acc[j][t] = mma32(w[q][j], x[q][t], acc[j][t]);
-          fetch(q, b + (kSets + q) * shares * 8);
+              for (int t = 0; t < TT; ++t) acc[j][t] = Block<T>::mma(w[q][j], x[q][t], acc[j][t]);
+          fetch(q, b + (kSets + q) * shares * kRanks);
         }
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
@@ -1167,7 +1191,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[j][t][r] = has(t) ? f * acc[j][t][r] : 0.f;
+          for (int r = 0; r < kAcc; ++r) acc[j][t][r] = has(t) ? f * acc[j][t][r] : 0.f;
       }
     } else if (any) {
       // for each adapter among 32 rows the product of all of them, kept where it is theirs
@@ -1178,22 +1202,22 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
         while (left) {
           const int cur = __builtin_amdgcn_readlane(mine[t], __builtin_ctzll(left));
           left &= ~__ballot(mine[t] == cur);
-          f16 d[TN] = {};
-          for (int b = 0; b < a.r; b += 8 * kSets) {
+          Acc d[TN] = {};
+          for (int b = 0; b < a.r; b += kRanks * kSets) {
             if (SPLIT && unit++ % shares != 0) continue;
             Frag x[kSets], w[TN][kSets];
 #pragma unroll
             for (int q = 0; q < kSets; ++q) {
-              if (b + q * 8 >= a.r) continue;
-              x[q] = x_of(t, b + q * 8);
+              if (b + q * kRanks >= a.r) continue;
+              x[q] = x_of(t, b + q * kRanks);
 #pragma unroll
-              for (int j = 0; j < TN; ++j) w[j][q] = w_of(cur, j, b + q * 8);
+              for (int j = 0; j < TN; ++j) w[j][q] = w_of(cur, j, b + q * kRanks);
             }
 #pragma unroll
             for (int q = 0; q < kSets; ++q)
-              if (b + q * 8 < a.r)
+              if (b + q * kRanks < a.r)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) d[j] = mma32(w[j][q], x[q], d[j]);
+                for (int j = 0; j < TN; ++j) d[j] = Block<T>::mma(w[j][q], x[q], d[j]);
           }
           const float f = factor(t, cur);
           if (mine[t] == cur)
@@ -1206,7 +1230,9 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   __builtin_amdgcn_s_waitcnt(0x0070);
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < kReads; ++q) read(0, 0, f0, q);
+  for (int q = 0; q < TH; ++q) x[0][q] = read_x(0, 0, q);
+#pragma unroll
+  for (int q = 0; q < TN; ++q) w[0][q] = read_w(0, 0, q);
   const int whole = min(k1, min(a.cu, a.cw) / BK);  // tiles without a part behind the end
   int kt = k0;
   for (; kt + 2 * S - 1 < whole; kt += S) {
@@ -1219,7 +1245,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
 #pragma unroll
         for (int m = 0; m < kMma; ++m) {
           total[m / TT][m % TT] += acc[m / TT][m % TT];
-          acc[m / TT][m % TT] = f16{};
+          acc[m / TT][m % TT] = Acc{};
         }
     }
   }
@@ -1241,14 +1267,14 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   Out* mem = (Out*)lds + wave * kHigh * kRowOut * EO;
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
-    const int i = t * 32 + l32;
+    const int i = t * kB + lb;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      f16 v = acc[j][t];
+      Acc v = acc[j][t];
       if (!SPLIT && (wrong >> t & 1)) v = v * __builtin_nanf("");
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int n = j * 32 + r * 2 + half * 4;
+      for (int r = 0; r < kAcc; r += 4) {
+        const int n = j * kB + r * 2 + g * 4;
         *(Four<Out>*)(mem + (i * kRowOut + ((n / EO) ^ (i % kRowOut))) * EO + n % EO) =
             Four<Out>{(Out)v[r], (Out)v[r + 1], (Out)v[r + 2], (Out)v[r + 3]};
       }
