@@ -16,7 +16,7 @@
 // tile of the large product has few adapters; the factors are laid out for the
 // matrix units once per call; U F_i is one pass over U; the accumulators of the
 // large product begin with s_i (U F_i) G_i.  8192 rows, bf16 8192 x 8192, rank 64:
-// 9 + 60 + 880 us, the large product at 1.25 PFLOP/s (a plain library product of
+// 9 + 60 + 870 us, the large product at 1.26 PFLOP/s (a plain library product of
 // that size: 1.27 to 1.56 by its layout).
 #include <hip/hip_runtime.h>
 
@@ -901,9 +901,10 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
 }
 
 // The large product: (U W) of BT places x BN columns, sum in steps of 128 bytes.  Bound by the matrix units at the
-// clock that the card holds under them, and by the waits at the barriers: 8192^3 in bf16 keeps them busy 64% of the
-// time at 1.75 to 1.85 GHz.  Against 8 waves of 128 x 64 on 256 x 256, 4 waves of 128 x 128 took 26% longer there,
-// 256 x 128 tiles alone 11%, and half steps with four or five tiles in LDS 3 to 6%.
+// clock that the card holds under them, 1.6 to 1.85 GHz, and by the waits at the barriers (8192^3 in bf16: 73% of the
+// cycles busy), so by what a product costs in power as well: 16 x 16 x 32 instructions instead of 32 x 32 x 16 took 876
+// instead of 909 us there.  Against 8 waves of 128 x 64 on 256 x 256, 4 waves of 128 x 128 took 26% longer, 256 x 128
+// tiles alone 11%, and half steps with four or five tiles in LDS 3 to 6%.
 struct Big {
   const void *U, *W, *G;
   int64_t ldu, ldw;
@@ -1738,7 +1739,7 @@ struct Many {
       int bt, bn;
       double fixed, step, fixed2, step2;  // step2 0: one fits
     };
-    static constexpr Shape k16[] = {{256, 256, 16.7, 1.61, 0, 0}, {256, 128, 11.9, 0.90, 0, 0},
+    static constexpr Shape k16[] = {{256, 256, 16.7, 1.55, 0, 0}, {256, 128, 11.9, 0.84, 0, 0},
                                     {128, 128, 9.4, 0.50, 0, 0}, {64, 64, 5.6, 0.26, 5.2, 0.39}};
     static constexpr Shape k32[] = {{128, 128, 12.3, 2.26, 0, 0}, {128, 64, 9.7, 1.17, 10.0, 2.37},
                                     {64, 64, 6.5, 0.65, 6.0, 1.30}};
