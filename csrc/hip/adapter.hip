@@ -1026,33 +1026,33 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
 
   Acc acc[TN][TT] = {}, total[sizeof(T) == 4 ? TN : 1][TT] = {};
   // Where this lane's fragments begin in a tile.  A step along the sum (of kParts) moves the chunk's number by an
-  // exclusive or, which the swap above leaves alone, or the row; the rest are constant distances.
+  // exclusive or, which the swap above leaves alone, or the row; a block of W's columns moves their number in the same
+  // way, as a wave's columns begin at a multiple of their number; the rest are constant distances.
   const int u_at = (wt + lb) * BK + (g ^ (lb >> 1 & 7)) * E;
-  int w_at[W_KC ? 1 : TN];
+  int w_at;  // of the wave's first block
   if constexpr (W_KC) {
-    w_at[0] = (wn + lb) * BK + (g ^ (lb >> 1 & 7)) * E;
+    w_at = (wn + lb) * BK + (g ^ (lb >> 1 & 7)) * E;
   } else {
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = wn + j * kB + (sizeof(T) == 2 ? lane % 4 * 4 : lb);
-      const int k = sizeof(T) == 2 ? g * 8 + lane % 16 / 4 : g * 4;
-      w_at[j] = k * BN + ((n / E) ^ swap_columns<T, kRowChunks>(k)) * E + n % E;
-    }
+    const int n = wn + (sizeof(T) == 2 ? lane % 4 * 4 : lb);
+    const int k = sizeof(T) == 2 ? g * 8 + lane % 16 / 4 : g * 4;
+    w_at = k * BN + ((n / E) ^ swap_columns<T, kRowChunks>(k)) * E + n % E;
   }
+  w_at += S * BT * BK;
+  asm("" : "+v"(w_at));  // one number: from U's first tile on, W's are too far away for an instruction's offset
   auto read_x = [&](int stage, int part, int t) {
     return *(const Frag*)&lds[stage * BT * BK + (u_at ^ (part * kLanes * E)) + t * kB * BK];
   };
   auto read_w = [&](int stage, int part, int j) {
-    const int ws = (S * BT + stage * BN) * BK;
+    const int ws = stage * BN * BK;
     if constexpr (W_KC) {
-      return *(const Frag*)&lds[ws + (w_at[0] ^ (part * kLanes * E)) + j * kB * BK];
+      return *(const Frag*)&lds[ws + (w_at ^ (part * kLanes * E)) + j * kB * BK];
     } else if constexpr (sizeof(T) == 2) {
       // 16 lanes read 4 rows (of the sum) x 16 columns, 8 bytes each, and get their column's 4 values
       s8 v;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s4*)&lds[ws + w_at[j] + (part * kLanes * E + h * 4) * BN]);
+            (__attribute__((address_space(3))) s4*)&lds[ws + (w_at ^ (j * kB)) + (part * kLanes * E + h * 4) * BN]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[h * 4 + e] = r[e];
       }
@@ -1060,7 +1060,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     } else {
       Frag v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = lds[ws + w_at[j] + (part * kLanes * E + e) * BN];
+      for (int e = 0; e < 4; ++e) v[e] = lds[ws + (w_at ^ (j * kB)) + (part * kLanes * E + e) * BN];
       return v;
     }
   };
