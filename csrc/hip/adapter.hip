@@ -75,8 +75,8 @@ struct Mma<float> {
   }
 };
 
-// The blocks of the large product: kB rows and columns; lane l has row (column) l % kB and, of a step along the sum, the
-// kE values from (l / kB) kE on.  16-bit types as above: 32 x 32 x 16 instructions alone, from registers, reach 1670
+// The blocks of the large product: kB rows and columns; lane l has row (column) l % kB and, of a step along the sum,
+// the kE values from (l / kB) kE on.  16-bit types as above: 32 x 32 x 16 instructions alone, from registers, reach 1670
 // TFLOP/s at the clock that the card holds under them, 16 x 16 x 32 1830.
 template <class T>
 struct Block {
