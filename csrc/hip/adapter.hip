@@ -722,9 +722,9 @@ __global__ __launch_bounds__(kPrepare) void prepare_kernel(Prepare p) {
 // adds their parts, always in the same order. Measured, bf16: 2048 x 4096, rank 16, 8.8 us; 8192 x 8192, rank 64,
 // 60 us (U at 2.2 TB/s; more loads under way, waves side by side along a row, or the pieces of an adapter on one
 // XCD changed that by less than the noise). Also in fragments of 32 places and 8 ranks for the matrix units of the
-// large product, with 16-bit types as the sum of two values of the type, the upper parts for the lower half of the
-// lanes.  One value's rounding alone would be as large as the result's.  fp16: a row is first brought to below 2^14
-// by a power of two (`by`), as it may be beyond the type's range.
+// large product, with 16-bit types as the sum of three values of the type, which hold all 24 bits of the fp32 sum.  fp16:
+// a row is first brought to below 2^14 by a power of two (`by`), as it may be beyond the type's range; small values of the
+// row are off by 2^-38 of its largest at most.
 struct Low {
   const void *U, *F;
   int64_t ldu;
@@ -746,11 +746,17 @@ constexpr int kLowWaves = 8;
 // one step 29)
 constexpr int low_flight(int rank_blocks) { return rank_blocks <= 4 ? 4 : rank_blocks == 8 ? 2 : 1; }
 
-// v as upper and lower part of the type; the lower is 0 beside an infinity or NaN
+// v as the sum of kTerms values of the type, each the rounding of what the ones before leave (a difference without a
+// rounding of its own); the lower ones are 0 beside an infinity or NaN
 template <class T>
-__device__ __forceinline__ void two_parts(float v, T& hi, T& lo) {
-  hi = (T)v;
-  lo = fabsf((float)hi) <= 3.4e38f ? (T)(v - (float)hi) : (T)0.f;
+constexpr int kTerms = sizeof(T) == 2 ? 3 : 1;
+template <class T>
+__device__ __forceinline__ void terms(float v, T (&out)[kTerms<T>]) {
+#pragma unroll
+  for (int h = 0; h < kTerms<T>; ++h) {
+    out[h] = (T)v;
+    v = fabsf((float)out[h]) <= 3.4e38f ? v - (float)out[h] : 0.f;
+  }
 }
 // a power of two that brings fp16's `most` to [2^13, 2^14)
 __device__ __forceinline__ int to_fp16_range(float most) {
@@ -885,14 +891,19 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
 #pragma unroll
     for (int j = 0; j < RB; ++j) {
       *(f4*)(a.low + at * rp + j * 16 + g * 4) = acc[j][t];
-      // in fragments of 8 ranks (j * 2 + g / 2) and 32 places: two halves of 32 lanes
-      T* out = (T*)a.split + ((at / 32 * (rp / 8) + j * 2 + g / 2) * 64 + at % 32) * E;
+      // in fragments of 8 ranks (j * 2 + g / 2) and 32 places: 32 lanes for each term, fp32 two halves of the ranks
+      T* out = (T*)a.split + ((at / 32 * (rp / 8) + j * 2 + g / 2) * (sizeof(T) == 2 ? 96 : 64) + at % 32) * E;
       if constexpr (sizeof(T) == 2) {
-        Four<T> hi, lo;
+        Four<T> v[kTerms<T>];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) two_parts(acc[j][t][i] * by, hi.v[i], lo.v[i]);
-        *(Four<T>*)(out + g % 2 * 4) = hi;
-        *(Four<T>*)(out + 32 * E + g % 2 * 4) = lo;
+        for (int i = 0; i < 4; ++i) {
+          T one[kTerms<T>];
+          terms(acc[j][t][i] * by, one);
+#pragma unroll
+          for (int h = 0; h < kTerms<T>; ++h) v[h].v[i] = one[h];
+        }
+#pragma unroll
+        for (int h = 0; h < kTerms<T>; ++h) *(Four<T>*)(out + h * 32 * E + g % 2 * 4) = v[h];
       } else {
         *(f4*)(out + g % 2 * 32 * E) = acc[j][t];
       }
@@ -1124,27 +1135,29 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
       wrong |= (unsigned)(mine[t] < -1 || mine[t] >= a.rows.n) << t;
     }
     // The accumulators begin with s_i (U F_i) G_i, while the first tiles load (SPLIT: each part of the sum with
-    // some of the adapters and ranks).  U F_i comes as two values of the type (fp32: itself), so 8 ranks are
-    // one step; the loads of kSets steps are under way at a time.  A row without this adapter loads its own
+    // some of the adapters and ranks).  U F_i comes as three values of the type (fp32: itself); the loads of kSets steps are under way at a time.  A row without this adapter loads its own
     // garbage, which reaches that row's accumulators alone, and these are set afterwards.
     auto has = [&](int t) { return mine[t] >= 0 && mine[t] < a.rows.n; };
     auto place = [&](int t) { return (int64_t)min(t0 + wt + t * kB + lb, a.rows.T - 1); };
-    // the fragments that the low-rank pass and the first launch wrote, of 32 places or columns and 8 ranks; with 16-bit
-    // types the lanes' four groups take the upper and the lower parts of two such blocks
-    constexpr int kRanks = sizeof(T) == 2 ? 16 : 8;  // of an instruction
+    // the fragments that the low-rank pass and the first launch wrote, of 32 places or columns and 8 ranks.  Such a
+    // block is a slot, with 16-bit types one for each of its terms; these types' instructions take four slots, one by
+    // each group of 16 lanes.  A slot behind the last is zeros on both sides.
+    constexpr int kSlots = sizeof(T) == 2 ? 4 : 1;
+    const int slots = (a.r + 7) / 8 * kTerms<T>;
     auto x_of = [&](int t, int b) {
       const int at = t0 + wt + t * kB;
-      const int64_t block = min(at / 32, (a.rows.T - 1) / 32);
+      const int64_t first = (int64_t)min(at / 32, (a.rows.T - 1) / 32) * (a.rp / 8) * kTerms<T>;
       if constexpr (sizeof(T) == 2)
-        return ((const Frag*)a.split)[(block * (a.rp / 8) + b / 8 + g % 2) * 64 + g / 2 * 32 + at % 32 + lb];
-      else return ((const Frag*)a.split)[(block * (a.rp / 8) + b / 8) * 64 + lane];
+        return b + g < slots ? ((const Frag*)a.split)[(first + b + g) * 32 + at % 32 + lb] : Frag{};
+      else return ((const Frag*)a.split)[(first + b) * 64 + lane];
     };
     auto w_of = [&](int cur, int j, int b) {
       const int n = n0 + wn + j * kB;
       const int64_t blocks = (a.N + 31) / 32, block = min((int64_t)n / 32, blocks - 1);
-      const int64_t at = (cur * blocks + block) * (a.rp / 8) + b / 8;
-      if constexpr (sizeof(T) == 2) return ((const Frag*)a.G)[(at + g % 2) * 32 + n % 32 + lb];
-      else return ((const Frag*)a.G)[at * 64 + lane];
+      const int64_t first = (cur * blocks + block) * (a.rp / 8);
+      if constexpr (sizeof(T) == 2)
+        return b + g < slots ? ((const Frag*)a.G)[(first + (unsigned)(b + g) / kTerms<T>) * 32 + n % 32 + lb] : Frag{};
+      else return ((const Frag*)a.G)[(first + b) * 64 + lane];
     };
     auto factor = [&](int t, int cur) {
       float f = scale_of(a.rows, cur);
@@ -1168,23 +1181,23 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
       // one adapter among all of the wave's rows: straight into the accumulators, zeros again where it is no row's
       Frag x[kSets][TT], w[kSets][TN];
       auto fetch = [&](int q, int b) {
-        if (b >= a.r) return;
+        if (b >= slots) return;
 #pragma unroll
         for (int t = 0; t < TT; ++t) x[q][t] = x_of(t, b);
 #pragma unroll
         for (int j = 0; j < TN; ++j) w[q][j] = w_of(first, j, b);
       };
 #pragma unroll
-      for (int q = 0; q < kSets; ++q) fetch(q, (share + q * shares) * kRanks);
-      for (int b = share * kRanks; b < a.r; b += kSets * shares * kRanks)
+      for (int q = 0; q < kSets; ++q) fetch(q, (share + q * shares) * kSlots);
+      for (int b = share * kSlots; b < slots; b += kSets * shares * kSlots)
 #pragma unroll
         for (int q = 0; q < kSets; ++q) {
-          if (b + q * shares * kRanks < a.r)
+          if (b + q * shares * kSlots < slots)
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
               for (int t = 0; t < TT; ++t) acc[j][t] = Block<T>::mma(w[q][j], x[q][t], acc[j][t]);
-          fetch(q, b + (kSets + q) * shares * kRanks);
+          fetch(q, b + (kSets + q) * shares * kSlots);
         }
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
@@ -1204,19 +1217,19 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
           const int cur = __builtin_amdgcn_readlane(mine[t], __builtin_ctzll(left));
           left &= ~__ballot(mine[t] == cur);
           Acc d[TN] = {};
-          for (int b = 0; b < a.r; b += kRanks * kSets) {
+          for (int b = 0; b < slots; b += kSlots * kSets) {
             if (SPLIT && unit++ % shares != 0) continue;
             Frag x[kSets], w[TN][kSets];
 #pragma unroll
             for (int q = 0; q < kSets; ++q) {
-              if (b + q * kRanks >= a.r) continue;
-              x[q] = x_of(t, b + q * kRanks);
+              if (b + q * kSlots >= slots) continue;
+              x[q] = x_of(t, b + q * kSlots);
 #pragma unroll
-              for (int j = 0; j < TN; ++j) w[j][q] = w_of(cur, j, b + q * kRanks);
+              for (int j = 0; j < TN; ++j) w[j][q] = w_of(cur, j, b + q * kSlots);
             }
 #pragma unroll
             for (int q = 0; q < kSets; ++q)
-              if (b + q * kRanks < a.r)
+              if (b + q * kSlots < slots)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) d[j] = Block<T>::mma(w[j][q], x[q], d[j]);
           }
@@ -1310,7 +1323,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
 // places of an adapter of U_t^T V_t, V = S or D, in pieces of `size` places (32 to kGradRows: with few rows smaller
 // ones, for enough workgroups, but not so small that the parts, a rank's 4 bytes a column each, outweigh U's).  A
 // workgroup takes 64 kE columns of U, a wave 16 kE, whose rows it turns in registers.  V is turned on its way to
-// LDS, as upper and lower part of the type (fp16: brought to below 2^14 by the piece's power of two).  Bound by
+// LDS, as the sum of three values of the type (fp16: brought to below 2^14 by the piece's power of two).  Bound by
 // reading U once: each wave keeps two steps' rows in flight.
 constexpr int kGradRows = 128;
 struct Outer {
@@ -1336,8 +1349,8 @@ template <class T, int RB, bool DIRECT>
 __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int E = M::kE, kHalves = sizeof(T) == 2 ? 2 : 1, kRanks = RB * 16, kPitch = kGradRows + 16 / sizeof(T);
-  __shared__ __attribute__((aligned(16))) T vs[kHalves][kRanks][kPitch];
+  constexpr int E = M::kE, kRanks = RB * 16, kPitch = kGradRows + 16 / sizeof(T);
+  __shared__ __attribute__((aligned(16))) T vs[kTerms<T>][kRanks][kPitch];
   __shared__ int32_t row[kGradRows];
   __shared__ float wave_most[4];
   const Outer& a = both.p[blockIdx.y];
@@ -1398,8 +1411,10 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int j = q * 8 + threadIdx.x % 2 * 4 + e;
-      if constexpr (kHalves == 2) two_parts(v[q][e] * by, vs[0][j][t], vs[1][j][t]);
-      else vs[0][j][t] = v[q][e];
+      T one[kTerms<T>];
+      terms(v[q][e] * by, one);
+#pragma unroll
+      for (int h = 0; h < kTerms<T>; ++h) vs[h][j][t] = one[h];
     }
   __syncthreads();
   if (n0 >= a.cu) return;
@@ -1410,7 +1425,7 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
       Frag w[E];
       turn<T>(in[q], w);
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h)
+      for (int h = 0; h < kTerms<T>; ++h)
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
           const Frag x = *(const Frag*)&vs[h][b * 16 + l16][(s + q) * M::kStep + g * E];
@@ -1696,7 +1711,7 @@ struct Many {
       l.arrived = prep.counter + prep.counters;
       prep.counters += l.pieces;
     }
-    l.split = ws.template take<T>(up(a.T, 32) * rp * (sizeof(T) == 2 ? 2 : 1));
+    l.split = ws.template take<T>(up(a.T, 32) * rp * kTerms<T>);
     if (std::is_same_v<T, _Float16>) l.by = ws.template take<float>(a.T);
     return l;
   }

@@ -8,7 +8,7 @@ W (K, N) is shared by all rows, A (n, K, r) and B (n, r, N) hold the factors
 of n adapters.  One call serves prompts, single tokens and any mixture of
 requests; the gradient call is its backward pass for training the adapters
 (W stays as it is).  fp32, bf16 and fp16; sums are held in fp32, and X @ A[i]
-enters the second product with at least 16 bits (csrc/hip/adapter.hip).
+enters the second product with all of its bits (csrc/hip/adapter.hip).
 """
 from __future__ import annotations
 
