@@ -739,6 +739,7 @@ struct LowPair {
   Rows rows;
   Order order;
   const Piece* table;
+  int r;
 };
 constexpr int kLowRows = 32;
 constexpr int kLowWaves = 8;
@@ -746,17 +747,26 @@ constexpr int kLowWaves = 8;
 // one step 29)
 constexpr int low_flight(int rank_blocks) { return rank_blocks <= 4 ? 4 : rank_blocks == 8 ? 2 : 1; }
 
-// v as the sum of kTerms values of the type, each the rounding of what the ones before leave (a difference without a
-// rounding of its own); the lower ones are 0 beside an infinity or NaN
+// v as the sum of kTerms values of the type, all of its sign and none of them zero: each but the last is the largest
+// one below what is left (in size), so that nothing is lost on the way (bf16: 8 + 8 + 8 bits).  Beside an infinite
+// factor the terms then give v's infinity; with the nearest values a second term of 0 or of the other sign would give
+// NaN.  0, infinities and NaN are all of their terms.
 template <class T>
 constexpr int kTerms = sizeof(T) == 2 ? 3 : 1;
 template <class T>
 __device__ __forceinline__ void terms(float v, T (&out)[kTerms<T>]) {
+  const bool whole = !(fabsf(v) > 0.f && fabsf(v) <= 3.402823466e38f);
 #pragma unroll
-  for (int h = 0; h < kTerms<T>; ++h) {
-    out[h] = (T)v;
-    v = fabsf((float)out[h]) <= 3.4e38f ? v - (float)out[h] : 0.f;
+  for (int h = 0; h < kTerms<T> - 1; ++h) {
+    const float below = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) - 1);
+    T t = 0;
+    if constexpr (std::is_same_v<T, _Float16>) t = (T)__builtin_amdgcn_cvt_pkrtz(below, 0.f)[0];
+    else if constexpr (sizeof(T) == 2)
+      t = __builtin_bit_cast(T, (unsigned short)(__builtin_bit_cast(unsigned, below) >> 16));
+    out[h] = whole ? (T)v : t;
+    v = whole ? v : v - (float)t;
   }
+  out[kTerms<T> - 1] = (T)v;
 }
 // a power of two that brings fp16's `most` to [2^13, 2^14)
 __device__ __forceinline__ int to_fp16_range(float most) {
@@ -867,6 +877,12 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
         for (int t = 0; t < 2; ++t) acc[j][t] = lds[0][j * 2 + t][lane];
   }
   if (wave) return;
+  // behind the last rank zeros, not an infinity times F's zeros there
+#pragma unroll
+  for (int j = 0; j < RB; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (j * 16 + g * 4 + i >= both.r) acc[j][0][i] = acc[j][1][i] = 0.f;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const bool in = t * 16 + l16 < pc.count;
@@ -1721,7 +1737,7 @@ struct Many {
   }
   void run_low(const Low* l, int count, hipStream_t s) {
     LowPair both{};
-    both.rows = g, both.order = order, both.table = prep.pieces[0].table;
+    both.rows = g, both.order = order, both.table = prep.pieces[0].table, both.r = (int)a.r;
     unsigned most = 0;
     for (int k = 0; k < count; ++k) {
       both.p[k] = l[k];

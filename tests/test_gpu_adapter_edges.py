@@ -56,3 +56,58 @@ def test_factor_gradients_of_32_bit_sums(gelim, cuda, T, r, dtype):
     assert (dB == 1024 * least).all()
     dA = gelim.ops.adapter_matmul_grad(low, other, W, zero, factor.transpose(1, 2))[1]
     assert (dA == 1024 * least).all()
+
+
+def same_kind(got, ref):
+    """Infinities of the same sign and NaN in the same places, finite values elsewhere."""
+    got, ref = got.detach().cpu().double(), ref
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    where = torch.isinf(ref)
+    assert torch.equal(torch.isinf(got), where) and torch.equal(got[where], ref[where])
+
+
+def mm(a, b):
+    """a @ b with each sum's terms as they are: no zeros of a padded tile beside an infinity."""
+    return (a.unsqueeze(-1) * b.unsqueeze(-3)).sum(-2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r", [1, 3, 16, 17])
+@pytest.mark.parametrize("T", [7, 64, 65, 130, 300])
+def test_infinities_are_what_the_formula_makes_of_them(gelim, cuda, T, r, dtype):
+    """An infinite weight, factor or input, on either side of the sizes at which other kernels take over.  Small whole
+    numbers, so that sums of a few bits (one part of the type holds them, the others are zero) stand beside infinities."""
+    K, N = 24, 40
+    g = torch.Generator().manual_seed(100 * T + r)
+
+    def whole(*shape):
+        v = torch.randint(1, 3, shape, generator=g) * (torch.randint(0, 2, shape, generator=g) * 2 - 1)
+        return v.double()
+
+    for k in range(5):
+        X, W, A, B, dY = whole(T, K), whole(K, N), whole(2, K, r), whole(2, r, N), whole(T, N)
+        index = torch.randint(-1, 2, (T,), generator=g)
+        index[T - 1] = 0
+        inf = float("inf") if k % 2 else -float("inf")
+        if k == 0:
+            B[0, r - 1, 5] = inf
+        elif k == 1:
+            A[0, 3, 0] = inf
+        elif k == 2:
+            X[T - 1, 7] = inf
+        elif k == 3:
+            dY[T - 1, 9] = inf
+        else:
+            W[3, 5] = inf
+        args = [v.to(dtype).to(cuda) for v in (X, W, A, B)] + [index.int().to(cuda), 2.0]
+        Y, dX = mm(X, W), mm(dY, W.t())
+        dA, dB = torch.zeros_like(A), torch.zeros_like(B)
+        for i in range(2):
+            t = index == i
+            S, D = mm(X[t], A[i]), mm(dY[t], B[i].t())
+            Y[t] += 2 * mm(S, B[i])
+            dX[t] += 2 * mm(D, A[i].t())
+            dA[i], dB[i] = 2 * mm(X[t].t(), D), 2 * mm(S.t(), dY[t])
+        same_kind(gelim.ops.adapter_matmul(*args), Y)
+        for got, ref in zip(gelim.ops.adapter_matmul_grad(dY.to(dtype).to(cuda), *args), (dX, dA, dB)):
+            same_kind(got, ref)
