@@ -1454,7 +1454,8 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
     fetch(s);
   }
   if constexpr (DIRECT) {
-    const float f = scale_of(both.rows, pc.adapter) * back;
+    // an adapter without rows gets zeros, whatever its factor holds
+    const float f = pc.count ? scale_of(both.rows, pc.adapter) * back : 0.f;
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       const int j = j0 + b * 16 + l16;
@@ -1529,7 +1530,7 @@ __global__ __launch_bounds__(256) void sum_kernel(SumPair both) {
       s += lds[0][lane] + lds[1][lane] + lds[2][lane];
     }
     if ((!SHARE || wave == 0) && c < a.cols) {
-      s = s * scale_of(both.rows, i);
+      s = s * (count ? scale_of(both.rows, i) : 0.f);  // without rows zeros, whatever the factor holds
       T* out = (T*)a.out + i * a.as + c * a.cs + j0 * a.rs;
       if (a.rs == 1 && j0 + 4 <= both.r) {
         *(Four<T>*)out = Four<T>{(T)s[0], (T)s[1], (T)s[2], (T)s[3]};

@@ -111,3 +111,28 @@ def test_infinities_are_what_the_formula_makes_of_them(gelim, cuda, T, r, dtype)
         same_kind(gelim.ops.adapter_matmul(*args), Y)
         for got, ref in zip(gelim.ops.adapter_matmul_grad(dY.to(dtype).to(cuda), *args), (dX, dA, dB)):
             same_kind(got, ref)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [40, 128, 129, 700, 9000])
+@pytest.mark.parametrize("n", [5, 30])
+def test_scales_of_adapters_without_rows(gelim, cuda, T, n, dtype):
+    """An adapter that no row has gets zeros whatever its scale is: a slot not filled yet, or alpha / 0."""
+    K, N, r = 72, 136, 12
+    g = torch.Generator().manual_seed(T + n)
+    X, W, A, B, dY = (torch.randn(s, generator=g).to(dtype).to(cuda) for s in
+                      ((T, K), (K, N), (n, K, r), (n, r, N), (T, N)))
+    index = (torch.arange(T) % 3 * 2 - 1).clamp(max=n - 1).int().to(cuda)  # -1, 1 and 3
+    scale = torch.full((n,), 0.5, device=cuda)
+    want = gelim.ops.adapter_matmul_grad(dY, X, W, A, B, index, scale)
+    wantY = gelim.ops.adapter_matmul(X, W, A, B, index, scale)
+    for bad in (math.nan, math.inf, -math.inf):
+        scale[[0, 2, 4]] = bad
+        scale[5:] = bad
+        assert torch.equal(gelim.ops.adapter_matmul(X, W, A, B, index, scale), wantY)
+        got = gelim.ops.adapter_matmul_grad(dY, X, W, A, B, index, scale)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        assert not got[1][0].any() and not got[2][4].any() and not got[1][5:].any()
+        norm = gelim.ops.clip_global_norm([got[1], got[2]], 1.0)
+        assert torch.isfinite(norm)
