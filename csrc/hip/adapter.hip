@@ -484,13 +484,13 @@ __device__ __forceinline__ int64_t row_at(const Order& o, int64_t at) { return o
 // floor((s + c) / size) - floor(s / size) + 1 >= ceil(c / size), and without a
 // sum over the adapters.  Numbers in between stay empty (count 0).
 struct Piece {
-  int adapter, begin, count, first;  // first: its adapter's first, also with count 0
+  int adapter, begin, count;
 };
 __device__ __forceinline__ int first_piece(const Order& o, int i, int size) {
   return o.start ? o.start[i] / size + i : 0;
 }
 __device__ __forceinline__ Piece piece_of(const Piece* table, const Rows& g, int number, int size) {
-  if (!table) return {0, number * size, max(0, min(size, g.T - number * size)), number == 0};
+  if (!table) return {0, number * size, max(0, min(size, g.T - number * size))};
   return table[number];
 }
 int pieces(int64_t T, int64_t n, bool ordered, int size) { return (int)(T / size + (ordered ? n : 1)); }
@@ -591,7 +591,7 @@ __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
     const int first = begin / size + i, end = i < n ? at / size + i + 1 : p.rows.T / size + n;
     for (int q = first + threadIdx.x; q < end; q += kPrepare) {
       const int from = begin + (q - first) * size;
-      p.pieces[k].table[q] = {i, from, i < n ? max(0, min(size, at - from)) : 0, i < n && q == first};
+      p.pieces[k].table[q] = {i, from, i < n ? max(0, min(size, at - from)) : 0};
     }
   }
 }
@@ -1348,7 +1348,7 @@ struct Outer {
   const float* low;  // V
   float* part;       // piece, rank, column
   int cu, ldp, blocks;
-  // with at most one piece an adapter: the gradient itself, at adapter as + column cs + rank rs
+  // DIRECT, with at most one piece an adapter: the gradient itself, at adapter as + column cs + rank rs
   void* out;
   int64_t as, cs, rs;
   int cols;
@@ -1360,6 +1360,11 @@ struct OuterPair {
   const Piece* table;
   int rp, pieces, size, r;
 };
+// all of adapter i's rows as one piece
+__device__ __forceinline__ Piece whole_of(const Order& o, const Rows& g, int i) {
+  if (!o.start) return {0, 0, g.T};
+  return {i, o.start[i], o.start[i + 1] - o.start[i]};
+}
 
 template <class T, int RB, bool DIRECT>
 __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
@@ -1372,8 +1377,8 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   const Outer& a = both.p[blockIdx.y];
   const int piece = blockIdx.x % both.pieces, block = blockIdx.x / both.pieces;
   if (block >= a.blocks) return;
-  const Piece pc = piece_of(both.table, both.rows, piece, both.size);
-  if (DIRECT ? !pc.first : pc.count == 0) return;
+  const Piece pc = DIRECT ? whole_of(both.order, both.rows, piece) : piece_of(both.table, both.rows, piece, both.size);
+  if (!DIRECT && pc.count == 0) return;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
   const int j0 = blockIdx.z * kRanks;
   if (threadIdx.x < kGradRows)
@@ -1889,8 +1894,8 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   int size = kGradRows;
   const bool direct = a.T > 0 && a.T <= size;  // no adapter has more than one piece: no parts to add up
   while (!direct && size > std::max(32, 2 * m.rp) && a.T / size * ((K + N) / (64 * Mma<T>::kE)) < 256) size /= 2;
-  const int pcs = pieces(a.T, a.n, a.index != nullptr, size);
-  m.set_pieces(1, size);
+  const int pcs = direct ? (int)a.n : pieces(a.T, a.n, a.index != nullptr, size);
+  if (!direct) m.set_pieces(1, size);
   OuterPair op{};
   SumPair sp{};
   op.rows = sp.rows = m.g, op.order = sp.order = m.order;
@@ -1909,7 +1914,7 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
     o.U = U.p, o.low = low[k].low, o.ldu = U.ld, o.cu = U.cols;
     o.blocks = (U.cols + 64 * Mma<T>::kE - 1) / (64 * Mma<T>::kE);
     o.ldp = (int)up(U.cols, 16 * Mma<T>::kE);
-    o.part = ws.take<float>((int64_t)pcs * m.rp * o.ldp);
+    if (!direct) o.part = ws.take<float>((int64_t)pcs * m.rp * o.ldp);
     u.part = o.part, u.out = k ? a.dB : a.dA, u.cols = cols, u.ldp = o.ldp;
     u.as = (int64_t)a.r * cols;
     const bool along = k ? !a.b_trans : a.a_trans;  // columns side by side

@@ -1,0 +1,20 @@
+"""What the adapter calls ask for as workspace: no more than the call at hand uses.  Sizes only, no GPU."""
+import pytest
+
+MIB = 2 ** 20
+
+
+def need(grad, T, K, N, r, n, dtype=1, indexed=True, x=0, w=0, y=0, wt=0):
+    from gelim.ops import adapter
+
+    return adapter._workspace_bytes(grad, dtype, T, K, N, r, n, K, K if wt else N, wt, r, 0, N, 0, N, x, w, y, indexed)
+
+
+@pytest.mark.parametrize("T", [5, 128])
+def test_no_parts_where_no_adapter_has_two_pieces(gelim, T):
+    """Up to 128 rows the factor gradients are written without parts to add up: three layouts of the factors (two of B's
+    and A's sums, one of A's columns) and what belongs to the rows is all there is: at most 16 parts of dX, as the
+    large product's sum is cut into no more, and per row less than 1 KB of low-rank sums at this rank."""
+    K, N, r, n = 4096, 4096, 16, 2000
+    layouts = n * r * (2 * K + N) * 2
+    assert need(True, T, K, N, r, n) <= layouts + 16 * T * K * 4 + T * 1024 + MIB
