@@ -1675,7 +1675,7 @@ struct Many {
     rb = rank_blocks(a.r);
     rp = 16 * rb;
     prep.rows = g;
-    if (a.index) {
+    if (a.index && a.T) {
       prep.perm = ws.template take<int32_t>(a.T);
       prep.start = ws.template take<int32_t>(a.n + 1);
       prep.order_groups = (int)a.n + 1;
@@ -1880,16 +1880,20 @@ int product(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
 
 template <class T>
 int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
-  const bool all = !run;  // the workspace is for all three
+  if (!a.dX && !a.dA && !a.dB) return GELIM_OK;
+  // what the wanted results need, and nothing else: S for dB, D for the others, X for the factors' gradients
+  const bool need_s = a.T && a.dB, need_d = a.T && (a.dX || a.dA), need_x = a.T && (a.dA || a.dB);
   Many<T> m(a, ws);
   const int K = (int)a.K, N = (int)a.N;
-  const auto X = m.wide(a.X, a.ldx, a.T, K), dY = m.wide(a.Y, a.ldy, a.T, N);
+  typename Many<T>::Wide X{}, dY{};
+  if (need_x) X = m.wide(a.X, a.ldx, a.T, K);
+  if (a.T) dY = m.wide(a.Y, a.ldy, a.T, N);
   const Problem back = back_of(a);
   typename Many<T>::Plan q{};
   Low low[2];  // D, S
-  low[0] = m.low_of(dY, back.F, N);
-  low[1] = m.low_of(X, view_a(a), K);
-  if ((a.dX && a.T) || all) q = m.big_of(back, dY);
+  if (need_d) low[0] = m.low_of(dY, back.F, N);
+  if (need_s) low[1] = m.low_of(X, view_a(a), K);
+  if (a.dX && a.T) q = m.big_of(back, dY);
   // the sides: dA = X^T D, dB^T = dY^T S
   int size = kGradRows;
   const bool direct = a.T > 0 && a.T <= size;  // no adapter has more than one piece: no parts to add up
@@ -1905,7 +1909,7 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   int sides = 0;
   int64_t outer_groups = 0, sum_groups = 0;
   for (int k = 0; k < 2; ++k) {
-    if (!(k ? a.dB : a.dA) && !all) continue;
+    if (!(k ? a.dB : a.dA)) continue;
     const auto& U = k ? dY : X;
     const int cols = k ? N : K;
     Outer& o = op.p[sides];
@@ -1931,7 +1935,6 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
   if (!run) return GELIM_OK;
   m.run_prepare(s);
   if (a.T) {
-    const bool need_d = a.dX || a.dA, need_s = a.dB != nullptr;
     m.run_low(need_d ? low : low + 1, need_d + need_s, s);
     if (a.dX) m.run_big(q, low[0], s);
   }

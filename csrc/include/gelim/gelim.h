@@ -298,6 +298,7 @@ typedef struct gelim_adapter_args {
 } gelim_adapter_args;
 /* sizeof (which = 0) or the offset of T / index / ws_bytes (1 / 2 / 3) */
 int64_t gelim_adapter_args_layout(int32_t which);
+/* bytes for a call with these sizes, layouts and addresses; of dX, dA and dB counts what is not NULL */
 int64_t gelim_adapter_workspace(const gelim_adapter_args* a, int grad);
 int gelim_adapter_matmul(const gelim_adapter_args* a, void* stream);
 int gelim_adapter_matmul_grad(const gelim_adapter_args* a, void* stream);

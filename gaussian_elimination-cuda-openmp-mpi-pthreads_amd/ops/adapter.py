@@ -94,13 +94,14 @@ def _check(X, W, A, B, index, scale):
 
 
 @lru_cache(maxsize=4096)
-def _workspace_bytes(grad: bool, *layout) -> int:
-    """What a call of these sizes and layouts needs."""
+def _workspace_bytes(grad: bool | tuple[bool, bool, bool], *layout) -> int:
+    """What a call of these sizes and layouts needs; grad: whether it is the gradient, or which of its results."""
     dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, ldy, x, w, y, indexed = layout
+    dX, dA, dB = grad if isinstance(grad, tuple) else (grad,) * 3
     # an address's low bits choose between reading in place and copying, so they take the place of the addresses
     args = _ARGS.pack(dtype, T, K, N, r, n, x, ldx, w, ldw, wt, 0, 0, lda, at, 0, 0, ldb, bt, indexed, 0, 0.0,
-                      y, ldy, 0, 0, 0, 0, 0, 0)
-    need = _native.lib().gelim_adapter_workspace(args, grad)
+                      y, ldy, dX, K, dA, dB, 0, 0)
+    need = _native.lib().gelim_adapter_workspace(args, bool(grad))
     if need < 0:
         _native.check(need, "adapter_matmul")
     return need
@@ -121,7 +122,8 @@ def _call(grad, dev, T, K, N, n, r, X, W, A, B, index, scale, Y, dX=None, dA=Non
         index = index.contiguous()
     dtype = TYPES[X.dtype]
     xp, wp, yp = X.data_ptr(), W.data_ptr(), Y.data_ptr()
-    ws_bytes = _workspace_bytes(grad, dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, ldy,
+    wanted = (dX is not None, dA is not None, dB is not None) if grad else False
+    ws_bytes = _workspace_bytes(wanted, dtype, T, K, N, r, n, ldx, ldw, wt, lda, at, ldb, bt, ldy,
                                 xp & 15, wp & 15, yp & 15, index is not None)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     args = _ARGS.pack(dtype, T, K, N, r, n, xp, ldx, wp, ldw, wt, A.data_ptr(), A.stride(0), lda, at, B.data_ptr(),

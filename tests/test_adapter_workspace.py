@@ -18,3 +18,21 @@ def test_no_parts_where_no_adapter_has_two_pieces(gelim, T):
     K, N, r, n = 4096, 4096, 16, 2000
     layouts = n * r * (2 * K + N) * 2
     assert need(True, T, K, N, r, n) <= layouts + 16 * T * K * 4 + T * 1024 + MIB
+
+
+@pytest.mark.parametrize("T", [100, 1000])
+def test_results_that_are_not_wanted_need_no_room(gelim, T):
+    """Each of the three results alone: the copies and layouts that it reads.  X one element behind a multiple of 16 bytes
+    is copied, 2 T K bytes and less than a page to fill rows up, for dA and dB only."""
+    K, N, r, n = 4096, 2048, 16, 40
+    layout = {"A as columns of S": n * r * K * 2, "B as columns of D": n * r * N * 2, "A as rows": n * r * K * 2}
+    whole = need(True, T, K, N, r, n, x=2)
+    dX, dA, dB = (need(tuple(k == j for j in range(3)), T, K, N, r, n, x=2) for k in range(3))
+    copy = T * K * 2
+    assert max(dX, dA, dB) < whole
+    assert dX <= whole - copy - layout["A as columns of S"]
+    assert dA <= whole - layout["A as columns of S"] - layout["A as rows"]
+    assert dB <= whole - layout["B as columns of D"] - layout["A as rows"]
+    assert need((False, True, True), T, K, N, r, n, x=2) - need((False, True, True), T, K, N, r, n) >= copy
+    assert need((True, False, False), T, K, N, r, n, x=2) == need((True, False, False), T, K, N, r, n)
+    assert need((False, False, False), T, K, N, r, n, x=2) == 0
