@@ -479,21 +479,21 @@ struct Order {
 };
 __device__ __forceinline__ int64_t row_at(const Order& o, int64_t at) { return o.perm ? o.perm[at] : at; }
 
-// Pieces of at most `size` places, each within one adapter.  Adapter i's
-// pieces have the numbers from start[i] / size + i on: distinct for different adapters, as
-// floor((s + c) / size) - floor(s / size) + 1 >= ceil(c / size), and without a
-// sum over the adapters.  Numbers in between stay empty (count 0).
+// Pieces of at most `size` places, each within one adapter.  Adapter i's pieces have the numbers from
+// start[i] / size + min(i, start[i]) on: distinct for different adapters, as floor((s + c) / size) - floor(s / size) + 1
+// >= ceil(c / size) and an adapter with rows moves both i and start on, and without a sum over the adapters.  So there
+// are no more than T / size + min(n, T) numbers, however many adapters are resident.  Some stay empty (count 0).
 struct Piece {
   int adapter, begin, count;
 };
-__device__ __forceinline__ int first_piece(const Order& o, int i, int size) {
-  return o.start ? o.start[i] / size + i : 0;
-}
+__device__ __forceinline__ int first_piece(int start, int i, int size) { return start / size + min(i, start); }
 __device__ __forceinline__ Piece piece_of(const Piece* table, const Rows& g, int number, int size) {
   if (!table) return {0, number * size, max(0, min(size, g.T - number * size))};
   return table[number];
 }
-int pieces(int64_t T, int64_t n, bool ordered, int size) { return (int)(T / size + (ordered ? n : 1)); }
+int pieces(int64_t T, int64_t n, bool ordered, int size) {
+  return (int)(T / size + std::min<int64_t>(ordered ? n : 1, T));
+}
 
 // A matrix (one per adapter) copied as rows x ld values, zeros behind the source's rows and columns; or in a matrix
 // instruction's fragments, so that a wave's load of one is 1 KB without gaps: kFrag16 by steps along ld, blocks of 16
@@ -588,7 +588,8 @@ __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
   for (int k = 0; k < 2; ++k) {
     const int size = p.pieces[k].size;
     if (!p.pieces[k].table) continue;
-    const int first = begin / size + i, end = i < n ? at / size + i + 1 : p.rows.T / size + n;
+    const int first = first_piece(begin, i, size);
+    const int end = i < n ? first_piece(at, i + 1, size) : p.rows.T / size + min(n, p.rows.T);
     for (int q = first + threadIdx.x; q < end; q += kPrepare) {
       const int from = begin + (q - first) * size;
       p.pieces[k].table[q] = {i, from, i < n ? max(0, min(size, at - from)) : 0};
@@ -1518,7 +1519,8 @@ __global__ __launch_bounds__(256) void sum_kernel(SumPair both) {
   const int c = blockIdx.x / groups * 64 + lane, j0 = blockIdx.x % groups * kRanks + (SHARE ? 0 : wave * 4);
   for (int i = blockIdx.z; i < both.rows.n; i += gridDim.z) {
     const int count = both.order.start ? both.order.start[i + 1] - both.order.start[i] : both.rows.T;
-    const int first = first_piece(both.order, i, both.size), many = (count + both.size - 1) / both.size;
+    const int first = both.order.start ? first_piece(both.order.start[i], i, both.size) : 0;
+    const int many = (count + both.size - 1) / both.size;
     f4 s = {0.f, 0.f, 0.f, 0.f};
     if (j0 < both.rp)
 #pragma unroll 4

@@ -36,3 +36,25 @@ def test_results_that_are_not_wanted_need_no_room(gelim, T):
     assert need((False, True, True), T, K, N, r, n, x=2) - need((False, True, True), T, K, N, r, n) >= copy
     assert need((True, False, False), T, K, N, r, n, x=2) == need((True, False, False), T, K, N, r, n)
     assert need((False, False, False), T, K, N, r, n, x=2) == 0
+
+
+@pytest.mark.parametrize("T", [130, 200, 3000])
+def test_pieces_go_by_rows_not_by_resident_adapters(gelim, T):
+    """Beyond as many adapters as rows another one costs its layouts and its entry of the order, no parts of gradients."""
+    K, N, r = 1024, 2048, 64
+    more = need(True, T, K, N, r, T + 300) - need(True, T, K, N, r, T)
+    assert more <= 300 * (r * (2 * K + N) * 2 + 4) + 1024
+
+
+@pytest.mark.parametrize("T", [128, 200])
+def test_small_batch_beside_many_adapters(gelim, T):
+    """What one piece a row would need, the most that rows can be cut into, for both gradients in fp32."""
+    K, N, r, n = 8192, 8192, 64, 500
+    layouts, parts = n * r * (2 * K + N) * 2, (T // 32 + T) * r * (K + N) * 4
+    assert need(True, T, K, N, r, n) <= layouts + parts + 16 * T * K * 4 + T * 8192
+
+
+def test_no_rows_need_the_same_with_and_without_an_index(gelim):
+    """An index of no rows has no address, so the call cannot tell the two apart."""
+    for grad in (False, True):
+        assert need(grad, 0, 64, 48, 4, 2) == need(grad, 0, 64, 48, 4, 2, indexed=False)

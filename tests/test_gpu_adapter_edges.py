@@ -136,3 +136,23 @@ def test_scales_of_adapters_without_rows(gelim, cuda, T, n, dtype):
         assert not got[1][0].any() and not got[2][4].any() and not got[1][5:].any()
         norm = gelim.ops.clip_global_norm([got[1], got[2]], 1.0)
         assert torch.isfinite(norm)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T, n, used", [(129, 500, 129), (200, 3000, 7), (400, 401, 400), (700, 900, 3), (1500, 40, 40)])
+def test_pieces_of_many_adapters(gelim, cuda, T, n, used, dtype):
+    """More adapters than rows, most with one row or none, a few with several pieces."""
+    from test_gpu_adapter import check, make, ref_grad, ref_product
+
+    K, N, r = 72, 40, 5
+    X, W, A, B, index, scale = make(cuda, T, K, N, r, n, dtype)
+    g = torch.Generator().manual_seed(T + n)
+    some = torch.randperm(n, generator=g)[:used]
+    which = torch.cat([some, some[torch.randint(0, min(3, used), (T,), generator=g)]])[:T]
+    index = which[torch.randperm(T, generator=g)].int().to(cuda)
+    index[T // 3] = -1
+    args = X, W, A, B, index, scale
+    check(gelim.ops.adapter_matmul(*args), *ref_product(*args, device=cuda))
+    dY = torch.randn(T, N, generator=g).to(dtype).to(cuda)
+    for v, t in zip(gelim.ops.adapter_matmul_grad(dY, *args), ref_grad(dY, *args, device=cuda)):
+        check(v, *t)
