@@ -476,19 +476,22 @@ void finish(const Finish& e, hipStream_t s) {
 
 struct Order {
   const int32_t *perm, *start;
+  bool packed;  // the layouts of the factors have a slot for each row's adapter at most, not one for each resident one
 };
 __device__ __forceinline__ int64_t row_at(const Order& o, int64_t at) { return o.perm ? o.perm[at] : at; }
+// adapter i's layout, if it has rows: both i and start grow from one adapter with rows to the next, and start < T
+__device__ __forceinline__ int packed_slot(int i, int start) { return min(i, start); }
 
 // Pieces of at most `size` places, each within one adapter.  Adapter i's pieces have the numbers from
 // start[i] / size + min(i, start[i]) on: distinct for different adapters, as floor((s + c) / size) - floor(s / size) + 1
 // >= ceil(c / size) and an adapter with rows moves both i and start on, and without a sum over the adapters.  So there
 // are no more than T / size + min(n, T) numbers, however many adapters are resident.  Some stay empty (count 0).
 struct Piece {
-  int adapter, begin, count;
+  int adapter, begin, count, slot;  // slot: where its factors are laid out
 };
 __device__ __forceinline__ int first_piece(int start, int i, int size) { return start / size + min(i, start); }
 __device__ __forceinline__ Piece piece_of(const Piece* table, const Rows& g, int number, int size) {
-  if (!table) return {0, number * size, max(0, min(size, g.T - number * size))};
+  if (!table) return {0, number * size, max(0, min(size, g.T - number * size)), 0};
   return table[number];
 }
 int pieces(int64_t T, int64_t n, bool ordered, int size) {
@@ -514,6 +517,7 @@ struct Prepare {
   Rows rows;
   int32_t *perm, *start;
   int order_groups;  // n + 1, or 0: the order is not needed
+  bool packed;
   struct Pieces {
     Piece* table;
     int size;
@@ -592,7 +596,7 @@ __device__ __forceinline__ void order_rows(const Prepare& p, int i) {
     const int end = i < n ? first_piece(at, i + 1, size) : p.rows.T / size + min(n, p.rows.T);
     for (int q = first + threadIdx.x; q < end; q += kPrepare) {
       const int from = begin + (q - first) * size;
-      p.pieces[k].table[q] = {i, from, i < n ? max(0, min(size, at - from)) : 0};
+      p.pieces[k].table[q] = {i, from, i < n ? max(0, min(size, at - from)) : 0, p.packed ? packed_slot(i, begin) : i};
     }
   }
 }
@@ -617,7 +621,7 @@ __device__ __forceinline__ void copy_straight(const Copy& c, int part) {
 
 // One 64 x 64 tile of a copy, read along the source's memory and written along the destination's, 16 bytes a thread.
 template <class T>
-__device__ __forceinline__ void copy_tile(const Copy& c, int m, int tile) {
+__device__ __forceinline__ void copy_tile(const Copy& c, int m, int slot, int tile) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
   constexpr int E = M::kE, kAcross = kCopyTile / E, kChunks = kCopyTile * kAcross;
@@ -625,7 +629,7 @@ __device__ __forceinline__ void copy_tile(const Copy& c, int m, int tile) {
   const int across = (c.ld + kCopyTile - 1) / kCopyTile;
   const int r0 = tile / across * kCopyTile, c0 = tile % across * kCopyTile;
   const T* src = (const T*)c.src.p + m * c.src.as;
-  T* dst = (T*)c.dst + (int64_t)m * c.rows * c.ld;
+  T* dst = (T*)c.dst + (int64_t)slot * c.rows * c.ld;
   const bool along = c.src.cs == 1;
   Frag v[kChunks / kPrepare];
 #pragma unroll
@@ -671,11 +675,13 @@ __device__ __forceinline__ void copy_tile(const Copy& c, int m, int tile) {
 
 // A workgroup's tiles of one matrix.  With more than a few adapters those that no row has are left out, as resident
 // adapters may be many more than a batch uses (500 of rank 16, 7 of them in use, 4096 x 4096: 149 -> 29 us for this
-// launch); beyond kScanRows rows looking for that would cost more than a tile's copy.
+// launch); beyond kScanRows rows looking for that would cost more than a tile's copy.  With more adapters than rows the
+// same look finds the layout's slot.
 constexpr int kScanAdapters = 8, kScanRows = 8192;
 template <class T>
-__device__ __forceinline__ void copy_tiles(const Copy& c, int part, const Rows& rows) {
+__device__ __forceinline__ void copy_tiles(const Copy& c, int part, const Rows& rows, bool packed) {
   const int parts = (c.tiles + c.per - 1) / c.per, m = part / parts, first = part % parts * c.per;
+  int slot = m;
   if (c.count > kScanAdapters && rows.T <= kScanRows) {
     constexpr int kLoads = kScanRows / (kPrepare * 4);  // all under way at once
     Four<int> id[kLoads];
@@ -692,10 +698,25 @@ __device__ __forceinline__ void copy_tiles(const Copy& c, int part, const Rows& 
 #pragma unroll
       for (int e = 0; e < 4; ++e) used |= id[q].v[e] == m;
     if (!__syncthreads_or(used)) return;
+    if (packed) {
+      __shared__ int below[kPrepare / 64];
+      int c = rest < rows.T && rows.index[rest] >= 0 && rows.index[rest] < m;  // rows of lower adapters
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c += id[q].v[e] >= 0 && id[q].v[e] < m;
+#pragma unroll
+      for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
+      if (threadIdx.x % 64 == 0) below[threadIdx.x / 64] = c;
+      __syncthreads();
+      int start = 0;
+      for (int w = 0; w < kPrepare / 64; ++w) start += below[w];
+      slot = packed_slot(m, start);
+    }
   }
   for (int tile = first; tile < min(c.tiles, first + c.per); ++tile) {
     if (tile != first) __syncthreads();
-    copy_tile<T>(c, m, tile);
+    copy_tile<T>(c, m, slot, tile);
   }
 }
 
@@ -713,7 +734,7 @@ __global__ __launch_bounds__(kPrepare) void prepare_kernel(Prepare p) {
   int k = p.copies - 1;
   while (k > 0 && b < p.copy[k].first) --k;
   if (p.copy[k].straight) copy_straight<T>(p.copy[k], b - p.copy[k].first);
-  else copy_tiles<T>(p.copy[k], b - p.copy[k].first, p.rows);
+  else copy_tiles<T>(p.copy[k], b - p.copy[k].first, p.rows, p.packed);
 }
 
 // low (place, rank) = U F_i, 32 places of one adapter by a workgroup, whose 8 waves cut the sum (16 waves were no
@@ -790,7 +811,7 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
     u[t] = (const T*)a.U + row_at(both.order, pc.begin + min(t * 16 + l16, pc.count - 1)) * a.ldu;
-  const Frag* f = (const Frag*)((const T*)a.F + (int64_t)pc.adapter * rp * a.ldf) + lane;
+  const Frag* f = (const Frag*)((const T*)a.F + (int64_t)pc.slot * rp * a.ldf) + lane;
   const int steps = (a.cu + M::kStep - 1) / M::kStep;
   const int shares = kWaves * a.splits, share = split * kWaves + wave;
   const int s0 = (int)((int64_t)steps * share / shares), s1 = (int)((int64_t)steps * (share + 1) / shares);
@@ -1142,7 +1163,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   unsigned wrong = 0;  // rows of this lane whose adapter does not exist
   {
     // this lane's rows, and their adapters
-    int row[TT], mine[TT];
+    int row[TT], mine[TT], slot[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) row[t] = (int)row_at(a.order, min(t0 + wt + t * kB + lb, a.rows.T - 1));
 #pragma unroll
@@ -1150,7 +1171,12 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
       mine[t] = adapter_of(a.rows, row[t]);
       if (t0 + wt + t * kB + lb >= a.rows.T) mine[t] = -1;
       wrong |= (unsigned)(mine[t] < -1 || mine[t] >= a.rows.n) << t;
+      slot[t] = mine[t];
     }
+    if (a.order.packed)
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+        if (mine[t] >= 0 && mine[t] < a.rows.n) slot[t] = packed_slot(mine[t], a.order.start[mine[t]]);
     // The accumulators begin with s_i (U F_i) G_i, while the first tiles load (SPLIT: each part of the sum with
     // some of the adapters and ranks).  U F_i comes as three values of the type (fp32: itself); the loads of kSets steps are under way at a time.  A row without this adapter loads its own
     // garbage, which reaches that row's accumulators alone, and these are set afterwards.
@@ -1164,17 +1190,19 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     auto x_of = [&](int t, int b) {
       const int at = t0 + wt + t * kB;
       const int64_t first = (int64_t)min(at / 32, (a.rows.T - 1) / 32) * (a.rp / 8) * kTerms<T>;
-      if constexpr (sizeof(T) == 2)
-        return b + g < slots ? ((const Frag*)a.split)[(first + b + g) * 32 + at % 32 + lb] : Frag{};
-      else return ((const Frag*)a.split)[(first + b) * 64 + lane];
+      if constexpr (sizeof(T) == 2) {
+        const Frag v = ((const Frag*)a.split)[(first + min(b + g, slots - 1)) * 32 + at % 32 + lb];
+        return b + g < slots ? v : Frag{};
+      } else return ((const Frag*)a.split)[(first + b) * 64 + lane];
     };
-    auto w_of = [&](int cur, int j, int b) {
+    auto w_of = [&](int slot, int j, int b) {
       const int n = n0 + wn + j * kB;
       const int64_t blocks = (a.N + 31) / 32, block = min((int64_t)n / 32, blocks - 1);
-      const int64_t first = (cur * blocks + block) * (a.rp / 8);
-      if constexpr (sizeof(T) == 2)
-        return b + g < slots ? ((const Frag*)a.G)[(first + (unsigned)(b + g) / kTerms<T>) * 32 + n % 32 + lb] : Frag{};
-      else return ((const Frag*)a.G)[(first + b) * 64 + lane];
+      const int64_t first = (slot * blocks + block) * (a.rp / 8);
+      if constexpr (sizeof(T) == 2) {
+        const Frag v = ((const Frag*)a.G)[(first + (unsigned)min(b + g, slots - 1) / kTerms<T>) * 32 + n % 32 + lb];
+        return b + g < slots ? v : Frag{};
+      } else return ((const Frag*)a.G)[(first + b) * 64 + lane];
     };
     auto factor = [&](int t, int cur) {
       float f = scale_of(a.rows, cur);
@@ -1184,11 +1212,14 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
     constexpr int kSets = (sizeof(T) == 2 ? 1 : 2) * (TT * TN * kB * kB <= 1024 ? 2 : 1);  // by the registers
     const int shares = SPLIT ? a.splits : 1, share = SPLIT ? blockIdx.y : 0;
     uint64_t some[TT], any = 0;
-    int first = -1;
+    int first = -1, first_slot = 0;
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       some[t] = __ballot(has(t));
-      if (some[t] && !any) first = __builtin_amdgcn_readlane(mine[t], __builtin_ctzll(some[t]));
+      if (some[t] && !any) {
+        first = __builtin_amdgcn_readlane(mine[t], __builtin_ctzll(some[t]));
+        first_slot = __builtin_amdgcn_readlane(slot[t], __builtin_ctzll(some[t]));
+      }
       any |= some[t];
     }
     bool one = true;
@@ -1202,7 +1233,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
 #pragma unroll
         for (int t = 0; t < TT; ++t) x[q][t] = x_of(t, b);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) w[q][j] = w_of(first, j, b);
+        for (int j = 0; j < TN; ++j) w[q][j] = w_of(first_slot, j, b);
       };
 #pragma unroll
       for (int q = 0; q < kSets; ++q) fetch(q, (share + q * shares) * kSlots);
@@ -1231,7 +1262,8 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
       for (int t = 0; t < TT; ++t) {
         uint64_t left = some[t];
         while (left) {
-          const int cur = __builtin_amdgcn_readlane(mine[t], __builtin_ctzll(left));
+          const int lead = __builtin_ctzll(left), cur = __builtin_amdgcn_readlane(mine[t], lead);
+          const int cur_slot = __builtin_amdgcn_readlane(slot[t], lead);
           left &= ~__ballot(mine[t] == cur);
           Acc d[TN] = {};
           for (int b = 0; b < slots; b += kSlots * kSets) {
@@ -1242,7 +1274,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
               if (b + q * kSlots >= slots) continue;
               x[q] = x_of(t, b + q * kSlots);
 #pragma unroll
-              for (int j = 0; j < TN; ++j) w[j][q] = w_of(cur, j, b + q * kSlots);
+              for (int j = 0; j < TN; ++j) w[j][q] = w_of(cur_slot, j, b + q * kSlots);
             }
 #pragma unroll
             for (int q = 0; q < kSets; ++q)
@@ -1363,8 +1395,8 @@ struct OuterPair {
 };
 // all of adapter i's rows as one piece
 __device__ __forceinline__ Piece whole_of(const Order& o, const Rows& g, int i) {
-  if (!o.start) return {0, 0, g.T};
-  return {i, o.start[i], o.start[i + 1] - o.start[i]};
+  if (!o.start) return {0, 0, g.T, 0};
+  return {i, o.start[i], o.start[i + 1] - o.start[i], 0};
 }
 
 template <class T, int RB, bool DIRECT>
@@ -1681,7 +1713,8 @@ struct Many {
       prep.perm = ws.template take<int32_t>(a.T);
       prep.start = ws.template take<int32_t>(a.n + 1);
       prep.order_groups = (int)a.n + 1;
-      order = {prep.perm, prep.start};
+      prep.packed = a.n > a.T && a.n > kScanAdapters && a.T <= kScanRows;
+      order = {prep.perm, prep.start, prep.packed};
       set_pieces(0, kLowRows);
     }
     groups = prep.order_groups;
@@ -1696,7 +1729,8 @@ struct Many {
     Copy& c = prep.copy[prep.copies++];
     const int64_t tiles = (int64_t)((rows + kCopyTile - 1) / kCopyTile) * ((ld + kCopyTile - 1) / kCopyTile);
     const int64_t per = std::clamp<int64_t>(count * tiles / 4096, 1, tiles);  // tiles of a workgroup: 16 of them a CU
-    c = {src, ws.template take<T>((int64_t)count * rows * ld), rows, cols, ld, count, have, order,
+    const int64_t slots = prep.packed ? std::min<int64_t>(count, a.T) : count;
+    c = {src, ws.template take<T>(slots * rows * ld), rows, cols, ld, count, have, order,
          order == kRows && src.cs == 1, (int)groups - prep.order_groups, (int)tiles, (int)per};
     groups += c.straight ? ((int64_t)count * rows * (ld / E) + kStraight - 1) / kStraight
                          : count * ((tiles + per - 1) / per);

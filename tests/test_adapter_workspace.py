@@ -58,3 +58,10 @@ def test_no_rows_need_the_same_with_and_without_an_index(gelim):
     """An index of no rows has no address, so the call cannot tell the two apart."""
     for grad in (False, True):
         assert need(grad, 0, 64, 48, 4, 2) == need(grad, 0, 64, 48, 4, 2, indexed=False)
+
+
+@pytest.mark.parametrize("T", [65, 200, 3000, 8192])
+def test_layouts_go_by_rows_not_by_resident_adapters(gelim, T):
+    """Beyond as many adapters as rows another one costs its entry of the order."""
+    for grad in (False, True):
+        assert need(grad, T, 1024, 2048, 64, T + 300) - need(grad, T, 1024, 2048, 64, T) <= 300 * 4 + 1024
