@@ -1379,9 +1379,9 @@ struct Outer {
   const void* U;
   int64_t ldu;
   const float* low;  // V
-  float* part;       // piece, rank, column
+  float* part;       // part, rank, column
   int cu, ldp, blocks;
-  // DIRECT, with at most one piece an adapter: the gradient itself, at adapter as + column cs + rank rs
+  // for adapters of one piece: the gradient itself, at adapter as + column cs + rank rs
   void* out;
   int64_t as, cs, rs;
   int cols;
@@ -1393,13 +1393,19 @@ struct OuterPair {
   const Piece* table;
   int rp, pieces, size, r;
 };
+// Adapters of one piece write their gradients at once, the others parts that are added up.  Such an adapter i has more
+// than `size` rows, so its parts have the numbers from start / size + min(i, start / size) on, as its pieces have theirs:
+// no more than T / size + min(n, T / size).
+__device__ __forceinline__ int first_part(int start, int i, int size) { return start / size + min(i, start / size); }
+int parts_of(int64_t T, int64_t n, int size) { return (int)(T / size + std::min(n, std::max<int64_t>(1, T / size))); }
 // all of adapter i's rows as one piece
 __device__ __forceinline__ Piece whole_of(const Order& o, const Rows& g, int i) {
   if (!o.start) return {0, 0, g.T, 0};
   return {i, o.start[i], o.start[i + 1] - o.start[i], 0};
 }
 
-template <class T, int RB, bool DIRECT>
+// BY_ADAPTER: with at most `size` rows a piece for each adapter, also for those without rows, whose gradients are zeros
+template <class T, int RB, bool BY_ADAPTER>
 __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
@@ -1410,8 +1416,10 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   const Outer& a = both.p[blockIdx.y];
   const int piece = blockIdx.x % both.pieces, block = blockIdx.x / both.pieces;
   if (block >= a.blocks) return;
-  const Piece pc = DIRECT ? whole_of(both.order, both.rows, piece) : piece_of(both.table, both.rows, piece, both.size);
-  if (!DIRECT && pc.count == 0) return;
+  const Piece pc =
+      BY_ADAPTER ? whole_of(both.order, both.rows, piece) : piece_of(both.table, both.rows, piece, both.size);
+  if (!BY_ADAPTER && pc.count == 0) return;
+  const Piece all = whole_of(both.order, both.rows, pc.adapter);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l16 = lane % 16, g = lane / 16;
   const int j0 = blockIdx.z * kRanks;
   if (threadIdx.x < kGradRows)
@@ -1491,7 +1499,7 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
     if (s * M::kStep >= pc.count) break;
     fetch(s);
   }
-  if constexpr (DIRECT) {
+  if (BY_ADAPTER || all.count <= both.size) {
     // an adapter without rows gets zeros, whatever its factor holds
     const float f = pc.count ? scale_of(both.rows, pc.adapter) * back : 0.f;
 #pragma unroll
@@ -1516,7 +1524,8 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   }
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    float* out = a.part + ((int64_t)piece * both.rp + j0 + b * 16 + l16) * a.ldp + n0;
+    const int part = first_part(all.begin, pc.adapter, both.size) + (pc.begin - all.begin) / both.size;
+    float* out = a.part + ((int64_t)part * both.rp + j0 + b * 16 + l16) * a.ldp + n0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1526,7 +1535,7 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   }
 }
 
-// Last their sums, times s_i, in the factor's layout: 64 columns of one adapter by a workgroup, whose four waves share
+// Last the sums of the parts, times s_i, in the factor's layout, and zeros for adapters without rows: 64 columns of one adapter by a workgroup, whose four waves share
 // the pieces of 4 ranks or, where the adapters have few pieces, take 4 ranks each.
 struct Sum {
   const float* part;
@@ -1550,9 +1559,10 @@ __global__ __launch_bounds__(256) void sum_kernel(SumPair both) {
   const int groups = (both.r + kRanks - 1) / kRanks, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int c = blockIdx.x / groups * 64 + lane, j0 = blockIdx.x % groups * kRanks + (SHARE ? 0 : wave * 4);
   for (int i = blockIdx.z; i < both.rows.n; i += gridDim.z) {
-    const int count = both.order.start ? both.order.start[i + 1] - both.order.start[i] : both.rows.T;
-    const int first = both.order.start ? first_piece(both.order.start[i], i, both.size) : 0;
-    const int many = (count + both.size - 1) / both.size;
+    const Piece all = whole_of(both.order, both.rows, i);
+    const int count = all.count, many = (count + both.size - 1) / both.size;
+    if (many == 1) continue;  // written already
+    const int first = first_part(all.begin, i, both.size);
     f4 s = {0.f, 0.f, 0.f, 0.f};
     if (j0 < both.rp)
 #pragma unroll 4
@@ -1954,7 +1964,7 @@ int gradient(const gelim_adapter_args& a, Space& ws, hipStream_t s, bool run) {
     o.U = U.p, o.low = low[k].low, o.ldu = U.ld, o.cu = U.cols;
     o.blocks = (U.cols + 64 * Mma<T>::kE - 1) / (64 * Mma<T>::kE);
     o.ldp = (int)up(U.cols, 16 * Mma<T>::kE);
-    if (!direct) o.part = ws.take<float>((int64_t)pcs * m.rp * o.ldp);
+    if (!direct) o.part = ws.take<float>((int64_t)parts_of(a.T, a.n, size) * m.rp * o.ldp);
     u.part = o.part, u.out = k ? a.dB : a.dA, u.cols = cols, u.ldp = o.ldp;
     u.as = (int64_t)a.r * cols;
     const bool along = k ? !a.b_trans : a.a_trans;  // columns side by side

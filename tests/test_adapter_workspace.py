@@ -65,3 +65,12 @@ def test_layouts_go_by_rows_not_by_resident_adapters(gelim, T):
     """Beyond as many adapters as rows another one costs its entry of the order."""
     for grad in (False, True):
         assert need(grad, T, 1024, 2048, 64, T + 300) - need(grad, T, 1024, 2048, 64, T) <= 300 * 4 + 1024
+
+
+@pytest.mark.parametrize("T, r, padded", [(200, 64, 64), (1000, 8, 16), (4000, 33, 64)])
+def test_parts_are_those_of_adapters_with_several_pieces(gelim, T, r, padded):
+    """Rows in pieces of 32 at least: adapters of more than one piece have no more than twice T / 32 together.  Beside
+    those the layouts with their ranks padded, dX's parts and per row the low-rank sums."""
+    K, N, n = 8192, 4096, 500
+    layouts, parts = min(n, T) * padded * (2 * K + N) * 2, 2 * (T // 32) * padded * (K + N) * 4
+    assert need(True, T, K, N, r, n) <= layouts + parts + 16 * T * K * 4 + T * 8192
