@@ -10,3 +10,33 @@ The reference's MPI programs are started as `mpirun -np P ./gauss_*_input`
 
 Single-GPU programs are native executables under bin/ (csrc/tools).
 """
+from __future__ import annotations
+
+import contextlib
+import os
+import sys
+
+
+@contextlib.contextmanager
+def library_reports_to_stderr():
+    """What libraries print on descriptor 1 meanwhile goes to stderr.
+
+    gloo reports its connections there, from C++ and in pieces that mix with
+    the other ranks', which would break up the lines of these programs.  For a
+    program that owns its process, while it has no other thread that prints;
+    without an effect where stdout or stderr is closed or something else's."""
+    try:
+        own = sys.stdout.fileno() == 1 and sys.stderr.fileno() == 2
+    except (AttributeError, OSError, ValueError):
+        own = False
+    if not own:
+        yield
+        return
+    sys.stdout.flush()
+    keep = os.dup(1)
+    os.dup2(2, 1)
+    try:
+        yield
+    finally:
+        os.dup2(keep, 1)
+        os.close(keep)

@@ -33,6 +33,7 @@ the elimination at panel boundaries (utils/checkpoint.py).
 from __future__ import annotations
 
 import argparse
+import contextlib
 import sys
 import time
 
@@ -45,6 +46,7 @@ from ..parallel import comm as C
 from ..parallel.dist_gauss import DistributedGauss
 from ..utils import io
 from ..utils.report import json_line
+from . import library_reports_to_stderr
 
 
 def parse(argv=None):
@@ -122,14 +124,16 @@ def make_solver(args, comm, n: int):
     return dg, (lambda: synthetic_local(dg)), dg.layout.D
 
 
-def main(argv=None) -> int:
+def main(argv=None, joining=contextlib.nullcontext) -> int:
+    """joining: a context for the time in which the ranks join."""
     args = parse(argv)
     if args.emulate and args.emulate > 1:
         from ..parallel.emulated import run_emulated
 
         dev = args.device or ("cuda:0" if torch.cuda.is_available() else "cpu")
         return max(run_emulated(args.emulate, lambda comm: run(args, comm), device=dev))
-    comm = C.init_from_env(device=args.device)
+    with joining():
+        comm = C.init_from_env(device=args.device)
     ok = False
     try:
         rc = run(args, comm)
@@ -211,4 +215,4 @@ def run(args, comm) -> int:
 
 
 if __name__ == "__main__":
-    sys.exit(main())
+    sys.exit(main(joining=library_reports_to_stderr))

@@ -12,6 +12,7 @@ Prints `GPU Time: <s>` (rank 0, max over ranks) like the reference.
 from __future__ import annotations
 
 import argparse
+import contextlib
 import sys
 import time
 
@@ -21,6 +22,7 @@ from ..ops.matmul import reference_inputs
 from ..parallel import comm as C
 from ..parallel.dist_matmul import allgather_matmul, grid_shape, make_summa_groups, ring_matmul, summa_matmul
 from ..utils.report import json_line
+from . import library_reports_to_stderr
 
 
 def parse(argv=None):
@@ -34,9 +36,11 @@ def parse(argv=None):
     return p.parse_args(argv)
 
 
-def main(argv=None) -> int:
+def main(argv=None, joining=contextlib.nullcontext) -> int:
+    """joining: a context for the time in which the ranks join."""
     args = parse(argv)
-    comm = C.init_from_env(device=args.device)
+    with joining():
+        comm = C.init_from_env(device=args.device)
     dev, P, r, n = comm.device, comm.world_size, comm.rank, args.size
     ok = False
     try:
@@ -101,4 +105,4 @@ def main(argv=None) -> int:
 
 
 if __name__ == "__main__":
-    sys.exit(main())
+    sys.exit(main(joining=library_reports_to_stderr))

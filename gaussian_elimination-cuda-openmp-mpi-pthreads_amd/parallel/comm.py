@@ -17,11 +17,9 @@ resolve).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import datetime
 import os
-import sys
 import threading
 import time
 from dataclasses import dataclass, field
@@ -655,20 +653,6 @@ def env_world() -> tuple[int, int, int]:
             int(os.environ.get("LOCAL_RANK", 0)))
 
 
-@contextlib.contextmanager
-def _stdout_to_stderr():
-    """gloo reports its connections on stdout from C++, in pieces that mix with
-    the other ranks': they would break up what the programs print there."""
-    sys.stdout.flush()
-    keep = os.dup(1)
-    os.dup2(2, 1)
-    try:
-        yield
-    finally:
-        os.dup2(keep, 1)
-        os.close(keep)
-
-
 def init_from_env(backend: str | None = None, device: str | None = None,
                   timeout_s: float = 600.0, force_pg: bool | None = None) -> Communicator:
     """Join the job described by RANK/WORLD_SIZE/LOCAL_RANK/MASTER_* (torchrun).
@@ -722,10 +706,7 @@ def init_from_env(backend: str | None = None, device: str | None = None,
         kw = dict(backend=backend, rank=rank, world_size=world, timeout=datetime.timedelta(seconds=timeout_s))
         if backend == "nccl":
             kw["device_id"] = dev
-            dist.init_process_group(**kw)
-        else:
-            with _stdout_to_stderr():
-                dist.init_process_group(**kw)
+        dist.init_process_group(**kw)
     return Communicator(rank, world, dev, backend)
 
 
