@@ -87,7 +87,8 @@ def _check(X, W, A, B, index, scale):
             raise TypeError("scale must be a number or float32")
         if scale.shape != (n,) or scale.get_device() != at:
             raise ValueError("scale must have one entry per adapter, on the device of X")
-    if torch.is_grad_enabled() and (X.requires_grad or W.requires_grad or A.requires_grad or B.requires_grad):
+    if torch.is_grad_enabled() and (X.requires_grad or W.requires_grad or A.requires_grad or B.requires_grad or
+                                    isinstance(scale, torch.Tensor) and scale.requires_grad):
         raise ValueError("adapter_matmul is not recorded by autograd: call it under torch.no_grad() and take the "
                          "gradients from adapter_matmul_grad")
     return dev, T, K, N, n, r

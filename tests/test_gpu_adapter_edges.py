@@ -156,3 +156,15 @@ def test_pieces_of_many_adapters(gelim, cuda, T, n, used, dtype):
     dY = torch.randn(T, N, generator=g).to(dtype).to(cuda)
     for v, t in zip(gelim.ops.adapter_matmul_grad(dY, *args), ref_grad(dY, *args, device=cuda)):
         check(v, *t)
+
+
+def test_a_scale_that_requires_gradients_is_refused(gelim, cuda):
+    X, W, A, B = (torch.randn(s, device=cuda).bfloat16() for s in ((6, 32), (32, 40), (2, 32, 4), (2, 4, 40)))
+    index, scale = torch.zeros(6, dtype=torch.int32, device=cuda), torch.ones(2, device=cuda, requires_grad=True)
+    with pytest.raises(ValueError, match="autograd"):
+        gelim.ops.adapter_matmul(X, W, A, B, index, scale)
+    with pytest.raises(ValueError, match="autograd"):
+        gelim.ops.adapter_matmul_grad(torch.zeros(6, 40, device=cuda).bfloat16(), X, W, A, B, index, scale)
+    with torch.no_grad():
+        Y = gelim.ops.adapter_matmul(X, W, A, B, index, scale)
+    assert torch.equal(Y, gelim.ops.adapter_matmul(X, W, A, B, index, scale.detach()))
