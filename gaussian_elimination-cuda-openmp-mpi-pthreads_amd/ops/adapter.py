@@ -18,7 +18,7 @@ from functools import lru_cache
 import torch
 
 from .. import _native
-from ..utils.tensors import stream_handle
+from ..utils.tensors import has_tangent, stream_handle
 
 MAX_RANK = 256
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -54,7 +54,7 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
-def _check(X, W, A, B, index, scale):
+def _check(X, W, A, B, index, scale, more=()):
     # called for single tokens as well, so short of anything that takes a microsecond
     dtype = X.dtype
     if dtype not in TYPES:
@@ -91,6 +91,8 @@ def _check(X, W, A, B, index, scale):
                                     isinstance(scale, torch.Tensor) and scale.requires_grad):
         raise ValueError("adapter_matmul is not recorded by autograd: call it under torch.no_grad() and take the "
                          "gradients from adapter_matmul_grad")
+    if has_tangent(t for t in (X, W, A, B, scale, *more) if isinstance(t, torch.Tensor)):
+        raise ValueError("adapter_matmul is not followed by forward-mode differentiation: it would drop the tangents")
     return dev, T, K, N, n, r
 
 
@@ -158,7 +160,7 @@ def adapter_matmul(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.T
     out: (T, N) with unit column stride; no input begins or ends between its
     first and last element.
     Runs on the current stream; may be captured into a graph."""
-    dev, T, K, N, n, r = _check(X, W, A, B, index, scale)
+    dev, T, K, N, n, r = _check(X, W, A, B, index, scale, (out,))
     if out is None:
         out = X.new_empty((T, N))
     else:
@@ -186,7 +188,7 @@ def adapter_matmul_grad(dY: torch.Tensor, X: torch.Tensor, W: torch.Tensor, A: t
     the shapes of A and B, stored as those are (row-major, or transposed);
     an adapter without rows gets zeros.  Rows without an adapter (-1) add
     nothing to dA and dB; rows with an index outside [-1, n) have a NaN dX."""
-    dev, T, K, N, n, r = _check(X, W, A, B, index, scale)
+    dev, T, K, N, n, r = _check(X, W, A, B, index, scale, (dY,))
     if dY.dtype != X.dtype:
         raise TypeError("dY must have the type of X")
     if dY.shape != (T, N) or dY.device != dev:

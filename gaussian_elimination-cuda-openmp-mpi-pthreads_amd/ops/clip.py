@@ -8,7 +8,7 @@ from typing import Sequence
 import torch
 
 from .. import _native
-from ..utils.tensors import stream_handle
+from ..utils.tensors import has_tangent, stream_handle
 from .adapter import TYPES
 
 
@@ -60,7 +60,8 @@ def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
     max_norm = math.inf only measures.  As the factor comes from the norm, a NaN anywhere
     makes all of them NaN, and an infinity makes the finite elements zero.
     Squares and their sum are held in float64, in an order that does not change
-    from run to run.  Autograd records nothing.  May be captured into a graph."""
+    from run to run.  Autograd records nothing; tensors with forward-mode tangents
+    are refused.  May be captured into a graph."""
     tensors = list(tensors)
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
@@ -84,6 +85,8 @@ def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
             if any(o.shape != t.shape or o.stride() != t.stride() for t, o in zip(tensors, out)):
                 raise ValueError("each out must have the strides of its input")
         dst = array("Q", map(_PTR, out))
+    if has_tangent(tensors if out is None else [*tensors, *out]):
+        raise ValueError("clip_global_norm is not followed by forward-mode differentiation: it would drop the tangents")
     norm = torch.empty((), dtype=torch.float32, device=dev)
     lib = _native.lib()
     ws = torch.empty(lib.gelim_clip_workspace(len(tensors)), dtype=torch.uint8, device=dev)

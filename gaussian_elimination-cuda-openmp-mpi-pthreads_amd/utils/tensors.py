@@ -2,7 +2,10 @@
 leading dimensions and the HIP stream handle of the current torch stream."""
 from __future__ import annotations
 
+from typing import Iterable
+
 import torch
+from torch.autograd import forward_ad
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -23,6 +26,12 @@ def stream_handle(device: torch.device | None = None) -> int | None:
         return None
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     return torch._C._cuda_getCurrentRawStream(index)  # 2 us less than by way of a Stream object
+
+
+def has_tangent(tensors: Iterable[torch.Tensor]) -> bool:
+    """Whether one of them carries a forward-mode tangent, which a native kernel would drop.  (requires_grad does not
+    say so, and torch.no_grad() does not end it.)"""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 _DEDICATED: dict[tuple[int, str], torch.cuda.ExternalStream] = {}

@@ -168,3 +168,30 @@ def test_a_scale_that_requires_gradients_is_refused(gelim, cuda):
     with torch.no_grad():
         Y = gelim.ops.adapter_matmul(X, W, A, B, index, scale)
     assert torch.equal(Y, gelim.ops.adapter_matmul(X, W, A, B, index, scale.detach()))
+
+
+def test_forward_mode_tangents_are_refused(gelim, cuda):
+    from torch.autograd import forward_ad
+
+    X, W, A, B = (torch.randn(s, device=cuda).bfloat16() for s in ((6, 32), (32, 40), (1, 32, 4), (1, 4, 40)))
+    dY, scale = torch.zeros(6, 40, device=cuda).bfloat16(), torch.ones(1, device=cuda)
+    want = gelim.ops.adapter_matmul(X, W, A, B, scale=scale)
+    with forward_ad.dual_level(), torch.no_grad():
+        for k in range(5):
+            args = [X, W, A, B, None, scale]
+            k += k == 4
+            args[k] = forward_ad.make_dual(args[k], torch.ones_like(args[k]))
+            with pytest.raises(ValueError, match="forward-mode"):
+                gelim.ops.adapter_matmul(*args)
+            with pytest.raises(ValueError, match="forward-mode"):
+                gelim.ops.adapter_matmul_grad(dY, *args)
+            with pytest.raises(ValueError, match="forward-mode"):
+                gelim.ops.clip_global_norm([A.clone(), args[k]], 1.0)
+        dual = forward_ad.make_dual(dY, torch.ones_like(dY))
+        with pytest.raises(ValueError, match="forward-mode"):
+            gelim.ops.adapter_matmul_grad(dual, X, W, A, B)
+        with pytest.raises(ValueError, match="forward-mode"):
+            gelim.ops.adapter_matmul(X, W, A, B, out=dual)
+        with pytest.raises(ValueError, match="forward-mode"):
+            gelim.ops.clip_global_norm([A], 1.0, out=[forward_ad.make_dual(A.clone(), A.clone())])
+        assert torch.equal(gelim.ops.adapter_matmul(X, W, A, B, scale=scale), want)  # others may be duals meanwhile
