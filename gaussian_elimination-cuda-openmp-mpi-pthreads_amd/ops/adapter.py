@@ -16,6 +16,7 @@ import struct
 from functools import lru_cache
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _native
 from ..utils.tensors import has_tangent, stream_handle
@@ -161,7 +162,8 @@ def adapter_matmul(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.T
     first and last element.
     Runs on the current stream; may be captured into a graph."""
     dev, T, K, N, n, r = _check(X, W, A, B, index, scale, (out,))
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = X.new_empty((T, N))
     else:
         if out.dtype != X.dtype or out.device != dev:
@@ -174,6 +176,8 @@ def adapter_matmul(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.T
             raise ValueError("out overlaps an input")
     if T:
         _call(False, dev, T, K, N, n, r, X, W, A, B, index, scale, out)
+        if not fresh:
+            increment_version(out)  # it may have been saved for a backward pass
     return out
 
 

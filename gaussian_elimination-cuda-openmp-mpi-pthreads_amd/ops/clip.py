@@ -6,6 +6,7 @@ from array import array
 from typing import Sequence
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _native
 from ..utils.tensors import has_tangent, stream_handle
@@ -60,7 +61,8 @@ def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
     max_norm = math.inf only measures.  As the factor comes from the norm, a NaN anywhere
     makes all of them NaN, and an infinity makes the finite elements zero.
     Squares and their sum are held in float64, in an order that does not change
-    from run to run.  Autograd records nothing; tensors with forward-mode tangents
+    from run to run.  Autograd records nothing, as under torch.no_grad(), and
+    sees that what is written has changed; tensors with forward-mode tangents
     are refused.  May be captured into a graph."""
     tensors = list(tensors)
     max_norm = float(max_norm)
@@ -101,4 +103,6 @@ def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
     else:
         with torch.cuda.device(dev):
             call()
+    if out is not None or max_norm != math.inf:
+        increment_version(tensors if out is None else out)  # they may have been saved for a backward pass
     return norm

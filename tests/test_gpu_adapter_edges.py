@@ -195,3 +195,34 @@ def test_forward_mode_tangents_are_refused(gelim, cuda):
         with pytest.raises(ValueError, match="forward-mode"):
             gelim.ops.clip_global_norm([A], 1.0, out=[forward_ad.make_dual(A.clone(), A.clone())])
         assert torch.equal(gelim.ops.adapter_matmul(X, W, A, B, scale=scale), want)  # others may be duals meanwhile
+
+
+def test_autograd_sees_what_is_written(gelim, cuda):
+    """A tensor saved for a backward pass and then written by a call: the backward pass must not go on with the new
+    values, as after any in-place operation."""
+    X, W, A, B = (torch.randn(s, device=cuda) for s in ((70, 32), (32, 40), (1, 32, 4), (1, 4, 40)))
+
+    def saved():
+        y = torch.randn(70, 40, device=cuda)
+        p = torch.ones(70, 40, device=cuda, requires_grad=True)
+        return y, (p * y).sum()
+
+    y, loss = saved()
+    gelim.ops.adapter_matmul(X, W, A, B, out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    for apart in (False, True):
+        y, loss = saved()
+        gelim.ops.clip_global_norm([X.clone(), W.clone() if apart else y], 1e-3,
+                                   out=[torch.empty_like(X), y[:32]] if apart else None)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    y, loss = saved()
+    gelim.ops.clip_global_norm([y], math.inf)  # only measures
+    gelim.ops.clip_global_norm([y], 1.0, out=[torch.empty_like(y)])
+    gelim.ops.adapter_matmul(X, W, A, B)
+    loss.backward()
+    with torch.inference_mode():  # such tensors have no version
+        y = torch.randn(70, 40, device=cuda)
+        gelim.ops.clip_global_norm([y], 1.0)
+        gelim.ops.adapter_matmul(X, W, A, B, out=y)
