@@ -25,7 +25,7 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-_PTR, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.numel
+_PTR, _NUMEL, _SAME_SIZE = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_same_size
 _DTYPE = torch.Tensor.dtype.__get__
 
 
@@ -81,10 +81,10 @@ def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
         dst = src
     else:
         out = list(out)
-        if len(out) != len(tensors) or _types(out) != types or array("q", map(_NUMEL, out)) != sizes:
+        if len(out) != len(tensors) or _types(out) != types or not all(map(_SAME_SIZE, out, tensors)):
             raise ValueError("out must have one tensor of the same type and shape per input")
         if not (_check_memory(out, dev) and contiguous):
-            if any(o.shape != t.shape or o.stride() != t.stride() for t, o in zip(tensors, out)):
+            if any(o.stride() != t.stride() for t, o in zip(tensors, out)):
                 raise ValueError("each out must have the strides of its input")
         dst = array("Q", map(_PTR, out))
     if has_tangent(tensors if out is None else [*tensors, *out]):

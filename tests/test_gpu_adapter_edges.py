@@ -226,3 +226,14 @@ def test_autograd_sees_what_is_written(gelim, cuda):
         y = torch.randn(70, 40, device=cuda)
         gelim.ops.clip_global_norm([y], 1.0)
         gelim.ops.adapter_matmul(X, W, A, B, out=y)
+
+
+def test_clipped_copies_have_their_inputs_shapes(gelim, cuda):
+    a, b = torch.ones(2, 3, device=cuda), torch.ones(4, device=cuda)
+    for out in ([torch.empty(3, 2, device=cuda), torch.empty_like(b)], [torch.empty(6, device=cuda), torch.empty_like(b)],
+                [torch.empty_like(a), torch.empty(2, 2, device=cuda)], [torch.empty_like(b), torch.empty_like(a)]):
+        with pytest.raises(ValueError, match="same type and shape"):
+            gelim.ops.clip_global_norm([a, b], 1.0, out=out)
+    out = [torch.empty_like(a), torch.empty_like(b)]
+    gelim.ops.clip_global_norm([a, b], 1.0, out=out)
+    assert torch.equal(out[0].flatten()[:4], out[1])
