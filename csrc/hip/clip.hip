@@ -113,6 +113,13 @@ __global__ __launch_bounds__(kThreads) void squares_kernel(const Table<false> tb
   if (threadIdx.x == 0) slots[blockIdx.x] = fresh ? s : slots[blockIdx.x] + s;
 }
 
+// v f, rounded to fp32: left to itself the compiler may round some of the products straight to fp16, by place
+__device__ __forceinline__ float times(float v, float f) {
+  float r = v * f;
+  asm("" : "+v"(r));
+  return r;
+}
+
 template <class T>
 __device__ __forceinline__ void scaled(const T* p, T* q, int len, float f) {
   constexpr int L = Pack<T>::kLen;
@@ -121,10 +128,10 @@ __device__ __forceinline__ void scaled(const T* p, T* q, int len, float f) {
   for (; e + L <= len; e += kThreads * L) {
     typename Pack<T>::Mem m = *(const typename Pack<T>::Mem*)(p + e);
 #pragma unroll
-    for (int i = 0; i < L; ++i) m.v[i] = (T)((float)m.v[i] * f);
+    for (int i = 0; i < L; ++i) m.v[i] = (T)times((float)m.v[i], f);
     *(typename Pack<T>::Mem*)(q + e) = m;
   }
-  for (; e < len; ++e) q[e] = (T)((float)p[e] * f);
+  for (; e < len; ++e) q[e] = (T)times((float)p[e], f);
 }
 
 template <bool APART>

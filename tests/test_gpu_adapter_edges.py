@@ -237,3 +237,17 @@ def test_clipped_copies_have_their_inputs_shapes(gelim, cuda):
     out = [torch.empty_like(a), torch.empty_like(b)]
     gelim.ops.clip_global_norm([a, b], 1.0, out=out)
     assert torch.equal(out[0].flatten()[:4], out[1])
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("max_norm", [26.69, 19.71, 21.25, 39.42, 30.23, 36.77])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_clipping_rounds_alike_at_every_place(gelim, cuda, dtype, max_norm, apart):
+    """Equal values have equal results, whether they stand in a whole pack of 16 bytes or at a tensor's end.  These norms
+    have factors for which 8 to 12 of the products in fp16 depend on whether they are rounded to fp32 before."""
+    v = torch.randn(4096, generator=torch.Generator().manual_seed(3)).to(dtype).to(cuda)
+    small = [torch.cat([v[:8], v[k:k + 1]]) for k in range(v.numel())]
+    tensors = [v.clone()] + small
+    out = [torch.empty_like(t) for t in tensors] if apart else tensors
+    gelim.ops.clip_global_norm(tensors, max_norm, out=out if apart else None)
+    assert torch.equal(torch.stack([o[8] for o in out[1:]]), out[0])
