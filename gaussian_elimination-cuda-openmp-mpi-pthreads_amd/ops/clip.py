@@ -51,7 +51,7 @@ def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
                      out: Sequence[torch.Tensor] | None = None) -> torch.Tensor:
     """Scales all tensors by min(1, max_norm / (norm + 1e-6)), norm the 2-norm of
     all their elements together, and returns that norm (a float32 scalar on
-    the device, nothing waits for it).
+    the device, infinite where it leaves that type; nothing waits for it).
 
     tensors: float32, bfloat16 and float16 in any mixture, on one device, each
     without gaps in memory (any order of dimensions).

@@ -251,3 +251,25 @@ def test_clipping_rounds_alike_at_every_place(gelim, cuda, dtype, max_norm, apar
     out = [torch.empty_like(t) for t in tensors] if apart else tensors
     gelim.ops.clip_global_norm(tensors, max_norm, out=out if apart else None)
     assert torch.equal(torch.stack([o[8] for o in out[1:]]), out[0])
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_factor_below_the_normal_numbers(gelim, cuda, dtype, apart):
+    """Norms so large that max_norm / norm is subnormal in fp32: the results are normal all the same and have the
+    accuracy that the others have.  Tolerance: the rounding of the factor and of the product to fp32 and of the result to
+    its type (2^-24 each and eps / 2), and half a step of the subnormal numbers of fp32, 2^-150, and of the type."""
+    g = torch.Generator().manual_seed(7)
+    for size, max_norm in ((1e38, 1e-3), (3e37, 1e-7), (1e30, 1e-14), (1e38, 1e-12)):
+        a = (torch.rand(4000, generator=g) + 0.5).mul(size).to(dtype).to(cuda)
+        a[1], a[2] = 2.0 ** -3 * a[1], 1.0
+        norm = math.sqrt(math.fsum(a.double().square().tolist()))
+        f = max_norm / (norm + 1e-6)
+        assert f < 2.0 ** -126
+        out = torch.empty_like(a) if apart else a.clone()
+        src = a if apart else out
+        gelim.ops.clip_global_norm([src], max_norm, out=[out] if apart else None)
+        want = a.double() * f
+        tol = (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * want.abs() + 2.0 ** -150
+        tol += torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+        assert ((out.double() - want).abs() <= tol).all()
