@@ -178,12 +178,10 @@ __device__ __forceinline__ float scale_of(const Rows& g, int i) { return g.scale
 struct Few {
   const void* U;
   int64_t ldu;
-  View W, F, G;
+  View W, F;
   Rows rows;
   float *part, *low;  // part: splits x T x ldp, low: low_splits x T x r
   int C, N, r, ldp, splits, blocks, low_splits;
-  void* Y;
-  int64_t ldy;
 };
 
 // The first of the kE columns that a lane takes where W's rows run along memory: at the end of a row the lane takes
@@ -960,7 +958,7 @@ struct Big {
   int cu, cw;  // values of a row of U / of the sum in W that exist (W_KC: multiples of 16 bytes); zeros behind
   Rows rows;
   Order order;
-  const float *low, *by;
+  const float* by;
   const void* split;
   int N, nw, r, rp, splits, tiles_t, tiles_n;  // nw: columns of W as stored
   void* Y;
@@ -993,7 +991,7 @@ __device__ __forceinline__ int swap_columns(int k) {  // in chunks
   else return (k >> 2 & 1) * 8 % kRowChunks;
 }
 
-// WT x WN waves share a tile in blocks of 32 x 32.  S tiles in
+// WT x WN waves share a tile in blocks of 16 x 16 (fp32: 32 x 32).  S tiles in
 // LDS and two sets of fragments in registers: while one quarter of a tile is
 // multiplied the next is read; when the last quarter is in registers the
 // tile's place is loaded again, S - 1 tiles' time before the barrier that waits for it.
@@ -1256,7 +1254,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
           for (int r = 0; r < kAcc; ++r) acc[j][t][r] = has(t) ? f * acc[j][t][r] : 0.f;
       }
     } else if (any) {
-      // for each adapter among 32 rows the product of all of them, kept where it is theirs
+      // for each adapter among a block's rows the product of all of them, kept where it is theirs
       int unit = shares - share;
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
@@ -1671,7 +1669,7 @@ template <class T>
 int few_product(const Problem& p, const Rows& g, int r, Space& ws, hipStream_t s, bool run) {
   using M = Mma<T>;
   Few f{};
-  f.U = p.U, f.ldu = p.ldu, f.W = p.W, f.F = p.F, f.G = p.G, f.rows = g, f.C = p.C, f.N = p.N, f.r = r;
+  f.U = p.U, f.ldu = p.ldu, f.W = p.W, f.F = p.F, f.rows = g, f.C = p.C, f.N = p.N, f.r = r;
   f.blocks = (int)((p.N + 16 * M::kE - 1) / (16 * M::kE));
   const int steps = (p.C + M::kStep - 1) / M::kStep;
   // workgroups: one a CU, as more cost the second launch what they save (32 rows of bf16 4096 x 4096: 16.2 us
@@ -1890,7 +1888,7 @@ struct Many {
   }
   void run_big(Plan& q, const Low& l, hipStream_t s) {
     Big& b = q.b;
-    b.low = l.low, b.by = l.by, b.split = l.split;
+    b.by = l.by, b.split = l.split;
     auto shape = [&](auto kc) {
       constexpr bool KC = decltype(kc)::value;
       if (q.bt == 64) launch<KC, 64, 64, 2, 2, 4>(b, s);

@@ -248,13 +248,13 @@ int clip(const void* const* in, void* const* out, const int64_t* sizes, const in
 }  // namespace
 }  // namespace gelim
 
-extern "C" int64_t gelim_clip_workspace(int64_t) { return gelim::kSlots * (int64_t)sizeof(double); }
+extern "C" int64_t gelim_clip_workspace(void) { return gelim::kSlots * (int64_t)sizeof(double); }
 
 extern "C" int gelim_clip_norm(const void* const* in, void* const* out, const int64_t* sizes, const int8_t* dtypes,
                                int64_t count, double max_norm, float* d_norm, void* ws, int64_t ws_bytes,
                                void* stream) {
   if (count < 0) return GELIM_FAIL(GELIM_E_ARG, "clip: negative count");
-  if (ws_bytes < gelim_clip_workspace(count)) return GELIM_FAIL(GELIM_E_ARG, "clip: workspace too small");
+  if (ws_bytes < gelim_clip_workspace()) return GELIM_FAIL(GELIM_E_ARG, "clip: workspace too small");
   try {
     return gelim::clip(in, out, sizes, dtypes, count, max_norm, d_norm, (double*)ws, (hipStream_t)stream);
   } catch (const std::bad_alloc&) {

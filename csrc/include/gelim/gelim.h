@@ -310,7 +310,7 @@ int gelim_adapter_matmul_grad(const gelim_adapter_args* a, void* stream);
  * elements, GELIM_T_*); out[i] is in[i] (in place) or memory that no other
  * entry uses.  d_norm: one float on the device.  ws: gelim_clip_workspace
  * bytes, 8-byte aligned. */
-int64_t gelim_clip_workspace(int64_t count);
+int64_t gelim_clip_workspace(void);
 int gelim_clip_norm(const void* const* in, void* const* out, const int64_t* sizes, const int8_t* dtypes,
                     int64_t count, double max_norm, float* d_norm, void* ws, int64_t ws_bytes, void* stream);
 

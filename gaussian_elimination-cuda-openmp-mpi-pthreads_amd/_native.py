@@ -154,7 +154,7 @@ _PROTOS = {
     "gelim_adapter_workspace": (_i64, [C.c_char_p, _int]),
     "gelim_adapter_matmul": (_int, [C.c_char_p, _vp]),
     "gelim_adapter_matmul_grad": (_int, [C.c_char_p, _vp]),
-    "gelim_clip_workspace": (_i64, [_i64]),
+    "gelim_clip_workspace": (_i64, []),
     "gelim_clip_norm": (_int, [_vp, _vp, _vp, C.c_char_p, _i64, _dbl, _vp, _vp, _i64, _vp]),
     "gelim_init_random_block_f64": (None, [_vp, _i64, _i64, _i64, _i64, _i64, _u64]),
     "gelim_gpu_init_random_block": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _u64, _vp]),

@@ -91,7 +91,7 @@ def clip_global_norm(tensors: Sequence[torch.Tensor], max_norm: float,
         raise ValueError("clip_global_norm is not followed by forward-mode differentiation: it would drop the tangents")
     norm = torch.empty((), dtype=torch.float32, device=dev)
     lib = _native.lib()
-    ws = torch.empty(lib.gelim_clip_workspace(len(tensors)), dtype=torch.uint8, device=dev)
+    ws = torch.empty(lib.gelim_clip_workspace(), dtype=torch.uint8, device=dev)
 
     def call():
         _native.check(lib.gelim_clip_norm(src.buffer_info()[0], dst.buffer_info()[0], sizes.buffer_info()[0], types,
