@@ -16,7 +16,7 @@
 // tile of the large product has few adapters; the factors are laid out for the
 // matrix units once per call; U F_i is one pass over U; the accumulators of the
 // large product begin with s_i (U F_i) G_i.  8192 rows, bf16 8192 x 8192, rank 64:
-// 9 + 60 + 870 us, the large product at 1.26 PFLOP/s (a plain library product of
+// 8 + 58 + 840 to 875 us, the large product at 1.26 to 1.31 PFLOP/s (a plain library product of
 // that size: 1.27 to 1.56 by its layout).
 #include <hip/hip_runtime.h>
 
@@ -77,7 +77,7 @@ struct Mma<float> {
 
 // The blocks of the large product: kB rows and columns; lane l has row (column) l % kB and, of a step along the sum,
 // the kE values from (l / kB) kE on.  16-bit types as above: 32 x 32 x 16 instructions alone, from registers, reach 1670
-// TFLOP/s at the clock that the card holds under them, 16 x 16 x 32 1830.
+// TFLOP/s at the clock that the card holds under them, 16 x 16 x 32 1800 (profiles/adapter_counters.txt).
 template <class T>
 struct Block {
   static constexpr int kB = 16;
@@ -673,8 +673,8 @@ __device__ __forceinline__ void copy_tile(const Copy& c, int m, int slot, int ti
 
 // A workgroup's tiles of one matrix.  With more than a few adapters those that no row has are left out, as resident
 // adapters may be many more than a batch uses (500 of rank 16, 7 of them in use, 4096 x 4096: 149 -> 29 us for this
-// launch); beyond kScanRows rows looking for that would cost more than a tile's copy.  With more adapters than rows the
-// same look finds the layout's slot.
+// launch); beyond kScanRows rows, where looking for that would cost more than a tile's copy, all are laid out.  With
+// more adapters than rows the same look finds the layout's slot.
 constexpr int kScanAdapters = 8, kScanRows = 8192;
 template <class T>
 __device__ __forceinline__ void copy_tiles(const Copy& c, int part, const Rows& rows, bool packed) {
@@ -736,15 +736,16 @@ __global__ __launch_bounds__(kPrepare) void prepare_kernel(Prepare p) {
 }
 
 // low (place, rank) = U F_i, 32 places of one adapter by a workgroup, whose 8 waves cut the sum (16 waves were no
-// faster at any size, 10.2 instead of 8.3 us for 150 rows of K 2048, rank 64). F is laid out in fragments, ldf
-// values along the sum with zeros behind C.  Bound by reading U and, for every 32 rows, F_i: each wave keeps
-// several steps' loads in flight.  With few rows several workgroups cut the sum once more; the last of them to end
-// adds their parts, always in the same order. Measured, bf16: 2048 x 4096, rank 16, 8.8 us; 8192 x 8192, rank 64,
-// 60 us (U at 2.2 TB/s; more loads under way, waves side by side along a row, or the pieces of an adapter on one
-// XCD changed that by less than the noise). Also in fragments of 32 places and 8 ranks for the matrix units of the
-// large product, with 16-bit types as the sum of three values of the type, which hold all 24 bits of the fp32 sum.  fp16:
-// a row is first brought to below 2^14 by a power of two (`by`), as it may be beyond the type's range; small values of the
-// row are off by 2^-38 of its largest at most.
+// faster at any size, 10.2 instead of 8.3 us for 150 rows of K 2048, rank 64). F is laid out in fragments, ldf values
+// along the sum with zeros behind C.  Bound by what goes through the L2 caches, U once and F_i for every 32 rows
+// (8192 x 8192, rank 64: 480 MB at 8.3 TB/s, more than half of it F_i); each wave keeps several steps' loads in
+// flight.  With few rows several workgroups cut the sum once more; the last of them to end adds their parts, always
+// in the same order. Measured, bf16: 2048 x 4096, rank 16, 8.8 us; 8192 x 8192, rank 64, 58 us (more loads under way,
+// waves side by side along a row, or the pieces of an adapter on one XCD changed that by less than the noise). Also
+// in fragments of 32 places and 8 ranks for the matrix units of the large product, with 16-bit types as the sum of
+// three values of the type, which hold all 24 bits of the fp32 sum.  fp16: a row is first brought to below 2^14 by a
+// power of two (`by`), as it may be beyond the type's range; small values of the row are off by 2^-38 of its largest
+// at most.
 struct Low {
   const void *U, *F;
   int64_t ldu;
@@ -948,10 +949,11 @@ __global__ __launch_bounds__(kLowWaves * 64) void low_kernel(LowPair both) {
 }
 
 // The large product: (U W) of BT places x BN columns, sum in steps of 128 bytes.  Bound by the matrix units at the
-// clock that the card holds under them, 1.6 to 1.85 GHz, and by the waits at the barriers (8192^3 in bf16: 73% of the
-// cycles busy), so by what a product costs in power as well: 16 x 16 x 32 instructions instead of 32 x 32 x 16 took 876
-// instead of 909 us there.  Against 8 waves of 128 x 64 on 256 x 256, 4 waves of 128 x 128 took 26% longer, 256 x 128
-// tiles alone 11%, and half steps with four or five tiles in LDS 3 to 6%.
+// clock that the card holds under them, 1.6 to 1.85 GHz, and by the waits at the barriers (8192^3 in bf16: the units
+// busy in 65% of the cycles at 1.57 GHz, fp32 4096^3 85% at 2.08, both under the profiler), so by what a product
+// costs in power as well: 16 x 16 x 32 instructions instead of 32 x 32 x 16 took 876 instead of 909 us there.
+// Against 8 waves of 128 x 64 on 256 x 256, 4 waves of 128 x 128 took 26% longer, 256 x 128 tiles alone 11%, and half
+// steps with four or five tiles in LDS 3 to 6%.
 struct Big {
   const void *U, *W, *G;
   int64_t ldu, ldw;
@@ -1175,9 +1177,10 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
 #pragma unroll
       for (int t = 0; t < TT; ++t)
         if (mine[t] >= 0 && mine[t] < a.rows.n) slot[t] = packed_slot(mine[t], a.order.start[mine[t]]);
-    // The accumulators begin with s_i (U F_i) G_i, while the first tiles load (SPLIT: each part of the sum with
-    // some of the adapters and ranks).  U F_i comes as three values of the type (fp32: itself); the loads of kSets steps are under way at a time.  A row without this adapter loads its own
-    // garbage, which reaches that row's accumulators alone, and these are set afterwards.
+    // The accumulators begin with s_i (U F_i) G_i, while the first tiles load (SPLIT: each part of the sum with some
+    // of the adapters and ranks).  U F_i comes as three values of the type (fp32: itself); the loads of kSets steps
+    // are under way at a time.  A row without this adapter loads its own garbage, which reaches that row's
+    // accumulators alone, and these are set afterwards.
     auto has = [&](int t) { return mine[t] >= 0 && mine[t] < a.rows.n; };
     auto place = [&](int t) { return (int64_t)min(t0 + wt + t * kB + lb, a.rows.T - 1); };
     // the fragments that the low-rank pass and the first launch wrote, of 32 places or columns and 8 ranks.  Such a
@@ -1366,7 +1369,7 @@ __global__ __launch_bounds__(WT * WN * 64) void big_kernel(Big a) {
   }
 }
 
-// The factors' gradients (4096 rows, 4096 + 4096 columns, rank 16, bf16: 20.6 us, U at 3.3 TB/s): sum over the
+// The factors' gradients (4096 rows, 4096 + 4096 columns, rank 16, bf16: 22 us, U at 3.0 TB/s): sum over the
 // places of an adapter of U_t^T V_t, V = S or D, in pieces of `size` places (32 to kGradRows: with few rows smaller
 // ones, for enough workgroups, but not so small that the parts, a rank's 4 bytes a column each, outweigh U's).  A
 // workgroup takes 64 kE columns of U, a wave 16 kE, whose rows it turns in registers.  V is turned on its way to
@@ -1533,8 +1536,9 @@ __global__ __launch_bounds__(256) void outer_kernel(OuterPair both) {
   }
 }
 
-// Last the sums of the parts, times s_i, in the factor's layout, and zeros for adapters without rows: 64 columns of one adapter by a workgroup, whose four waves share
-// the pieces of 4 ranks or, where the adapters have few pieces, take 4 ranks each.
+// Last the sums of the parts, times s_i, in the factor's layout, and zeros for adapters without rows: 64 columns of
+// one adapter by a workgroup, whose four waves share the pieces of 4 ranks or, where the adapters have few pieces,
+// take 4 ranks each.
 struct Sum {
   const float* part;
   void* out;
